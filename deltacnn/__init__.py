@@ -5,8 +5,9 @@ import sys
 
 import deltacnn_b200
 from deltacnn_b200 import *  # noqa: F401,F403
-from deltacnn_b200 import cuda_kernels, filter_conversion, sparse_layers
+from deltacnn_b200 import channel_ops, cuda_kernels, filter_conversion, sparse_layers
 
 sys.modules[__name__ + ".sparse_layers"] = sparse_layers
+sys.modules[__name__ + ".channel_ops"] = channel_ops
 sys.modules[__name__ + ".cuda_kernels"] = cuda_kernels
 sys.modules[__name__ + ".filter_conversion"] = filter_conversion

@@ -9,7 +9,7 @@ import os
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdeltacnn_b200.so")
 
-DC_F32, DC_F16 = 0, 1
+DC_F32, DC_F16, DC_BF16 = 0, 1, 2
 DC_FILTER_HWIO, DC_FILTER_UMMA = 0, 1
 
 c_int, c_i64, c_float, c_void_p, c_size_t = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p, ctypes.c_size_t
@@ -78,6 +78,16 @@ _SIGNATURES = {
     "dc_linear_delta": (c_int, [_P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "dc_heatmap_argmax": (c_int, [_P, _P, _P, c_int, c_int, c_int, c_int, c_int, _P]),
     "dc_centernet_decode": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, c_float, c_int, c_int, _P]),
+    "dc_layer_norm": (c_int, [_P, _P, _P, _P, _P, _P, c_i64, c_int, c_int, c_int, c_float, _P]),
+    "dc_layer_norm_backward_workspace_bytes": (c_size_t, [c_i64, c_int, c_int]),
+    "dc_layer_norm_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_i64, c_int, c_int, c_int, _P, c_size_t, _P]),
+    "dc_layer_norm_delta": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_i64, c_int, c_int, c_int, c_float, c_float, _P]),
+    "dc_mx4_data_bytes": (c_size_t, [c_i64, c_i64]),
+    "dc_mx4_scale_bytes": (c_size_t, [c_i64, c_i64]),
+    "dc_mx4_colsum_workspace_bytes": (c_size_t, [c_i64, c_i64]),
+    "dc_mx4_quantize": (c_int, [_P, _P, _P, _P, _P, _P, c_i64, c_i64, c_int, c_int, _P, c_size_t, _P]),
+    "dc_mx4_dequantize": (c_int, [_P, _P, _P, c_i64, c_i64, c_int, _P]),
+    "dc_mx4_matmul": (c_int, [_P, _P, _P, _P, _P, _P, c_i64, c_i64, c_i64, c_int, c_int, _P]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
 

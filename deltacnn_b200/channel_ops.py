@@ -1,0 +1,359 @@
+"""Operators on the channel vectors of dense features: layer norm (forward, backward, delta form) and the 4-bit microscaled
+format MXFP4 (quantisation, products, a linear layer with gradients).
+
+A tensor is seen as rows x channels: a 4-D tensor is a feature map (N, C, H, W) in channels-last memory, one row per pixel;
+any other tensor is (..., C), contiguous, one row per token. Types are float32, float16 and bfloat16 (the delta form: those of
+the delta path, float32 and float16). As everywhere in this package there is no CPU path, a wrong device, type or
+memory format raises before a launch, and launches go to torch's current stream on the tensor's device; an argument is never
+copied to make it fit, except an incoming gradient, whose layout the caller cannot choose.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from ._lib import lib, check
+from .cuda_kernels import _check_feature, _check_like, _check_mask
+
+_CODES = {torch.float32: _lib.DC_F32, torch.float16: _lib.DC_F16, torch.bfloat16: _lib.DC_BF16}
+
+
+class _on:
+    """Makes a tensor's device the current one for the launch (nothing to do on the usual path)."""
+    __slots__ = ("guard",)
+
+    def __init__(self, t):
+        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _fail(op, text):
+    raise RuntimeError(f"deltacnn_b200.{op}: {text}")
+
+
+def _code(t, op, name):
+    code = _CODES.get(t.dtype)
+    if code is None:
+        _fail(op, f"{name} has unsupported dtype {t.dtype} (float32, float16 and bfloat16 only)")
+    return code
+
+
+def _rows(x, op, name="x"):
+    """(rows, channels) of a feature map or token tensor."""
+    if not x.is_cuda:
+        _fail(op, f"{name} must be a CUDA tensor (there is no CPU path)")
+    if x.dim() == 4:
+        if not x.is_contiguous(memory_format=torch.channels_last):
+            _fail(op, f"{name} is 4-D and must be a channels_last contiguous feature map (N, C, H, W)")
+        n, c, h, w = x.shape
+        rows = n * h * w
+    else:
+        if x.dim() == 0 or not x.is_contiguous():
+            _fail(op, f"{name} must be a contiguous (..., channels) tensor or a 4-D channels_last feature map")
+        c = x.shape[-1]
+        rows = x.numel() // c if c > 0 else 0
+    if c == 0:
+        _fail(op, f"{name} has no channels")
+    return rows, c
+
+
+def _like_rows(g, x):
+    """An incoming gradient in x's layout."""
+    if x.dim() == 4:
+        return g.contiguous(memory_format=torch.channels_last)
+    return g.contiguous()
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+# ---- layer norm ------------------------------------------------------------------------------------------------
+
+def _ln_params(x, c, code, weight, bias, op):
+    """The weight's dtype code; weight and bias are (C,) of x's type or float32, of one type."""
+    wcode = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.dim() != 1 or t.shape[0] != c or not t.is_contiguous() or t.device != x.device or (t.dtype != x.dtype and t.dtype != torch.float32):
+            _fail(op, f"{name} must be a contiguous ({c},) tensor of type {x.dtype} or float32 on {x.device}")
+        if wcode is not None and wcode != _CODES[t.dtype]:
+            _fail(op, "weight and bias must have the same type")
+        wcode = _CODES[t.dtype]
+    return code if wcode is None else wcode
+
+
+def _ln_forward(x, weight, bias, eps, keep):
+    op = "layer_norm"
+    rows, c = _rows(x, op)
+    code = _code(x, op, "x")
+    wcode = _ln_params(x, c, code, weight, bias, op)
+    y = torch.empty_like(x)
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+    mean, rstd = (stats.data_ptr(), stats.data_ptr() + 4 * rows) if keep and rows > 0 else (None, None)
+    if rows > 0:
+        with _on(x) as stream:
+            check(lib.dc_layer_norm(x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, rstd, rows, c, code, wcode, eps, stream), op)
+    return y, stats
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, stats = _ln_forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, stats)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, weight, stats = ctx.saved_tensors
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        rows, c = _rows(x, "layer_norm")
+        dy = _like_rows(dy, x)
+        wtype = weight.dtype if weight is not None else ctx.bias_dtype if ctx.bias_dtype is not None else x.dtype
+        dx = torch.empty_like(x) if need_x else None
+        dw = torch.empty(c, dtype=wtype, device=x.device) if need_w else None
+        db = torch.empty(c, dtype=wtype, device=x.device) if need_b else None
+        code = _CODES[x.dtype]
+        with _on(x) as stream:
+            ws, nbytes = None, 0
+            if need_w or need_b:
+                nbytes = lib.dc_layer_norm_backward_workspace_bytes(rows, c, code)
+                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+            mean = stats.data_ptr()
+            check(lib.dc_layer_norm_backward(_ptr(dy), _ptr(x), _ptr(weight), mean, mean + 4 * rows if rows > 0 else None, _ptr(dx), _ptr(dw), _ptr(db),
+                                             rows, c, code, _CODES[wtype], _ptr(ws), nbytes, stream), "layer_norm_backward")
+        return dx, dw, db, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+    """``(x - mean) / sqrt(var + eps) * weight + bias`` over the channels, statistics and arithmetic in float32. ``weight`` and
+    ``bias``: (C,) in x's type or float32, or None. Differentiable in x, weight and bias (once); the sums over rows are added
+    in a fixed order, so equal inputs give equal bits. No reference counterpart."""
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _ln_forward(x, weight, bias, eps, False)[0]
+
+
+def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, threshold=0.0, eps=1e-5, out=None, out_mask=None):
+    """Layer norm over the channels of a (delta, mask) pair with its caches (no gradient): on masked pixels
+    ``prev_in += delta`` and ``e = layer_norm(prev_in) - prev_out``; where any ``|e| > threshold`` the pixel stays in the mask,
+    ``out = e`` and ``prev_out += e``; elsewhere the out-mask is 0 and ``out`` and ``prev_out`` keep what they hold.
+    ``prev_in``: the accumulated input, ``prev_out``: the sum of what was handed on, both updated in place. ``out`` may be
+    ``delta`` and ``out_mask`` may be ``mask``; new tensors where None. Returns (out, out_mask). No reference counterpart."""
+    op = "layer_norm_delta"
+    _check_feature(delta, "delta")
+    if delta.dtype not in (torch.float32, torch.float16):
+        _fail(op, f"unsupported dtype {delta.dtype} (float32 and float16 only)")
+    _check_mask(mask, delta, "mask")
+    _check_like(prev_in, delta, "prev_in")
+    _check_like(prev_out, delta, "prev_out")
+    n, c, h, w = delta.shape
+    if c == 0:
+        _fail(op, "delta has no channels")
+    code = _CODES[delta.dtype]
+    wcode = _ln_params(delta, c, code, weight, bias, op)
+    if out is None:
+        out = torch.empty_like(delta)
+    else:
+        _check_like(out, delta, "out")
+    if out_mask is None:
+        out_mask = torch.empty_like(mask)
+    else:
+        _check_mask(out_mask, delta, "out_mask")
+    for t, name in ((mask, "mask"), (out_mask, "out_mask")):
+        if t.device != delta.device or not t.is_contiguous():
+            _fail(op, f"{name} must be contiguous and on {delta.device}")
+    with _on(delta) as stream:
+        check(lib.dc_layer_norm_delta(delta.data_ptr(), mask.data_ptr(), prev_in.data_ptr(), prev_out.data_ptr(), _ptr(weight), _ptr(bias),
+                                      out.data_ptr(), out_mask.data_ptr(), n * h * w, c, code, wcode, float(threshold), eps, stream), op)
+    return out, out_mask
+
+
+# ---- MXFP4 -----------------------------------------------------------------------------------------------------
+
+def _mx4_shapes(rows, cols):
+    nb = (cols + 31) // 32
+    return (rows, 16 * nb), ((rows + 127) // 128, (nb + 3) // 4, 32, 4, 4)
+
+
+class MX4Tensor:
+    """A packed rows x cols matrix. ``data``: uint8 (rows, 16 * nb), nb = ceil(cols / 32), two e2m1 codes a byte, the even
+    column in the low half, zeros behind the last column. ``scales``: uint8 (ceil(rows / 128), ceil(nb / 4), 32, 4, 4), block b of
+    row r at [r // 128, b // 4, r % 32, r % 128 // 32, b % 4] (what the tensor core reads); its entries for rows behind
+    the last one are never looked at, those for blocks behind the last one must not be 255."""
+    __slots__ = ("data", "scales", "shape")
+
+    def __init__(self, data, scales, shape):
+        rows, cols = shape
+        want_data, want_scales = _mx4_shapes(rows, cols)
+        if cols <= 0 or data.dtype != torch.uint8 or scales.dtype != torch.uint8 or tuple(data.shape) != want_data or tuple(scales.shape) != want_scales:
+            raise RuntimeError(f"deltacnn_b200.MX4Tensor: a {rows} x {cols} matrix needs uint8 data {want_data} and scales {want_scales}")
+        if not data.is_contiguous() or not scales.is_contiguous() or data.device != scales.device:
+            raise RuntimeError("deltacnn_b200.MX4Tensor: data and scales must be contiguous and on one device")
+        self.data, self.scales, self.shape = data, scales, (rows, cols)
+
+    def dequantize(self, dtype=torch.float32):
+        return mx4_dequantize(self, dtype)
+
+
+def _mx4_empty(rows, cols, device):
+    data, scales = _mx4_shapes(rows, cols)
+    q = MX4Tensor.__new__(MX4Tensor)
+    q.data, q.scales, q.shape = torch.empty(data, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device), (rows, cols)
+    return q
+
+
+def _quantize(x, rows, cols, along_rows, along_cols, colsum=None):
+    """(packed x or None, packed x^T or None); ``colsum``: a (cols,) tensor that receives the column sums. An empty x has no
+    packed transpose (a matrix without columns)."""
+    code = _code(x, "mx4_quantize", "x")
+    q = _mx4_empty(rows, cols, x.device) if along_rows else None
+    qt = _mx4_empty(cols, rows, x.device) if along_cols and rows > 0 else None
+    ws, nbytes = None, 0
+    if colsum is not None:
+        nbytes = lib.dc_mx4_colsum_workspace_bytes(rows, cols)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    if rows > 0 or colsum is not None:
+        with _on(x) as stream:
+            check(lib.dc_mx4_quantize(x.data_ptr(), q and q.data.data_ptr(), q and q.scales.data_ptr(), qt and qt.data.data_ptr(),
+                                      qt and qt.scales.data_ptr(), _ptr(colsum), rows, cols, code, 0 if colsum is None else _CODES[colsum.dtype],
+                                      _ptr(ws), nbytes, stream), "mx4_quantize")
+    return q, qt
+
+
+def mx4_quantize(x):
+    """x packed along its channels: an ``MX4Tensor`` of rows x channels. Blocks of 32 values share the scale
+    2^(floor(log2 max|v|) - 2); values are rounded to the nearest of +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} times the scale (ties to
+    even, saturating); a block with an infinity or a NaN becomes NaN. No gradient, no reference counterpart."""
+    rows, cols = _rows(x, "mx4_quantize")
+    return _quantize(x, rows, cols, True, False)[0]
+
+
+def mx4_quantize_both(x):
+    """(packed x, packed x^T) from one read of x; the second is cols x rows with blocks along x's columns (what the products
+    of a backward pass contract over)."""
+    rows, cols = _rows(x, "mx4_quantize_both")
+    if rows == 0:
+        _fail("mx4_quantize_both", "x has no rows")
+    return _quantize(x, rows, cols, True, True)
+
+
+def mx4_dequantize(q, dtype=torch.float32):
+    """The values that an ``MX4Tensor`` stands for, as a (rows, cols) tensor."""
+    op = "mx4_dequantize"
+    rows, cols = q.shape
+    if dtype not in _CODES:
+        _fail(op, f"unsupported dtype {dtype} (float32, float16 and bfloat16 only)")
+    if not q.data.is_cuda:
+        _fail(op, "data must be a CUDA tensor (there is no CPU path)")
+    out = torch.empty((rows, cols), dtype=dtype, device=q.data.device)
+    if rows > 0:
+        with _on(q.data) as stream:
+            check(lib.dc_mx4_dequantize(q.data.data_ptr(), q.scales.data_ptr(), out.data_ptr(), rows, cols, _CODES[dtype], stream), op)
+    return out
+
+
+def mx4_matmul(a, b, bias=None, dtype=torch.float16, out=None):
+    """``a @ b.T + bias`` of two packed matrices (m x k and n x k, a weight in nn.Linear's layout): products and sums in float32,
+    one rounding to ``dtype``. ``bias``: (n,) or None. ``out``: a contiguous (m, n) tensor to write to."""
+    op = "mx4_matmul"
+    (m, k), (n, k2) = a.shape, b.shape
+    if k != k2:
+        _fail(op, f"the matrices have {k} and {k2} columns")
+    if dtype not in _CODES:
+        _fail(op, f"unsupported dtype {dtype} (float32, float16 and bfloat16 only)")
+    device = a.data.device
+    if not a.data.is_cuda or b.data.device != device:
+        _fail(op, "both matrices must be on one CUDA device (there is no CPU path)")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous() or bias.device != device or bias.dtype not in _CODES):
+        _fail(op, f"bias must be a contiguous ({n},) tensor on {device}")
+    if out is None:
+        out = torch.empty((m, n), dtype=dtype, device=device)
+    elif out.dtype != dtype or tuple(out.shape) != (m, n) or not out.is_contiguous() or out.device != device:
+        _fail(op, f"out must be a contiguous ({m}, {n}) tensor of type {dtype} on {device}")
+    if m > 0 and n > 0:
+        with _on(out) as stream:
+            check(lib.dc_mx4_matmul(a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(), _ptr(bias), out.data_ptr(), m, n, k,
+                                    0 if bias is None else _CODES[bias.dtype], _CODES[dtype], stream), op)
+    return out
+
+
+def _unrows(out, x):
+    """A (rows, n) result in the shape of x with n channels."""
+    if x.dim() == 4:
+        n, _, h, w = x.shape
+        return out.view(n, h, w, out.shape[1]).permute(0, 3, 1, 2)
+    return out.view(*x.shape[:-1], out.shape[1]) if x.dim() != 2 else out
+
+
+class _MX4Linear(torch.autograd.Function):
+    """y = Q(x) Q(w)^T + b; dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, db = sum dy: every operand is rounded along the axis that
+    its product sums over, the rounding's own gradient is taken as 1. What is kept for the backward pass is 4-bit."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        rows, cols = _rows(x, "mx4_linear")
+        need_x, need_w, _ = ctx.needs_input_grad
+        xq, xt = _quantize(x, rows, cols, True, need_w)
+        wq, wt = _quantize(weight, weight.shape[0], cols, True, need_x)
+        ctx.xt, ctx.wt = xt, wt
+        ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
+        ctx.sizes = (rows, cols, weight.shape[0])
+        return _unrows(mx4_matmul(xq, wq, bias, x.dtype), x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w, need_b = ctx.needs_input_grad
+        rows, cols, outs = ctx.sizes
+        dy = _like_rows(dy, dy)
+        db = torch.empty(outs, dtype=ctx.dtypes[2], device=dy.device) if need_b else None
+        if rows == 0:
+            dx = dy.new_zeros(ctx.x_shape, dtype=ctx.dtypes[0]) if need_x else None
+            return dx, dy.new_zeros((outs, cols), dtype=ctx.dtypes[1]) if need_w else None, None if db is None else db.zero_()
+        dq, dt = _quantize(dy, rows, outs, need_x, need_w, db)
+        dx = None
+        if need_x:
+            dx = mx4_matmul(dq, ctx.wt, None, ctx.dtypes[0])
+            if len(ctx.x_shape) == 4:
+                n, _, h, w = ctx.x_shape
+                dx = dx.view(n, h, w, cols).permute(0, 3, 1, 2)
+            else:
+                dx = dx.view(ctx.x_shape)
+        return dx, mx4_matmul(dt, ctx.xt, None, ctx.dtypes[1]) if need_w else None, db
+
+
+def mx4_linear(x, weight, bias=None):
+    """Linear layer over the channels in MXFP4, result in x's type. ``weight``: an ``MX4Tensor`` of outputs x inputs (packed once,
+    inference only), or a (outputs, inputs) tensor, which is packed in the call and, like x and ``bias``, gets a gradient from
+    4-bit products (dx and dw have the types of x and weight; differentiable once)."""
+    op = "mx4_linear"
+    rows, cols = _rows(x, op)
+    _code(x, op, "x")
+    packed = isinstance(weight, MX4Tensor)
+    outs, k = weight.shape
+    if k != cols:
+        _fail(op, f"x has {cols} channels, the weight {k} columns")
+    grad = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not packed and weight.requires_grad))
+    if packed:
+        if grad:
+            _fail(op, "a packed weight is for inference: pass the unpacked weight to train, or call under torch.no_grad()")
+        return _unrows(mx4_matmul(_quantize(x, rows, cols, True, False)[0], weight, bias, x.dtype), x)
+    if not weight.is_contiguous() or weight.device != x.device or weight.dtype not in _CODES or outs == 0:
+        _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != outs or not bias.is_contiguous() or bias.device != x.device or bias.dtype not in _CODES):
+        _fail(op, f"bias must be a contiguous ({outs},) tensor on {x.device}")
+    if grad:
+        return _MX4Linear.apply(x, weight, bias)
+    return _unrows(mx4_matmul(_quantize(x, rows, cols, True, False)[0], _quantize(weight, outs, cols, True, False)[0], bias, x.dtype), x)

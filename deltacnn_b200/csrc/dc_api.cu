@@ -49,6 +49,7 @@ int umma_error_code();
 int stem_umma_error_code();
 int irb_error_code();
 int halo_error_code();
+int mx4_error_code();
 int conv_stem_umma(const dc_conv_desc* d, const void* in, const int32_t* mi, const void* filt, const void* bias, void* out,
                    int32_t* mo, const dc_epilogue* ep, cudaStream_t st);
 int conv_thin(const dc_conv_desc* d, const void* in, const int32_t* mi, const void* filt, const void* bias, void* out,
@@ -86,7 +87,7 @@ const char* dc_status_string(int status) {
         case DC_ERR_UNSUPPORTED: return "unsupported kernel size, stride, groups or mode";
         case DC_ERR_ALIGNMENT: return "pointer not aligned for the vector width in use";
         case DC_ERR_SHAPE: return "inconsistent or non-positive sizes";
-        case DC_ERR_DTYPE: return "dtype must be float32 (0) or float16 (1)";
+        case DC_ERR_DTYPE: return "dtype must be float32 (0) or float16 (1) (or bfloat16 (2) where the entry point takes it)";
         case DC_ERR_LAUNCH: return "CUDA launch failed";
         case DC_ERR_WORKSPACE: return "workspace too small";
         default: return "unknown status";
@@ -101,7 +102,9 @@ int dc_umma_error(void) {
     const int b = stem_umma_error_code();
     if (b != 0) return b;
     const int c = irb_error_code();
-    return c != 0 ? c : halo_error_code();
+    if (c != 0) return c;
+    const int d = halo_error_code();
+    return d != 0 ? d : mx4_error_code();
 }
 
 int dc_conv2d_ws(const dc_conv_desc* desc, const void* in, const int32_t* mask_in, const void* filter, int32_t filter_layout,

@@ -1,0 +1,307 @@
+// MXFP4 quantisation (blocks along the rows, along the columns, or both from one read) and dequantisation.
+//
+// Bound: memory. x is read once; a value leaves as half a byte plus 1/32 byte of scale per image.
+//
+// Rows only (k_mx4_rows): a lane owns eight neighbouring values (one or two 16-byte reads), four lanes a block: the block's
+// largest magnitude takes two shuffles, the codes of a lane are one 4-byte store, the scales of four blocks one more.
+//
+// Both images (k_mx4_tile): a CTA owns 128 x 128 values, which is exactly one 512-byte scale tile of either image. The rows
+// are encoded on the way from global to shared memory; the columns are then read from shared memory, two neighbouring
+// columns of a 32-row block per thread. Rows 32 apart would meet in the same banks, so every 32 rows are skewed by 16 values:
+// a warp reads 8 column pairs x 4 blocks without a conflict and writes 64 contiguous bytes per column. The column sums (the
+// bias gradient of a linear layer, whose dy this kernel reads anyway) fall out of the second phase.
+#include "dc_mx4.cuh"
+
+namespace dc {
+
+int col_reduce(const float* partial, int n, int c, int64_t pitch, void* o0, void* o1, int dtype, cudaStream_t st);   // dc_norm.cu
+
+// Eight values of a row starting at column col (cols in all); zeros behind the end.
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(float (&v)[8], const T* row, int64_t col, int64_t cols) {
+    if constexpr (VEC) {
+        constexpr int N = 8 / VecTraits<T>::kVec;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            Pack<T, VecTraits<T>::kVec> p;
+            if (col + k * VecTraits<T>::kVec < cols) p.load(row + col + k * VecTraits<T>::kVec);
+            else p.zero();
+#pragma unroll
+            for (int i = 0; i < VecTraits<T>::kVec; ++i) v[k * VecTraits<T>::kVec + i] = p.get(i);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? to_f<T>(row[col + i]) : 0.f;
+    }
+}
+
+__device__ __forceinline__ uint32_t amax8_bits(const float (&v)[8]) {
+    uint32_t m = 0;      // as integers: a NaN is above every number, so it is not lost
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+}
+__device__ __forceinline__ uint32_t encode_scaled(const float (&v)[8], uint32_t s) {
+    if (s == 255u) return 0u;
+    const float f = mx4_factor(s);
+    float u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = v[i] * f;
+    return mx4_encode8(u);
+}
+
+constexpr int kMxChunk = 256;          // values of a row that a warp takes at once (eight blocks)
+constexpr int kMxAhead = 4;            // chunks of a row whose reads a warp has in flight
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_mx4_rows(const T* __restrict__ x, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int64_t rows,
+                                                  int64_t cols, int segments) {
+    grid_dep_launch();
+    grid_dep_wait();
+    const int lane = threadIdx.x & 31;
+    const int64_t nb = mx4_blocks(cols), tiles = mx4_scale_tiles(cols);
+    const int64_t items = rows * segments, nwarps = (int64_t)gridDim.x * 8;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += nwarps) {
+        const int64_t r = it / segments;
+        const int64_t c0 = (it - r * segments) * (kMxChunk * kMxAhead) + lane * 8;
+        const T* row = x + r * cols;
+        float v[kMxAhead][8];
+#pragma unroll
+        for (int a = 0; a < kMxAhead; ++a) load8<T, VEC>(v[a], row, c0 + a * kMxChunk, cols);
+#pragma unroll
+        for (int a = 0; a < kMxAhead; ++a) {
+            const int64_t col = c0 + a * kMxChunk, b = col >> 5;
+            uint32_t m = amax8_bits(v[a]);
+            m = max(m, __shfl_xor_sync(DC_FULL, m, 1));
+            m = max(m, __shfl_xor_sync(DC_FULL, m, 2));
+            const uint32_t s = mx4_scale_byte(m);
+            if (b < nb) *reinterpret_cast<uint32_t*>(data + r * nb * 16 + (col >> 1)) = encode_scaled(v[a], s);
+            // the scale bytes of four blocks as one word, written by the first lane of every sixteen
+            uint32_t word = s << (8 * ((lane >> 2) & 3));
+            word |= __shfl_xor_sync(DC_FULL, word, 4);
+            word |= __shfl_xor_sync(DC_FULL, word, 8);
+            if ((lane & 15) == 0 && (b >> 2) < tiles) *reinterpret_cast<uint32_t*>(scales + mx4_scale_word(r, b >> 2, tiles)) = word;
+        }
+    }
+}
+
+constexpr int kTile = 128;             // rows and columns of a tile
+template <typename T> __host__ __device__ constexpr int tile_bytes() { return (kTile * kTile + 3 * 16) * (int)sizeof(T); }
+template <typename T> __device__ __forceinline__ int tile_at(int r, int c) { return (r * kTile + (r >> 5) * 16 + c) * (int)sizeof(T); }
+
+struct MxTileParams {
+    const void* x;
+    uint8_t *data, *scales, *data_t, *scales_t;      // either pair may be NULL
+    float* colsum;                                   // [ceil(rows / 128)][cols], or NULL
+    int64_t rows, cols;
+};
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_mx4_tile(MxTileParams p) {
+    extern __shared__ __align__(16) uint8_t tile[];
+    __shared__ float sums[4][kTile];
+    grid_dep_launch();
+    grid_dep_wait();
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t r0 = (int64_t)blockIdx.y * kTile, c0 = (int64_t)blockIdx.x * kTile;
+    const int64_t nb = mx4_blocks(p.cols), tiles = mx4_scale_tiles(p.cols);
+    // phase 1: sixteen lanes a row (eight values each), so a warp takes two rows at a time
+    const int lr = warp * 2 + (lane >> 4), lc = (lane & 15) * 8;
+#pragma unroll 4
+    for (int q = 0; q < kTile / 16; ++q) {
+        const int tr = q * 16 + lr;
+        const int64_t r = r0 + tr;
+        float v[8];
+        if (r < p.rows) load8<T, VEC>(v, (const T*)p.x + r * p.cols, c0 + lc, p.cols);
+        else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        }
+        T* at = reinterpret_cast<T*>(tile + tile_at<T>(tr, lc));
+#pragma unroll
+        for (int k = 0; k < 8 / VecTraits<T>::kVec; ++k) {
+            Pack<T, VecTraits<T>::kVec> o;
+#pragma unroll
+            for (int i = 0; i < VecTraits<T>::kVec; ++i) o.set(i, v[k * VecTraits<T>::kVec + i]);
+            o.store(at + k * VecTraits<T>::kVec);
+        }
+        if (p.data != nullptr) {
+            uint32_t m = amax8_bits(v);
+            m = max(m, __shfl_xor_sync(DC_FULL, m, 1));
+            m = max(m, __shfl_xor_sync(DC_FULL, m, 2));
+            const uint32_t s = mx4_scale_byte(m);
+            if (r < p.rows && (c0 + lc) >> 5 < nb) *reinterpret_cast<uint32_t*>(p.data + r * nb * 16 + ((c0 + lc) >> 1)) = encode_scaled(v, s);
+            uint32_t word = s << (8 * ((lane >> 2) & 3));
+            word |= __shfl_xor_sync(DC_FULL, word, 4);
+            word |= __shfl_xor_sync(DC_FULL, word, 8);
+            if ((lane & 15) == 0 && r < p.rows) *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_word(r, blockIdx.x, tiles)) = word;
+        }
+    }
+    __syncthreads();
+    // phase 2: a thread takes two columns of a 32-row block; a warp 8 column pairs x the 4 blocks
+    const int pair = warp * 8 + (lane & 7), blk = lane >> 3;
+    const int64_t nbt = mx4_blocks(p.rows), tiles_t = mx4_scale_tiles(p.rows);
+    float u[2][8];
+    float sum[2] = {0.f, 0.f};
+    uint32_t m[2] = {0u, 0u};
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+        const T* at = reinterpret_cast<const T*>(tile + tile_at<T>(blk * 32 + i, pair * 2));
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float f = to_f<T>(at[k]);
+            sum[k] += f;
+            m[k] = max(m[k], __float_as_uint(f) & 0x7fffffffu);
+        }
+    }
+    if (p.data_t != nullptr) {
+        uint32_t code[2][4];
+        const uint32_t s[2] = {mx4_scale_byte(m[0]), mx4_scale_byte(m[1])};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const T* at = reinterpret_cast<const T*>(tile + tile_at<T>(blk * 32 + j * 8 + i, pair * 2));
+                u[0][i] = to_f<T>(at[0]);
+                u[1][i] = to_f<T>(at[1]);
+            }
+            code[0][j] = encode_scaled(u[0], s[0]);
+            code[1][j] = encode_scaled(u[1], s[1]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const int64_t c = c0 + pair * 2 + k, b = (int64_t)blockIdx.y * 4 + blk;
+            if (c < p.cols) {
+                if (b < nbt) *reinterpret_cast<uint4*>(p.data_t + (c * nbt + b) * 16) = make_uint4(code[k][0], code[k][1], code[k][2], code[k][3]);
+                p.scales_t[mx4_scale_word(c, blockIdx.y, tiles_t) + blk] = (uint8_t)s[k];
+            }
+        }
+    }
+    if (p.colsum != nullptr) {
+        sums[blk][pair * 2] = sum[0];
+        sums[blk][pair * 2 + 1] = sum[1];
+        __syncthreads();
+        if (threadIdx.x < kTile && c0 + threadIdx.x < p.cols)
+            p.colsum[blockIdx.y * p.cols + c0 + threadIdx.x] =
+                (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
+    }
+}
+
+// A lane takes eight codes and their scale byte; 16 (or 32) bytes leave.
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, T* __restrict__ out,
+                                                        int64_t rows, int64_t cols, int packs) {
+    grid_dep_launch();
+    grid_dep_wait();
+    const int64_t nb = mx4_blocks(cols), tiles = mx4_scale_tiles(cols);
+    const int64_t n = rows * packs;
+    for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < n; it += (int64_t)gridDim.x * 256) {
+        const int64_t r = it / packs, c = (it - r * packs) * 8, b = c >> 5;
+        const uint32_t code = *reinterpret_cast<const uint32_t*>(data + r * nb * 16 + (c >> 1));
+        const float s = mx4_scale_value(scales[mx4_scale_word(r, b >> 2, tiles) + (b & 3)]);
+        T* o = out + r * cols + c;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = mx4_decode(code >> (4 * i)) * s;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int k = 0; k < 8 / VecTraits<T>::kVec; ++k) {
+                Pack<T, VecTraits<T>::kVec> q;
+#pragma unroll
+                for (int i = 0; i < VecTraits<T>::kVec; ++i) q.set(i, v[k * VecTraits<T>::kVec + i]);
+                if (c + k * VecTraits<T>::kVec < cols) q.store(o + k * VecTraits<T>::kVec);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c + i < cols) o[i] = from_f<T>(v[i]);
+        }
+    }
+}
+
+template <typename T>
+static int quantize_t(const void* x, void* data, void* scales, void* data_t, void* scales_t, float* colsum, int64_t rows, int64_t cols, cudaStream_t st) {
+    const bool vec = aligned16(x) && cols % VecTraits<T>::kVec == 0;
+    if (data_t == nullptr && colsum == nullptr) {
+        const int segments = (int)divup64(mx4_scale_tiles(cols) * 128, kMxChunk * kMxAhead);
+        int64_t ctas = divup64(rows * segments, 8);
+        const int64_t cap = (int64_t)sm_count() * 8;
+        if (ctas > cap) ctas = cap;
+        if (vec) return launch_pdl(k_mx4_rows<T, true>, dim3((unsigned)ctas), dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, rows, cols, segments);
+        return launch_pdl(k_mx4_rows<T, false>, dim3((unsigned)ctas), dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, rows, cols, segments);
+    }
+    if (divup64(rows, kTile) > 65535) return DC_ERR_SHAPE;
+    MxTileParams p{x, (uint8_t*)data, (uint8_t*)scales, (uint8_t*)data_t, (uint8_t*)scales_t, colsum, rows, cols};
+    const dim3 grid((unsigned)divup64(cols, kTile), (unsigned)divup64(rows, kTile));
+    static PerDeviceOnce once;
+    bool* set = once.slot();
+    if (set == nullptr) return DC_ERR_LAUNCH;
+    if (!*set) {
+        if (cudaFuncSetAttribute(k_mx4_tile<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_bytes<T>()) != cudaSuccess ||
+            cudaFuncSetAttribute(k_mx4_tile<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_bytes<T>()) != cudaSuccess)
+            return check_launch();
+        *set = true;
+    }
+    if (vec) return launch_pdl(k_mx4_tile<T, true>, grid, dim3(256), tile_bytes<T>(), st, p);
+    return launch_pdl(k_mx4_tile<T, false>, grid, dim3(256), tile_bytes<T>(), st, p);
+}
+
+template <typename T>
+static int dequantize_t(const void* data, const void* scales, void* out, int64_t rows, int64_t cols, cudaStream_t st) {
+    const int packs = (int)divup64(cols, 8);
+    int64_t ctas = divup64(rows * packs, 256);
+    const int64_t cap = (int64_t)sm_count() * 16;
+    if (ctas > cap) ctas = cap;
+    if (aligned16(out) && cols % VecTraits<T>::kVec == 0)
+        return launch_pdl(k_mx4_dequantize<T, true>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scales, (T*)out, rows, cols, packs);
+    return launch_pdl(k_mx4_dequantize<T, false>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scales, (T*)out, rows, cols, packs);
+}
+
+}  // namespace dc
+
+using namespace dc;
+
+extern "C" {
+
+size_t dc_mx4_data_bytes(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : (size_t)(rows * mx4_blocks(cols) * 16); }
+size_t dc_mx4_scale_bytes(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : (size_t)(divup64(rows, 128) * mx4_scale_tiles(cols) * 512); }
+size_t dc_mx4_colsum_workspace_bytes(int64_t rows, int64_t cols) { return rows <= 0 || cols <= 0 ? 0 : (size_t)(divup64(rows, kTile) * cols) * sizeof(float); }
+
+int dc_mx4_quantize(const void* x, void* data, void* scales, void* data_t, void* scales_t, void* colsum, int64_t rows, int64_t cols, int32_t dtype,
+                    int32_t colsum_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (rows < 0 || cols <= 0 || cols > 0x7fffff00LL) return DC_ERR_SHAPE;
+    if (dtype < DC_F32 || dtype > DC_BF16 || (colsum != nullptr && (colsum_dtype < DC_F32 || colsum_dtype > DC_BF16))) return DC_ERR_DTYPE;
+    if ((data == nullptr) != (scales == nullptr) || (data_t == nullptr) != (scales_t == nullptr)) return DC_ERR_NULL_POINTER;
+    if (data == nullptr && data_t == nullptr && colsum == nullptr) return DC_ERR_NULL_POINTER;
+    cudaStream_t st = (cudaStream_t)stream;
+    if (rows == 0) return colsum != nullptr ? col_reduce(nullptr, 0, (int)cols, 0, colsum, nullptr, colsum_dtype, st) : (int)DC_OK;
+    if (x == nullptr) return DC_ERR_NULL_POINTER;
+    if (!aligned16(data) || !aligned16(scales) || !aligned16(data_t) || !aligned16(scales_t) || !aligned16(workspace)) return DC_ERR_ALIGNMENT;
+    if (colsum != nullptr && workspace == nullptr) return DC_ERR_NULL_POINTER;
+    if (colsum != nullptr && workspace_bytes < dc_mx4_colsum_workspace_bytes(rows, cols)) return DC_ERR_WORKSPACE;
+    float* part = colsum != nullptr ? (float*)workspace : nullptr;
+    int rc;
+    switch (dtype) {
+        case DC_F32: rc = quantize_t<float>(x, data, scales, data_t, scales_t, part, rows, cols, st); break;
+        case DC_F16: rc = quantize_t<__half>(x, data, scales, data_t, scales_t, part, rows, cols, st); break;
+        default: rc = quantize_t<__nv_bfloat16>(x, data, scales, data_t, scales_t, part, rows, cols, st); break;
+    }
+    if (rc != DC_OK || colsum == nullptr) return rc;
+    return col_reduce(part, (int)divup64(rows, kTile), (int)cols, cols, colsum, nullptr, colsum_dtype, st);
+}
+
+int dc_mx4_dequantize(const void* data, const void* scales, void* out, int64_t rows, int64_t cols, int32_t dtype, void* stream) {
+    if (rows < 0 || cols <= 0 || cols > 0x7fffff00LL) return DC_ERR_SHAPE;
+    if (dtype < DC_F32 || dtype > DC_BF16) return DC_ERR_DTYPE;
+    if (rows == 0) return DC_OK;
+    if (data == nullptr || scales == nullptr || out == nullptr) return DC_ERR_NULL_POINTER;
+    if (!aligned16(data) || !aligned16(scales)) return DC_ERR_ALIGNMENT;
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (dtype) {
+        case DC_F32: return dequantize_t<float>(data, scales, out, rows, cols, st);
+        case DC_F16: return dequantize_t<__half>(data, scales, out, rows, cols, st);
+        default: return dequantize_t<__nv_bfloat16>(data, scales, out, rows, cols, st);
+    }
+}
+
+}  // extern "C"

@@ -1,0 +1,339 @@
+// Product of two MXFP4 matrices on the block-scaled tensor core path: out[t][f] = sum_k a[t][k] b[f][k] + bias[f], a with
+// `m` rows (tokens), b with `n` rows (features, a weight in nn.Linear's layout), both packed along k (dc_mx4.cuh).
+//
+// tcgen05.mma kind::mxf4 multiplies 128 rows of one operand by up to 256 rows of the other, 64 values of k at a time, applies
+// the two scale bytes of each row's blocks in the multiplier and adds in float32 in tensor memory. The FEATURES are the 128
+// rows here and the tokens the columns of the accumulator: few tokens are then a narrow accumulator (16 columns for one
+// token) instead of 128 rows of padding, a thread of the epilogue owns one feature (one bias value), and the 32 lanes of a
+// warp store 32 neighbouring features of a token.
+//
+// A step is 256 values of k: one TMA box per operand (rows of 128 bytes, 128-byte swizzle) and the step's two 512-byte scale
+// tiles per 128 rows, in one contiguous copy each; tcgen05.cp spreads a scale tile over the four lane quarters of tensor
+// memory. Roles: one thread issues the copies, one the scale copies and MMAs, four warps drain accumulators; persistent CTAs,
+// two accumulators where the tensor memory holds them.
+//
+// Bound: many tokens, the tensor core and the shared memory that feeds it; few tokens, the weight's bytes. Then the tiles
+// do not fill the GPU, and the CTAs of a cluster share a tile along k: each leaves its float32 sums in its own shared
+// memory, and after a cluster barrier every CTA adds a share of the columns in the order of the ranks (same bits every time).
+#include <cstring>
+#include "dc_umma.cuh"
+#include "dc_mx4.cuh"
+
+namespace dc {
+
+__device__ int g_mx4_error = 0;
+
+constexpr int kMxThreads = 192;            // TMA warp, MMA warp, four epilogue warps
+constexpr int kMxStep = 256;               // values of k per step: one 128-byte row
+constexpr uint32_t kMxTmem = 512;
+
+// Columns (tokens) per tile -> stages of the ring, accumulators, tensor memory columns of a stage's scales.
+template <int NT> struct MxCfg {
+    static constexpr int kRowTiles = NT <= 128 ? 1 : 2;                 // 128-row scale tiles of the tokens
+    static constexpr int kB = NT * 128;
+    static constexpr int kScB = kRowTiles * 1024;
+    static constexpr int kStage = kABytes + kB + 1024 + kScB;
+    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 6 : 8;
+    static constexpr int kAcc = NT == 256 ? 1 : 2;
+    static constexpr int kScCols = 8 + 8 * kRowTiles;
+    static constexpr int kSmem = kStages * kStage + 1024;
+    static_assert(kAcc * NT + kStages * kScCols <= (int)kMxTmem, "tensor memory");
+    static_assert(kSmem <= 227 * 1024 - 1024, "shared memory");
+};
+
+struct MxGemmParams {
+    const uint8_t *a_sc, *b_sc;            // scales of the tokens, of the features
+    const void* bias;
+    void* out;
+    int64_t m;
+    int n, nb, tiles_k, steps;             // blocks, scale tiles and steps along k
+    int tiles_f, tiles;                    // feature tiles, all tiles
+    int bias_dtype, out_dtype;
+};
+
+__device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem_addr) {
+    uint64_t d = 0;                                       // rows of 16 bytes, 8-row groups 128 bytes apart, no swizzle
+    d |= (uint64_t)((smem_addr & 0x3FFFF) >> 4);
+    d |= (uint64_t)(128 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    return d;
+}
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+__device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+// kind::mxf4: A and B e2m1 (format 1) K-major, scales ue8m0 (bit 23), M = 128 (1 in bits 27-28), N = n; the scale data id of
+// either operand (bits 29-30, 4-5) picks the half of a 32-bit scale word: 0 or 2.
+__host__ __device__ constexpr uint32_t mx_idesc(int n) { return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27); }
+__device__ __forceinline__ uint32_t mx_idesc_half(uint32_t half) { return (half << 30) | (half << 5); }      // half * 2 in bits 29-30 and 4-5
+
+__device__ __forceinline__ float mx_bias(const MxGemmParams& p, int f) {
+    if (p.bias == nullptr) return 0.f;
+    if (p.bias_dtype == DC_F32) return ((const float*)p.bias)[f];
+    if (p.bias_dtype == DC_F16) return __half2float(((const __half*)p.bias)[f]);
+    return __bfloat162float(((const __nv_bfloat16*)p.bias)[f]);
+}
+
+template <typename OT, int NT, bool SPLIT>
+__global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+    using Cfg = MxCfg<NT>;
+    constexpr int S = Cfg::kStages;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t bars[2 * S + 4];
+    __shared__ uint32_t s_u32[2];
+    volatile uint32_t* ok_flag = &s_u32[1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };
+    auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+    auto acc_full = [&](int a) { return bar0 + 8u * (2 * S + a); };
+    auto acc_empty = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 4); }
+        *ok_flag = 1;
+        fence_barrier_init();
+    }
+    if (warp == 1) tmem_alloc(smem_u32(&s_u32[0]), kMxTmem);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_u32[0];
+    const uint32_t tmem_sc = tmem + Cfg::kAcc * NT;
+    grid_dep_launch();
+    grid_dep_wait();
+
+    // this CTA's steps of every tile: all of them, or (SPLIT) its rank's share
+    const int rank = SPLIT ? (int)blockIdx.y : 0, ranks = SPLIT ? (int)gridDim.y : 1;
+    const int k_lo = (int)((int64_t)p.steps * rank / ranks), k_hi = (int)((int64_t)p.steps * (rank + 1) / ranks);
+
+    if (warp == 0) {
+        // ---- copies: tokens' and features' boxes and scales of a step into a stage
+        int issued = 0;
+        if (elect_one()) {
+            int s = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x) {
+                const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
+                for (int ks = k_lo; ks < k_hi; ++ks) {
+                    if (!mbar_wait(empty(s), phase ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 1); ok = false; break; }
+                    const uint32_t at = ring + s * Cfg::kStage;
+                    const int nsc = min(2, p.tiles_k - ks * 2);
+                    const int rt = Cfg::kRowTiles == 1 ? 1 : min(2, (int)((p.m - (int64_t)tt * NT + 127) >> 7));
+                    mbar_expect_tx(full(s), (uint32_t)(kABytes + Cfg::kB + nsc * 512 * (1 + rt)));
+                    tma_load_rows(at, &map_b, ks * 128, tf * 128, full(s));
+                    tma_load_rows(at + kABytes, &map_a, ks * 128, tt * NT, full(s));
+                    bulk_g2s(at + kABytes + Cfg::kB, p.b_sc + ((int64_t)tf * p.tiles_k + ks * 2) * 512, (uint32_t)nsc * 512u, full(s));
+                    for (int q = 0; q < rt; ++q)
+                        bulk_g2s(at + kABytes + Cfg::kB + 1024 + q * 1024,
+                                 p.a_sc + (((int64_t)tt * NT / 128 + q) * p.tiles_k + ks * 2) * 512, (uint32_t)nsc * 512u, full(s));
+                    ++issued;
+                    if (++s == S) { s = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok) {       // leave no copy in flight behind
+                const int last = issued < S ? issued : S;
+                for (int i = issued - last; i < issued; ++i)
+                    for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(full(i % S), (uint32_t)(i / S) & 1u); ++w) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        // ---- scales to tensor memory, MMAs
+        if (elect_one()) {
+            int s = 0, it = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
+                const int a = Cfg::kAcc == 2 ? it & 1 : 0, use = Cfg::kAcc == 2 ? it >> 1 : it;
+                if (!mbar_wait(acc_empty(a), (uint32_t)(use & 1) ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 2); break; }
+                tc_fence_after();
+                const uint32_t d = tmem + a * NT;
+                for (int ks = k_lo; ks < k_hi; ++ks) {
+                    if (!mbar_wait(full(s), phase, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 3); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = ring + s * Cfg::kStage, sc = tmem_sc + s * Cfg::kScCols;
+                    const int nsc = min(2, p.tiles_k - ks * 2);
+                    for (int q = 0; q < nsc; ++q) {
+                        tmem_cp_scales(sc + q * 4, mx_scale_desc(at + kABytes + Cfg::kB + q * 512));
+#pragma unroll
+                        for (int t = 0; t < Cfg::kRowTiles; ++t)
+                            tmem_cp_scales(sc + 8 + (q * Cfg::kRowTiles + t) * 4, mx_scale_desc(at + kABytes + Cfg::kB + 1024 + t * 1024 + q * 512));
+                    }
+                    const uint64_t da = make_smem_desc(at), db = make_smem_desc(at + kABytes);
+                    const int chunks = min(4, (p.nb - ks * 8 + 1) >> 1);          // 64 values of k each
+                    for (int c = 0; c < chunks; ++c)
+                        umma_mxf4(d, da + c * 2, db + c * 2, mx_idesc(NT) | mx_idesc_half(c & 1), sc + (c >> 1) * 4,
+                                  sc + 8 + (c >> 1) * 4 * Cfg::kRowTiles, (ks > k_lo || c > 0) ? 1u : 0u);
+                    umma_commit(empty(s));
+                    if (++s == S) { s = 0; phase ^= 1u; }
+                }
+                if (ok) umma_commit(acc_full(a));
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- accumulators out: warp w owns lanes 32 (w % 4) .. + 31, a lane is a feature
+        const int quarter = warp & 3;
+        int it = 0;
+        for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, ++it) {
+            const int a = Cfg::kAcc == 2 ? it & 1 : 0, use = Cfg::kAcc == 2 ? it >> 1 : it;
+            const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
+            const int f = tf * 128 + quarter * 32 + lane;
+            const float bias = f < p.n && !SPLIT ? mx_bias(p, f) : 0.f;
+            if (!mbar_wait_warp(acc_full(a), (uint32_t)(use & 1), ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 4); break; }
+            tc_fence_after();
+            const uint32_t src = tmem + a * NT + ((uint32_t)quarter << 21);
+            const int64_t t0 = (int64_t)tt * NT;
+            const int cols = (int)(p.m - t0 < NT ? p.m - t0 : NT);
+            for (int c = 0; c < NT; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(src + c, r);
+                tmem_ld_wait();
+                if constexpr (SPLIT) {
+                    float* part = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));        // the stages are free: every MMA has read its own
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) part[(c + i) * 128 + quarter * 32 + lane] = __uint_as_float(r[i]);
+                } else if (f < p.n) {
+                    OT* o = (OT*)p.out + (t0 + c) * p.n + f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        if (c + i < cols) o[(int64_t)i * p.n] = from_f<OT>(__uint_as_float(r[i]) + bias);
+                }
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(acc_empty(a));
+        }
+    }
+    if constexpr (SPLIT) {
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+        // columns rank, rank + ranks, ... of the tile: sum over the ranks in their order
+        const int tile = blockIdx.x, tf = tile % p.tiles_f, tt = tile / p.tiles_f;
+        const int64_t t0 = (int64_t)tt * NT;
+        const int cols = (int)(p.m - t0 < NT ? p.m - t0 : NT);
+        const bool good = *ok_flag != 0;
+        for (int i = threadIdx.x; i < 128 * ((cols - rank + ranks - 1) / ranks); i += kMxThreads) {
+            const int col = rank + (i >> 7) * ranks, f = tf * 128 + (i & 127);
+            if (f >= p.n || !good) continue;
+            float v = 0.f;
+            for (int q = 0; q < ranks; ++q) {
+                uint32_t remote;
+                float x;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(ring + (uint32_t)(col * 128 + (i & 127)) * 4u), "r"(q));
+                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote) : "memory");
+                v += x;
+            }
+            ((OT*)p.out)[(t0 + col) * p.n + f] = from_f<OT>(v + mx_bias(p, f));
+        }
+        asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) tmem_dealloc(tmem, kMxTmem);
+}
+
+// Packed matrix [rows][16 nb] bytes as a tensor map, box 128 bytes x `box_rows`, 128-byte swizzle.
+typedef CUresult (*MxEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int64_t row_bytes, int box_rows) {
+    static const MxEncodeFn fn = [] {
+        void* ptr = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+            return reinterpret_cast<MxEncodeFn>(ptr);
+        (void)cudaGetLastError();
+        return (MxEncodeFn) nullptr;
+    }();
+    if (fn == nullptr) return false;
+    const cuuint64_t gdim[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
+    const cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
+    const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
+    const cuuint32_t estride[2] = {1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename OT, int NT, bool SPLIT>
+static int launch_mx4(const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
+    // a cluster's CTAs wait for one another: they take an SM's whole shared memory, so that no other kernel's CTA that waits in
+    // a cluster too can hold tensor memory on the same SM
+    constexpr size_t smem = SPLIT ? (size_t)226 * 1024 : (size_t)MxCfg<NT>::kSmem;
+    static PerDeviceOnce once;
+    bool* set = once.slot();
+    if (set == nullptr) return DC_ERR_LAUNCH;
+    if (!*set) {
+        if (cudaFuncSetAttribute(k_mx4_gemm<OT, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return check_launch();
+        *set = true;
+    }
+    const int sms = sm_count();
+    const dim3 grid((unsigned)(SPLIT ? p.tiles : p.tiles < sms ? p.tiles : sms), (unsigned)split);
+    return launch_pdl_cluster(k_mx4_gemm<OT, NT, SPLIT>, grid, dim3(kMxThreads), smem, st, split, p, ma, mb);
+}
+
+template <typename OT, bool SPLIT>
+static int launch_mx4_nt(int nt, const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
+    switch (nt) {
+        case 16: return launch_mx4<OT, 16, SPLIT>(p, split, ma, mb, st);
+        case 32: return launch_mx4<OT, 32, SPLIT>(p, split, ma, mb, st);
+        case 64: return launch_mx4<OT, 64, SPLIT>(p, split, ma, mb, st);
+        case 128: return launch_mx4<OT, 128, SPLIT>(p, split, ma, mb, st);
+        default: return launch_mx4<OT, 256, SPLIT>(p, split, ma, mb, st);
+    }
+}
+template <typename OT>
+static int launch_mx4_split(int nt, const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
+    return split > 1 ? launch_mx4_nt<OT, true>(nt, p, split, ma, mb, st) : launch_mx4_nt<OT, false>(nt, p, 1, ma, mb, st);
+}
+
+int mx4_error_code() {
+    int v = 0;
+    if (cudaMemcpyFromSymbol(&v, g_mx4_error, sizeof(int)) != cudaSuccess) return -1;
+    return v;
+}
+
+}  // namespace dc
+
+using namespace dc;
+
+extern "C" int dc_mx4_matmul(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m,
+                             int64_t n, int64_t k, int32_t bias_dtype, int32_t out_dtype, void* stream) {
+    if (m < 0 || n < 0 || k <= 0 || m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return DC_ERR_SHAPE;
+    if (out_dtype < DC_F32 || out_dtype > DC_BF16 || (bias != nullptr && (bias_dtype < DC_F32 || bias_dtype > DC_BF16))) return DC_ERR_DTYPE;
+    if (m == 0 || n == 0) return DC_OK;
+    if (a_data == nullptr || a_scales == nullptr || b_data == nullptr || b_scales == nullptr || out == nullptr) return DC_ERR_NULL_POINTER;
+    if (!aligned16(a_data) || !aligned16(a_scales) || !aligned16(b_data) || !aligned16(b_scales)) return DC_ERR_ALIGNMENT;
+    const int sms = sm_count();
+    // columns of a tile: no more than the tokens need; beyond 128 the wide tile, if its tiles still fill the GPU (it reads half
+    // as many feature bytes per product)
+    int nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    const int64_t tiles_f = divup64(n, 128);
+    if (m > 128 && tiles_f * divup64(m, 256) >= sms) nt = 256;
+    const int64_t tiles = tiles_f * divup64(m, nt);
+    if (tiles > 0x7fffffffLL) return DC_ERR_SHAPE;
+    MxGemmParams p{};
+    p.a_sc = (const uint8_t*)a_scales; p.b_sc = (const uint8_t*)b_scales; p.bias = bias; p.out = out;
+    p.m = m; p.n = (int)n; p.nb = (int)mx4_blocks(k); p.tiles_k = (int)mx4_scale_tiles(k); p.steps = (int)divup64(k, kMxStep);
+    p.tiles_f = (int)tiles_f; p.tiles = (int)tiles;
+    p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
+    // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each
+    int split = 1;
+    while (split < 8 && tiles * split * 2 <= sms && p.steps >= split * 2) split *= 2;
+    alignas(64) CUtensorMap ma, mb;
+    if (!encode_mx4_map(&ma, a_data, m, (int64_t)p.nb * 16, nt) || !encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128)) return DC_ERR_UNSUPPORTED;
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (out_dtype) {
+        case DC_F32: return launch_mx4_split<float>(nt, p, split, ma, mb, st);
+        case DC_F16: return launch_mx4_split<__half>(nt, p, split, ma, mb, st);
+        default: return launch_mx4_split<__nv_bfloat16>(nt, p, split, ma, mb, st);
+    }
+}

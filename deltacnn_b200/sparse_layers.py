@@ -20,6 +20,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
+from . import channel_ops as C
 from . import cuda_kernels as K
 from .filter_conversion import convert_filter_out_channels_last, convert_half_filter
 
@@ -141,6 +142,8 @@ class DCModule(nn.Module):
         ``.to(device, memory_format=channels_last)`` and the optional ``.half()``)."""
         for mod in self.modules():
             if type(mod) in (DCConv2d, DCConvTranspose2d):
+                mod.process_filters()
+            elif type(mod) is DCMX4Linear and mod is not self:
                 mod.process_filters()
 
     def reset_layers(self):
@@ -905,6 +908,79 @@ class DCLinear(nn.Linear, DCModule):
         DCModule.reset(self)
         self.acc = None
         self._out = None
+
+
+class DCLayerNorm(nn.LayerNorm, DCModule):
+    """Layer norm over the channels of a feature map. On a (delta, mask) pair it keeps the accumulated input and what it has
+    handed on so far, and hands on the change of the norm where any channel's change is above ``delta_threshold`` (the same
+    truncation as ``DCActivation``, mask cleared in place); the first frame is normalised as a whole. A dense tensor
+    (N, C, H, W channels-last, or (..., C)) is normalised by the same arithmetic and has gradients. No reference counterpart
+    (the reference's only norm is DCBatchNorm2d, src/deltacnn/sparse_layers.py:1516-1585)."""
+
+    def __init__(self, num_features, eps=1e-5, elementwise_affine=True, bias=True, delta_threshold=None, name="", inplace=True):
+        nn.LayerNorm.__init__(self, num_features, eps=eps, elementwise_affine=elementwise_affine, bias=bias)
+        if len(self.normalized_shape) != 1:
+            raise RuntimeError("DCLayerNorm normalises over the channels: num_features must be one number")
+        self.name = name
+        self.inplace = inplace
+        self.delta_threshold = delta_threshold if delta_threshold is not None else DCThreshold.t_default
+        self.first_iter = True
+        self.prev_in = None
+        self.prev_out = None
+
+    def forward(self, input):
+        if type(input) != tuple:
+            return C.layer_norm(input, self.weight, self.bias, self.eps)
+        val, mask = input
+        weight = None if self.weight is None else self.weight.detach()
+        bias = None if self.bias is None else self.bias.detach()
+        if self.first_iter:
+            K._check_feature(val, "input")
+            self.first_iter = False
+            if self not in DCThreshold.t:
+                DCThreshold.set(self, self.delta_threshold)
+            self.prev_in = val.detach().clone()
+            self.prev_out = C.layer_norm(self.prev_in, weight, bias, self.eps)
+            DCModule.temp_buffers.append(self.prev_in)
+            DCModule.temp_buffers.append(self.prev_out)
+            return self.prev_out.clone(), mask
+        if not self.inplace:
+            val = val.clone()
+            mask = mask.clone()
+        mask_before = mask.clone() if K.DCPerformanceMetricsManager.enabled else None
+        C.layer_norm_delta(val, mask, self.prev_in, self.prev_out, weight, bias, DCThreshold.get(self), self.eps, out=val, out_mask=mask)
+        if mask_before is not None:
+            K.DCPerformanceMetricsManager.add_activation(mask_before, val.shape[1], DCTruncation.max.value, mask)
+        return val, mask
+
+    def reset(self):
+        DCModule.reset(self)
+        self.first_iter = True
+        self.prev_in = None
+        self.prev_out = None
+
+
+class DCMX4Linear(nn.Linear, DCModule):
+    """Fully connected (or pointwise) layer on dense features in MXFP4: activations and weight are rounded to 4 bits with a
+    scale per 32 values and multiplied on the block-scaled tensor core path. ``process_filters()`` packs the weight once for
+    inference; before it the weight is packed in every call and the layer has gradients (three 4-bit products, the
+    rounding's own gradient taken as 1). Takes (..., in_features), or (N, C, H, W) channels-last maps. A (delta, mask) pair is refused: rounding
+    errors of deltas would add up over the frames (put it behind ``DCDensify``). No reference counterpart."""
+
+    def __init__(self, in_features, out_features, bias=True):
+        nn.Linear.__init__(self, in_features, out_features, bias)
+        self.weight_mx4 = None
+
+    def process_filters(self):
+        """Pack the weight; call again after changing it."""
+        self.weight_mx4 = C.mx4_quantize(self.weight.detach().contiguous())
+
+    def forward(self, input):
+        if type(input) == tuple:
+            raise RuntimeError("DCMX4Linear takes dense features: put it behind DCDensify")
+        if self.weight_mx4 is None:
+            return C.mx4_linear(input, self.weight, self.bias)
+        return C.mx4_linear(input, self.weight_mx4, None if self.bias is None else self.bias.detach())
 
 
 class DCHeatmapArgmax(DCModule):

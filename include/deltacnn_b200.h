@@ -31,12 +31,13 @@ typedef enum dc_status {
     DC_ERR_UNSUPPORTED = 2,    /* kernel size / stride / groups / mode not supported */
     DC_ERR_ALIGNMENT = 3,      /* a pointer is not aligned for the vector width in use */
     DC_ERR_SHAPE = 4,          /* inconsistent or non-positive sizes */
-    DC_ERR_DTYPE = 5,          /* dtype is neither DC_F32 nor DC_F16 */
+    DC_ERR_DTYPE = 5,          /* dtype is neither DC_F32 nor DC_F16 (nor DC_BF16, where that is understood) */
     DC_ERR_LAUNCH = 6,         /* the CUDA runtime refused the launch (see dc_last_cuda_error) */
     DC_ERR_WORKSPACE = 7       /* caller-provided workspace too small */
 } dc_status;
 
-typedef enum dc_dtype { DC_F32 = 0, DC_F16 = 1 } dc_dtype;
+/* DC_BF16 is understood by the entry points that say so (dc_layer_norm, dc_layer_norm_backward, dc_mx4_*). */
+typedef enum dc_dtype { DC_F32 = 0, DC_F16 = 1, DC_BF16 = 2 } dc_dtype;
 
 /* Activation codes, as src/deltacnn/sparse_layers.py:20-34 (<=0: identity). */
 typedef enum dc_activation {
@@ -320,6 +321,63 @@ int dc_heatmap_argmax(const void* heat, const int32_t* mask, float* out, int32_t
 int dc_centernet_decode(const void* heat, const void* wh, const void* offset, const int32_t* mask, float* peaks, float* det,
                         int32_t* count, int32_t n, int32_t h, int32_t w, int32_t classes, int32_t topk, float min_score,
                         float stride, int32_t apply_sigmoid, int32_t dtype, void* stream);
+
+/* ---- layer norm ------------------------------------------------------------------------------------------
+ * No counterpart in the reference, whose only norm is DCBatchNorm2d (src/deltacnn/sparse_layers.py:1516-1585).
+ * A row is the channel vector of one pixel or token: rows x c contiguous elements. Statistics, sums and products are
+ * float32, each stored value is rounded once. dtype: DC_F32, DC_F16 or DC_BF16; weight_dtype: dtype or DC_F32.
+ * weight and bias (c elements) may be NULL (1 and 0). */
+
+/* y = (x - mean) * rstd * weight + bias, mean and rstd = 1 / sqrt(variance + eps) over the row (variance with divisor
+ * c). mean, rstd: float32 per row for the backward pass, or both NULL. y may be x. */
+int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, int64_t rows, int32_t c,
+                  int32_t dtype, int32_t weight_dtype, float eps, void* stream);
+
+/* Gradients of dc_layer_norm: with g = dy * weight and n = (x - mean) * rstd,
+ *   dx = rstd * (g - mean(g) - n * mean(g * n)),  dweight = sum_rows(dy * n),  dbias = sum_rows(dy).
+ * dx, dweight, dbias may be NULL where not wanted. dx may be dy. workspace: dc_layer_norm_backward_workspace_bytes of device
+ * memory, only meaningful during the call (per-CTA partial sums of the column reductions, added in a fixed order: the same
+ * inputs give the same bits). rows == 0 writes zeros to dweight and dbias. */
+size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype);
+int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
+                           void* dweight, void* dbias, int64_t rows, int32_t c, int32_t dtype, int32_t weight_dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* Layer norm over the channels in delta form (DC_F32, DC_F16). prev_in holds the accumulated input, prev_out the sum of what
+ * was handed on so far. On pixels with mask != 0: prev_in += delta; e = layer_norm(prev_in) - prev_out; where any
+ * |e| > threshold: out = e, prev_out += e, mask_out = 1. Everywhere else mask_out = 0, and out and prev_out stay as they are
+ * (a change below the threshold is not lost: it stays in prev_in). out may be delta, mask_out may be mask. */
+int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, void* prev_out, const void* weight, const void* bias,
+                        void* out, int32_t* mask_out, int64_t npix, int32_t c, int32_t dtype, int32_t weight_dtype, float threshold,
+                        float eps, void* stream);
+
+/* ---- MXFP4: quantisation and products ----------------------------------------------------------------------
+ * No counterpart in the reference. A row of a matrix is cut into blocks of 32 values; a block is 32 e2m1 codes (+-{0, 1/2, 1,
+ * 3/2, 2, 3, 4, 6}) under one scale 2^(s - 127). With E the biased float32 exponent of the block's largest magnitude,
+ * s = max(E - 2, 0); values are rounded to nearest even and saturate at 6; s = 255 marks a block that holds an infinity
+ * or a NaN and stands for NaN as a whole. nb = ceil(cols / 32):
+ *   data:   [rows][16 nb] bytes, the even column in the low half of a byte, zeros behind the last column
+ *   scales: [ceil(rows / 128)][ceil(nb / 4)][32][4][4] bytes, block b of row r at [r/128][b/4][r%32][r%128/32][b%4]. Bytes of
+ *           blocks nb .. are written for every row, bytes of rows behind the last one are not.
+ * All four pointers 16-byte aligned; x and out need no alignment beyond their type's. dtypes: DC_F32, DC_F16, DC_BF16. */
+size_t dc_mx4_data_bytes(int64_t rows, int64_t cols);
+size_t dc_mx4_scale_bytes(int64_t rows, int64_t cols);
+
+/* x (rows x cols, contiguous) packed along its rows (data, scales) and / or along its columns, as the transposed matrix of
+ * cols x rows (data_t, scales_t); either pair may be NULL. colsum (cols elements of colsum_dtype, may be NULL): the column
+ * sums of x in float32, added in a fixed order; needs dc_mx4_colsum_workspace_bytes of device memory, only meaningful
+ * during the call. x is read once. */
+size_t dc_mx4_colsum_workspace_bytes(int64_t rows, int64_t cols);
+int dc_mx4_quantize(const void* x, void* data, void* scales, void* data_t, void* scales_t, void* colsum, int64_t rows, int64_t cols, int32_t dtype,
+                    int32_t colsum_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The values a packed matrix stands for, rows x cols contiguous. */
+int dc_mx4_dequantize(const void* data, const void* scales, void* out, int64_t rows, int64_t cols, int32_t dtype, void* stream);
+
+/* out[i][j] = sum_k a[i][k] * b[j][k] + bias[j] in float32, rounded once to out_dtype: a is m x k, b is n x k (a weight in
+ * nn.Linear's layout), both packed; out m x n contiguous; bias n elements or NULL. */
+int dc_mx4_matmul(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m,
+                  int64_t n, int64_t k, int32_t bias_dtype, int32_t out_dtype, void* stream);
 
 #ifdef __cplusplus
 }
