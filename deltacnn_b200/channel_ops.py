@@ -17,17 +17,31 @@ from .cuda_kernels import _check_feature, _check_like, _check_mask
 _CODES = {torch.float32: _lib.DC_F32, torch.float16: _lib.DC_F16, torch.bfloat16: _lib.DC_BF16}
 
 
-class _on:
-    """Makes a tensor's device the current one for the launch (nothing to do on the usual path)."""
+_raw_stream = torch._C._cuda_getCurrentRawStream      # what torch.cuda.current_stream(i).cuda_stream gives, at a fortieth of the time
+
+
+def _launch(op, fn, t, *args):
+    """Calls a library entry point on t's device and that device's current stream."""
+    index = t.get_device()
+    if index == torch.cuda.current_device():
+        status = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, _raw_stream(index))
+    if status:
+        check(status, op)
+
+
+class _device:
+    """Makes a tensor's device the current one (nothing to do on the usual path)."""
     __slots__ = ("guard",)
 
     def __init__(self, t):
-        self.guard = torch.cuda.device(t.device) if t.device.index != torch.cuda.current_device() else None
+        self.guard = torch.cuda.device(t.device) if t.get_device() != torch.cuda.current_device() else None
 
     def __enter__(self):
         if self.guard is not None:
             self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
 
     def __exit__(self, *exc):
         if self.guard is not None:
@@ -91,49 +105,59 @@ def _ln_params(x, c, code, weight, bias, op):
     return code if wcode is None else wcode
 
 
-def _ln_forward(x, weight, bias, eps, keep):
-    op = "layer_norm"
-    rows, c = _rows(x, op)
-    code = _code(x, op, "x")
-    wcode = _ln_params(x, c, code, weight, bias, op)
+def _ln_forward(x, rows, c, weight, bias, eps, keep):
+    code = _code(x, "layer_norm", "x")
+    wcode = _ln_params(x, c, code, weight, bias, "layer_norm")
     y = torch.empty_like(x)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
-    mean, rstd = (stats.data_ptr(), stats.data_ptr() + 4 * rows) if keep and rows > 0 else (None, None)
+    stats = mean = rstd = None
+    if keep:
+        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean = stats.data_ptr()
+        rstd = mean + 4 * rows
     if rows > 0:
-        with _on(x) as stream:
-            check(lib.dc_layer_norm(x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, rstd, rows, c, code, wcode, eps, stream), op)
+        _launch("layer_norm", lib.dc_layer_norm, x, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean, rstd, rows, c, code, wcode, eps)
     return y, stats
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, stats = _ln_forward(x, weight, bias, eps, True)
+        rows, c = _rows(x, "layer_norm")
+        y, stats = _ln_forward(x, rows, c, weight, bias, eps, True)
         ctx.save_for_backward(x, weight, stats)
-        ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.sizes = rows, c
+        ctx.wtype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        return _LayerNorm._again(ctx, dy) if torch.is_grad_enabled() else _LayerNorm._backward(ctx, dy)
+
+    @staticmethod
+    def _backward(ctx, dy):
         x, weight, stats = ctx.saved_tensors
         need_x, need_w, need_b, _ = ctx.needs_input_grad
-        rows, c = _rows(x, "layer_norm")
+        rows, c = ctx.sizes
         dy = _like_rows(dy, x)
-        wtype = weight.dtype if weight is not None else ctx.bias_dtype if ctx.bias_dtype is not None else x.dtype
+        code, wtype = _CODES[x.dtype], ctx.wtype
         dx = torch.empty_like(x) if need_x else None
-        dw = torch.empty(c, dtype=wtype, device=x.device) if need_w else None
-        db = torch.empty(c, dtype=wtype, device=x.device) if need_b else None
-        code = _CODES[x.dtype]
-        with _on(x) as stream:
-            ws, nbytes = None, 0
-            if need_w or need_b:
-                nbytes = lib.dc_layer_norm_backward_workspace_bytes(rows, c, code)
-                ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-            mean = stats.data_ptr()
-            check(lib.dc_layer_norm_backward(_ptr(dy), _ptr(x), _ptr(weight), mean, mean + 4 * rows if rows > 0 else None, _ptr(dx), _ptr(dw), _ptr(db),
-                                             rows, c, code, _CODES[wtype], _ptr(ws), nbytes, stream), "layer_norm_backward")
+        dw = x.new_empty(c, dtype=wtype) if need_w else None
+        db = x.new_empty(c, dtype=wtype) if need_b else None
+        ws, floats = None, 0
+        if need_w or need_b:
+            with _device(x):
+                floats = lib.dc_layer_norm_backward_workspace_bytes(rows, c, code) // 4
+            ws = x.new_empty(floats, dtype=torch.float32)
+        mean = stats.data_ptr()
+        _launch("layer_norm_backward", lib.dc_layer_norm_backward, x, dy.data_ptr(), x.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw),
+                _ptr(db), rows, c, code, _CODES[wtype], _ptr(ws), 4 * floats)
         return dx, dw, db, None
+
+    @staticmethod
+    @once_differentiable
+    def _again(ctx, dy):
+        # under create_graph: the gradients' own gradients raise instead of being wrong
+        return _LayerNorm._backward(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -142,7 +166,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     in a fixed order, so equal inputs give equal bits. No reference counterpart."""
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
-    return _ln_forward(x, weight, bias, eps, False)[0]
+    rows, c = _rows(x, "layer_norm")
+    return _ln_forward(x, rows, c, weight, bias, eps, False)[0]
 
 
 def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, threshold=0.0, eps=1e-5, out=None, out_mask=None):
@@ -174,9 +199,8 @@ def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, thr
     for t, name in ((mask, "mask"), (out_mask, "out_mask")):
         if t.device != delta.device or not t.is_contiguous():
             _fail(op, f"{name} must be contiguous and on {delta.device}")
-    with _on(delta) as stream:
-        check(lib.dc_layer_norm_delta(delta.data_ptr(), mask.data_ptr(), prev_in.data_ptr(), prev_out.data_ptr(), _ptr(weight), _ptr(bias),
-                                      out.data_ptr(), out_mask.data_ptr(), n * h * w, c, code, wcode, float(threshold), eps, stream), op)
+    _launch(op, lib.dc_layer_norm_delta, delta, delta.data_ptr(), mask.data_ptr(), prev_in.data_ptr(), prev_out.data_ptr(), _ptr(weight), _ptr(bias),
+            out.data_ptr(), out_mask.data_ptr(), n * h * w, c, code, wcode, float(threshold), eps)
     return out, out_mask
 
 
@@ -192,44 +216,59 @@ class MX4Tensor:
     column in the low half, zeros behind the last column. ``scales``: uint8 (ceil(rows / 128), ceil(nb / 4), 32, 4, 4), block b of
     row r at [r // 128, b // 4, r % 32, r % 128 // 32, b % 4] (what the tensor core reads); its entries for rows behind
     the last one are never looked at, those for blocks behind the last one must not be 255."""
-    __slots__ = ("data", "scales", "shape")
+    __slots__ = ("_data", "_scales", "_at", "shape")
 
     def __init__(self, data, scales, shape):
         rows, cols = shape
         want_data, want_scales = _mx4_shapes(rows, cols)
-        if cols <= 0 or data.dtype != torch.uint8 or scales.dtype != torch.uint8 or tuple(data.shape) != want_data or tuple(scales.shape) != want_scales:
+        if cols <= 0 or data.dtype != torch.uint8 or scales.dtype != torch.uint8 or data.shape != want_data or scales.shape != want_scales:
             raise RuntimeError(f"deltacnn_b200.MX4Tensor: a {rows} x {cols} matrix needs uint8 data {want_data} and scales {want_scales}")
         if not data.is_contiguous() or not scales.is_contiguous() or data.device != scales.device:
             raise RuntimeError("deltacnn_b200.MX4Tensor: data and scales must be contiguous and on one device")
-        self.data, self.scales, self.shape = data, scales, (rows, cols)
+        self._data, self._scales, self._at, self.shape = data, scales, None, (rows, cols)
+
+    @classmethod
+    def _empty(cls, rows, cols, like):
+        """A new matrix in one allocation: the scales stand behind the codes, ``_at`` bytes into it."""
+        q = cls.__new__(cls)
+        nb = (cols + 31) // 32
+        q._at = rows * nb * 16
+        q._data, q._scales, q.shape = like.new_empty(q._at + (rows + 127) // 128 * ((nb + 3) // 4) * 512, dtype=torch.uint8), None, (rows, cols)
+        return q
+
+    @property
+    def data(self):
+        return self._data if self._at is None else self._data[:self._at].view(_mx4_shapes(*self.shape)[0])
+
+    @property
+    def scales(self):
+        return self._scales if self._at is None else self._data[self._at:].view(_mx4_shapes(*self.shape)[1])
+
+    def _ptrs(self):
+        p = self._data.data_ptr()
+        return p, (self._scales.data_ptr() if self._at is None else p + self._at)
 
     def dequantize(self, dtype=torch.float32):
         return mx4_dequantize(self, dtype)
-
-
-def _mx4_empty(rows, cols, device):
-    data, scales = _mx4_shapes(rows, cols)
-    q = MX4Tensor.__new__(MX4Tensor)
-    q.data, q.scales, q.shape = torch.empty(data, dtype=torch.uint8, device=device), torch.empty(scales, dtype=torch.uint8, device=device), (rows, cols)
-    return q
 
 
 def _quantize(x, rows, cols, along_rows, along_cols, colsum=None):
     """(packed x or None, packed x^T or None); ``colsum``: a (cols,) tensor that receives the column sums. An empty x has no
     packed transpose (a matrix without columns)."""
     code = _code(x, "mx4_quantize", "x")
-    q = _mx4_empty(rows, cols, x.device) if along_rows else None
-    qt = _mx4_empty(cols, rows, x.device) if along_cols and rows > 0 else None
-    ws, nbytes = None, 0
+    q = MX4Tensor._empty(rows, cols, x) if along_rows else None
+    qt = MX4Tensor._empty(cols, rows, x) if along_cols and rows > 0 else None
+    ws, nbytes, sum_code = None, 0, 0
     if colsum is not None:
-        nbytes = lib.dc_mx4_colsum_workspace_bytes(rows, cols)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        nbytes, sum_code = lib.dc_mx4_colsum_workspace_bytes(rows, cols), _CODES[colsum.dtype]
+        ws = x.new_empty(nbytes // 4, dtype=torch.float32)
     if rows > 0 or colsum is not None:
-        with _on(x) as stream:
-            check(lib.dc_mx4_quantize(x.data_ptr(), q and q.data.data_ptr(), q and q.scales.data_ptr(), qt and qt.data.data_ptr(),
-                                      qt and qt.scales.data_ptr(), _ptr(colsum), rows, cols, code, 0 if colsum is None else _CODES[colsum.dtype],
-                                      _ptr(ws), nbytes, stream), "mx4_quantize")
+        _launch("mx4_quantize", lib.dc_mx4_quantize, x, x.data_ptr(), *(q._ptrs() if q is not None else _NONE), *(qt._ptrs() if qt is not None else _NONE),
+                _ptr(colsum), rows, cols, code, sum_code, _ptr(ws), nbytes)
     return q, qt
+
+
+_NONE = (None, None)
 
 
 def mx4_quantize(x):
@@ -255,13 +294,17 @@ def mx4_dequantize(q, dtype=torch.float32):
     rows, cols = q.shape
     if dtype not in _CODES:
         _fail(op, f"unsupported dtype {dtype} (float32, float16 and bfloat16 only)")
-    if not q.data.is_cuda:
+    if not q._data.is_cuda:
         _fail(op, "data must be a CUDA tensor (there is no CPU path)")
-    out = torch.empty((rows, cols), dtype=dtype, device=q.data.device)
+    out = q._data.new_empty((rows, cols), dtype=dtype)
     if rows > 0:
-        with _on(q.data) as stream:
-            check(lib.dc_mx4_dequantize(q.data.data_ptr(), q.scales.data_ptr(), out.data_ptr(), rows, cols, _CODES[dtype], stream), op)
+        _launch(op, lib.dc_mx4_dequantize, out, *q._ptrs(), out.data_ptr(), rows, cols, _CODES[dtype])
     return out
+
+
+def _check_bias(op, bias, n, device):
+    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous() or bias.device != device or bias.dtype not in _CODES):
+        _fail(op, f"bias must be a contiguous ({n},) tensor on {device}")
 
 
 def mx4_matmul(a, b, bias=None, dtype=torch.float16, out=None):
@@ -271,21 +314,19 @@ def mx4_matmul(a, b, bias=None, dtype=torch.float16, out=None):
     (m, k), (n, k2) = a.shape, b.shape
     if k != k2:
         _fail(op, f"the matrices have {k} and {k2} columns")
-    if dtype not in _CODES:
+    code = _CODES.get(dtype)
+    if code is None:
         _fail(op, f"unsupported dtype {dtype} (float32, float16 and bfloat16 only)")
-    device = a.data.device
-    if not a.data.is_cuda or b.data.device != device:
+    device = a._data.device
+    if not a._data.is_cuda or b._data.device != device:
         _fail(op, "both matrices must be on one CUDA device (there is no CPU path)")
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous() or bias.device != device or bias.dtype not in _CODES):
-        _fail(op, f"bias must be a contiguous ({n},) tensor on {device}")
+    _check_bias(op, bias, n, device)
     if out is None:
-        out = torch.empty((m, n), dtype=dtype, device=device)
+        out = a._data.new_empty((m, n), dtype=dtype)
     elif out.dtype != dtype or tuple(out.shape) != (m, n) or not out.is_contiguous() or out.device != device:
         _fail(op, f"out must be a contiguous ({m}, {n}) tensor of type {dtype} on {device}")
     if m > 0 and n > 0:
-        with _on(out) as stream:
-            check(lib.dc_mx4_matmul(a.data.data_ptr(), a.scales.data_ptr(), b.data.data_ptr(), b.scales.data_ptr(), _ptr(bias), out.data_ptr(), m, n, k,
-                                    0 if bias is None else _CODES[bias.dtype], _CODES[dtype], stream), op)
+        _launch(op, lib.dc_mx4_matmul, out, *a._ptrs(), *b._ptrs(), _ptr(bias), out.data_ptr(), m, n, k, 0 if bias is None else _CODES[bias.dtype], code)
     return out
 
 
@@ -313,12 +354,20 @@ class _MX4Linear(torch.autograd.Function):
         return _unrows(mx4_matmul(xq, wq, bias, x.dtype), x)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        return _MX4Linear._again(ctx, dy) if torch.is_grad_enabled() else _MX4Linear._backward(ctx, dy)
+
+    @staticmethod
+    @once_differentiable
+    def _again(ctx, dy):
+        return _MX4Linear._backward(ctx, dy)
+
+    @staticmethod
+    def _backward(ctx, dy):
         need_x, need_w, need_b = ctx.needs_input_grad
         rows, cols, outs = ctx.sizes
         dy = _like_rows(dy, dy)
-        db = torch.empty(outs, dtype=ctx.dtypes[2], device=dy.device) if need_b else None
+        db = dy.new_empty(outs, dtype=ctx.dtypes[2]) if need_b else None
         if rows == 0:
             dx = dy.new_zeros(ctx.x_shape, dtype=ctx.dtypes[0]) if need_x else None
             return dx, dy.new_zeros((outs, cols), dtype=ctx.dtypes[1]) if need_w else None, None if db is None else db.zero_()
@@ -352,8 +401,7 @@ def mx4_linear(x, weight, bias=None):
         return _unrows(mx4_matmul(_quantize(x, rows, cols, True, False)[0], weight, bias, x.dtype), x)
     if not weight.is_contiguous() or weight.device != x.device or weight.dtype not in _CODES or outs == 0:
         _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != outs or not bias.is_contiguous() or bias.device != x.device or bias.dtype not in _CODES):
-        _fail(op, f"bias must be a contiguous ({outs},) tensor on {x.device}")
+    _check_bias(op, bias, outs, x.device)
     if grad:
         return _MX4Linear.apply(x, weight, bias)
     return _unrows(mx4_matmul(_quantize(x, rows, cols, True, False)[0], _quantize(weight, outs, cols, True, False)[0], bias, x.dtype), x)
