@@ -49,6 +49,7 @@ struct MxGemmParams {
     int n, nb, tiles_k, steps;             // blocks, scale tiles and steps along k
     int tiles_f, tiles;                    // feature tiles, all tiles
     int bias_dtype, out_dtype;
+    int out_even;                          // out is 4-byte aligned (16-bit results)
 };
 
 __device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem_addr) {
@@ -71,8 +72,21 @@ __device__ __forceinline__ void umma_mxf4(uint32_t tmem_d, uint64_t adesc, uint6
 // kind::mxf4: A and B e2m1 (format 1) K-major, scales ue8m0 (bit 23), M = 128 (1 in bits 27-28), N = n; the scale data id of
 // either operand (bits 29-30, 4-5) picks the half of a 32-bit scale word: 0 or 2.
 __host__ __device__ constexpr uint32_t mx_idesc(int n) { return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (1u << 27); }
+__host__ __device__ constexpr uint32_t mx_idesc2(int n) { return (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | (2u << 27); }      // M = 256
 __device__ __forceinline__ uint32_t mx_idesc_half(uint32_t half) { return (half << 30) | (half << 5); }      // half * 2 in bits 29-30 and 4-5
 
+template <typename OT> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void cluster_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
 __device__ __forceinline__ float mx_bias(const MxGemmParams& p, int f) {
     if (p.bias == nullptr) return 0.f;
     if (p.bias_dtype == DC_F32) return ((const float*)p.bias)[f];
@@ -242,10 +256,224 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
     if (warp == 1) tmem_dealloc(tmem, kMxTmem);
 }
 
+// ---------------------------------------------------------------------------------------------
+// Many tokens: two SMs per tile
+// ---------------------------------------------------------------------------------------------
+// A cluster of two CTAs computes 256 features x 256 tokens with tcgen05.mma.cta_group::2: either CTA holds 128 features and
+// stages its features' rows and HALF of the tokens' rows, the tensor cores read the other half from the peer. Per step an SM
+// stages 32 KB of codes for 128 x 256 outputs instead of 48 KB. Either CTA's copies count on the leader's barrier, the
+// leader issues the scale copies and MMAs for both, its commits arrive in both.
+// The accumulator takes 256 of the 512 columns and the stages' scales 120, so there is one accumulator; the epilogue (eight
+// warps, a thread holds 128 tokens of its feature) therefore first drains it into registers, hands it back, and
+// stores while the next tile's MMAs run. Lanes hold neighbouring features of one token pair per register: a shuffle with the
+// neighbour lane makes four-byte stores of two features where the row width is even.
+constexpr int kM2Threads = 320;            // TMA warp, MMA warp, eight epilogue warps
+constexpr int kM2Stages = 5;
+constexpr int kM2Tok = 256;                // tokens of a tile (128 rows staged per CTA)
+constexpr int kM2Stage = kABytes + kABytes + 1024 + 2048;
+constexpr int kM2ScCols = 24;
+constexpr int kM2Smem = kM2Stages * kM2Stage + 1024;
+static_assert(kM2Stage % 1024 == 0, "stages are swizzle-aligned");
+static_assert(kM2Tok + kM2Stages * kM2ScCols <= (int)kMxTmem, "tensor memory");
+
+__device__ __forceinline__ void tma2_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void umma2_mxf4(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void tmem2_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// Arrives on the barrier at this offset in both CTAs once everything issued so far has been executed.
+__device__ __forceinline__ void umma2_commit(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+template <typename OT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kM2Threads, 1)
+k_mx4_gemm2(const MxGemmParams p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+            const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb) {
+    constexpr int S = kM2Stages;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t bars[2 * S + 2];
+    __shared__ uint32_t s_u32[2];
+    volatile uint32_t* ok_flag = &s_u32[1];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    const uint32_t ring = (smem_u32(raw) + 1023u) & ~1023u;
+    const uint32_t bar0 = smem_u32(bars);
+    auto full = [&](int s) { return bar0 + 8u * s; };              // used in the leader only
+    auto empty = [&](int s) { return bar0 + 8u * (S + s); };
+    const uint32_t acc_full = bar0 + 8u * (2 * S), acc_empty = bar0 + 8u * (2 * S + 1);      // the latter in the leader only
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        mbar_init(acc_full, 1);
+        mbar_init(acc_empty, 16);
+        *ok_flag = 1;
+        fence_barrier_init();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_u32[0])), "r"(kMxTmem) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();
+    tc_fence_after();
+    const uint32_t tmem = s_u32[0];
+    const uint32_t tmem_sc = tmem + kM2Tok;
+    grid_dep_launch();
+    grid_dep_wait();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if (warp == 0) {
+        if (elect_one()) {
+            int s = 0, issued = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int tile = pair; tile < p.tiles && ok; tile += pairs) {
+                const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
+                for (int ks = 0; ks < p.steps; ++ks) {
+                    if (!mbar_wait(empty(s), phase ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 5); ok = false; break; }
+                    const uint32_t at = ring + s * kM2Stage;
+                    const uint32_t bar = full(s) & 0xFEFFFFFFu;       // the leader's: the copies of both CTAs count there
+                    if (rank == 0) mbar_expect_tx(full(s), 2 * kM2Stage);
+                    tma2_load(at, &map_b, ks * 128, tf * 256 + (int)rank * 128, bar);
+                    tma2_load(at + kABytes, &map_a, ks * 128, tt * kM2Tok + (int)rank * 128, bar);
+                    // two scale tiles of this CTA's features, two of either half of the tokens
+                    tma2_load(at + 2 * kABytes, &map_sb, 0, (tf * 2 + (int)rank) * p.tiles_k + ks * 2, bar);
+                    tma2_load(at + 2 * kABytes + 1024, &map_sa, 0, tt * 2 * p.tiles_k + ks * 2, bar);
+                    tma2_load(at + 2 * kABytes + 2048, &map_sa, 0, (tt * 2 + 1) * p.tiles_k + ks * 2, bar);
+                    ++issued;
+                    if (++s == S) { s = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok && rank == 0) {       // leave no copy in flight behind, the peer's included
+                const int last = issued < S ? issued : S;
+                for (int i = issued - last; i < issued; ++i)
+                    for (uint32_t w = 0; w < kWaitLimit && !mbar_try_wait(full(i % S), (uint32_t)(i / S) & 1u); ++w) {}
+            }
+        }
+        __syncwarp();
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            int s = 0;
+            uint32_t phase = 0, use = 0;
+            bool ok = true;
+            for (int tile = pair; tile < p.tiles && ok; tile += pairs, use ^= 1u) {
+                if (!mbar_wait(acc_empty, use ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 6); break; }
+                tc_fence_after();
+                for (int ks = 0; ks < p.steps; ++ks) {
+                    if (!mbar_wait(full(s), phase, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 7); ok = false; break; }
+                    tc_fence_after();
+                    const uint32_t at = ring + s * kM2Stage, sc = tmem_sc + s * kM2ScCols;
+                    const int nsc = min(2, p.tiles_k - ks * 2);
+                    for (int q = 0; q < nsc; ++q) {
+                        tmem2_cp_scales(sc + q * 4, mx_scale_desc(at + 2 * kABytes + q * 512));
+                        tmem2_cp_scales(sc + 8 + q * 8, mx_scale_desc(at + 2 * kABytes + 1024 + q * 512));
+                        tmem2_cp_scales(sc + 8 + q * 8 + 4, mx_scale_desc(at + 2 * kABytes + 2048 + q * 512));
+                    }
+                    const uint64_t da = make_smem_desc(at), db = make_smem_desc(at + kABytes);
+                    const int chunks = min(4, (p.nb - ks * 8 + 1) >> 1);
+                    for (int c = 0; c < chunks; ++c)
+                        umma2_mxf4(tmem, da + c * 2, db + c * 2, mx_idesc2(kM2Tok) | mx_idesc_half(c & 1), sc + (c >> 1) * 4, sc + 8 + (c >> 1) * 8,
+                                   (ks > 0 || c > 0) ? 1u : 0u);
+                    umma2_commit(empty(s));
+                    if (++s == S) { s = 0; phase ^= 1u; }
+                }
+                if (ok) umma2_commit(acc_full);
+            }
+        }
+        __syncwarp();
+    } else {
+        const int quarter = warp & 3, half = (warp - 2) >> 2;
+        const uint32_t acc_empty_leader = cluster_addr(acc_empty, 0);
+        uint32_t use = 0;
+        for (int tile = pair; tile < p.tiles; tile += pairs, use ^= 1u) {
+            const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
+            const int f = tf * 256 + (int)rank * 128 + quarter * 32 + lane;
+            const float bias = f < p.n ? mx_bias(p, f) : 0.f;
+            if (!mbar_wait_warp(acc_full, use, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 8); break; }
+            tc_fence_after();
+            const uint32_t src = tmem + half * 128 + ((uint32_t)quarter << 21);
+            const int64_t t0 = (int64_t)tt * kM2Tok + half * 128;
+            const int cols = (int)(p.m - t0 < 128 ? p.m - t0 : 128);          // may be negative: nothing to store
+            OT* o = (OT*)p.out + t0 * p.n + f;
+            if constexpr (sizeof(OT) == 4) {
+                uint32_t r[128];
+#pragma unroll
+                for (int c = 0; c < 128; c += 16) tmem_ld16(src + c, *reinterpret_cast<uint32_t(*)[16]>(&r[c]));
+                tmem_ld_wait();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) cluster_arrive(acc_empty_leader);
+                if (f < p.n) {
+#pragma unroll
+                    for (int c = 0; c < 128; ++c)
+                        if (c < cols) o[(int64_t)c * p.n] = __uint_as_float(r[c]) + bias;
+                }
+            } else {
+                uint32_t r[64];          // tokens 2 i (low half) and 2 i + 1 of this lane's feature
+#pragma unroll
+                for (int c = 0; c < 128; c += 32) {
+                    uint32_t v[2][16];
+                    tmem_ld16(src + c, v[0]);
+                    tmem_ld16(src + c + 16, v[1]);
+                    tmem_ld_wait();
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        r[c / 2 + i] = pack2<OT>(__uint_as_float(v[i >> 3][(2 * i) & 15]) + bias, __uint_as_float(v[i >> 3][(2 * i + 1) & 15]) + bias);
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) cluster_arrive(acc_empty_leader);
+                if ((p.n & 1) == 0 && p.out_even) {
+                    const int odd = lane & 1;
+                    uint32_t* o2 = reinterpret_cast<uint32_t*>(o - odd + (int64_t)odd * p.n);
+                    const int64_t step = p.n;          // two rows, in words
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        const uint32_t q = __shfl_xor_sync(DC_FULL, r[i], 1);
+                        const uint32_t v = odd ? __byte_perm(q, r[i], 0x7632) : __byte_perm(r[i], q, 0x5410);
+                        if (2 * i + odd < cols && f < p.n) o2[i * step] = v;          // f and its neighbour are in or out together
+                    }
+                } else if (f < p.n) {
+                    uint16_t* o1 = reinterpret_cast<uint16_t*>(o);
+#pragma unroll
+                    for (int i = 0; i < 64; ++i) {
+                        if (2 * i < cols) o1[(int64_t)(2 * i) * p.n] = (uint16_t)r[i];
+                        if (2 * i + 1 < cols) o1[(int64_t)(2 * i + 1) * p.n] = (uint16_t)(r[i] >> 16);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync();          // no arrival, copy or MMA of the pair is outstanding behind this
+    tc_fence_after();
+    if (warp == 1) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kMxTmem) : "memory");
+}
+
 // Packed matrix [rows][16 nb] bytes as a tensor map, box 128 bytes x `box_rows`, 128-byte swizzle.
 typedef CUresult (*MxEncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int64_t row_bytes, int box_rows) {
+static MxEncodeFn mx_encoder() {
     static const MxEncodeFn fn = [] {
         void* ptr = nullptr;
         cudaDriverEntryPointQueryResult q;
@@ -254,6 +482,10 @@ static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int
         (void)cudaGetLastError();
         return (MxEncodeFn) nullptr;
     }();
+    return fn;
+}
+static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int64_t row_bytes, int box_rows) {
+    const MxEncodeFn fn = mx_encoder();
     if (fn == nullptr) return false;
     const cuuint64_t gdim[2] = {(cuuint64_t)row_bytes, (cuuint64_t)rows};
     const cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
@@ -261,6 +493,31 @@ static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int
     const cuuint32_t estride[2] = {1u, 1u};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// The scale tiles as rows of 128 words, a box of two consecutive tiles along k.
+static bool encode_mx4_scales(CUtensorMap* map, const void* scales, int64_t tiles) {
+    const MxEncodeFn fn = mx_encoder();
+    if (fn == nullptr) return false;
+    const cuuint64_t gdim[2] = {128u, (cuuint64_t)tiles};
+    const cuuint64_t gstride[1] = {512u};
+    const cuuint32_t box[2] = {128u, 2u};
+    const cuuint32_t estride[2] = {1u, 1u};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <typename OT>
+static int launch_mx4_pair(const MxGemmParams& p, const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& msa, const CUtensorMap& msb, cudaStream_t st) {
+    static PerDeviceOnce once;
+    bool* set = once.slot();
+    if (set == nullptr) return DC_ERR_LAUNCH;
+    if (!*set) {
+        if (cudaFuncSetAttribute(k_mx4_gemm2<OT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kM2Smem) != cudaSuccess) return check_launch();
+        *set = true;
+    }
+    const int pairs = sm_count() / 2 > 0 ? sm_count() / 2 : 1;
+    return launch_pdl(k_mx4_gemm2<OT>, dim3((unsigned)(2 * (p.tiles < pairs ? p.tiles : pairs))), dim3(kM2Threads), kM2Smem, st, p, ma, mb, msa, msb);
 }
 
 template <typename OT, int NT, bool SPLIT>
@@ -286,8 +543,7 @@ static int launch_mx4_nt(int nt, const MxGemmParams& p, int split, const CUtenso
         case 16: return launch_mx4<OT, 16, SPLIT>(p, split, ma, mb, st);
         case 32: return launch_mx4<OT, 32, SPLIT>(p, split, ma, mb, st);
         case 64: return launch_mx4<OT, 64, SPLIT>(p, split, ma, mb, st);
-        case 128: return launch_mx4<OT, 128, SPLIT>(p, split, ma, mb, st);
-        default: return launch_mx4<OT, 256, SPLIT>(p, split, ma, mb, st);
+        default: return launch_mx4<OT, 128, SPLIT>(p, split, ma, mb, st);
     }
 }
 template <typename OT>
@@ -313,24 +569,38 @@ extern "C" int dc_mx4_matmul(const void* a_data, const void* a_scales, const voi
     if (a_data == nullptr || a_scales == nullptr || b_data == nullptr || b_scales == nullptr || out == nullptr) return DC_ERR_NULL_POINTER;
     if (!aligned16(a_data) || !aligned16(a_scales) || !aligned16(b_data) || !aligned16(b_scales)) return DC_ERR_ALIGNMENT;
     const int sms = sm_count();
-    // columns of a tile: no more than the tokens need; beyond 128 the wide tile, if its tiles still fill the GPU (it reads half
-    // as many feature bytes per product)
-    int nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-    const int64_t tiles_f = divup64(n, 128);
-    if (m > 128 && tiles_f * divup64(m, 256) >= sms) nt = 256;
-    const int64_t tiles = tiles_f * divup64(m, nt);
-    if (tiles > 0x7fffffffLL) return DC_ERR_SHAPE;
     MxGemmParams p{};
     p.a_sc = (const uint8_t*)a_scales; p.b_sc = (const uint8_t*)b_scales; p.bias = bias; p.out = out;
     p.m = m; p.n = (int)n; p.nb = (int)mx4_blocks(k); p.tiles_k = (int)mx4_scale_tiles(k); p.steps = (int)divup64(k, kMxStep);
-    p.tiles_f = (int)tiles_f; p.tiles = (int)tiles;
     p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
+    p.out_even = (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+    cudaStream_t st = (cudaStream_t)stream;
+    alignas(64) CUtensorMap ma, mb;
+    // many tokens: pairs of SMs, where their tiles fill most of the GPU
+    const int64_t pair_tiles = divup64(n, 256) * divup64(m, kM2Tok);
+    const int64_t scale_tiles_max = divup64(m > n ? m : n, 128) * p.tiles_k;
+    if (m > 128 && pair_tiles * 4 >= sms && pair_tiles <= 0x7fffffffLL && scale_tiles_max + 256 <= 0x7fffffffLL) {
+        alignas(64) CUtensorMap msa, msb;
+        p.tiles_f = (int)divup64(n, 256); p.tiles = (int)pair_tiles;
+        if (!encode_mx4_map(&ma, a_data, m, (int64_t)p.nb * 16, 128) || !encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128) ||
+            !encode_mx4_scales(&msa, a_scales, divup64(m, 128) * p.tiles_k) || !encode_mx4_scales(&msb, b_scales, divup64(n, 128) * p.tiles_k))
+            return DC_ERR_UNSUPPORTED;
+        switch (out_dtype) {
+            case DC_F32: return launch_mx4_pair<float>(p, ma, mb, msa, msb, st);
+            case DC_F16: return launch_mx4_pair<__half>(p, ma, mb, msa, msb, st);
+            default: return launch_mx4_pair<__nv_bfloat16>(p, ma, mb, msa, msb, st);
+        }
+    }
+    // columns of a tile: no more than the tokens need
+    const int nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    const int64_t tiles_f = divup64(n, 128);
+    const int64_t tiles = tiles_f * divup64(m, nt);
+    if (tiles > 0x7fffffffLL) return DC_ERR_SHAPE;
+    p.tiles_f = (int)tiles_f; p.tiles = (int)tiles;
     // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each
     int split = 1;
     while (split < 8 && tiles * split * 2 <= sms && p.steps >= split * 2) split *= 2;
-    alignas(64) CUtensorMap ma, mb;
     if (!encode_mx4_map(&ma, a_data, m, (int64_t)p.nb * 16, nt) || !encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128)) return DC_ERR_UNSUPPORTED;
-    cudaStream_t st = (cudaStream_t)stream;
     switch (out_dtype) {
         case DC_F32: return launch_mx4_split<float>(nt, p, split, ma, mb, st);
         case DC_F16: return launch_mx4_split<__half>(nt, p, split, ma, mb, st);

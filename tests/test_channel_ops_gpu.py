@@ -349,7 +349,7 @@ def product_bound(a, b, k):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 32), (3, 8, 33), (16, 128, 64), (17, 130, 96), (32, 1000, 255), (33, 127, 256), (64, 1000, 1280), (65, 257, 257),
                                    (127, 129, 512), (128, 128, 1024), (129, 384, 300), (200, 100, 4096), (256, 256, 768), (300, 1001, 2000), (1, 4096, 4096), (2, 1000, 5000),
-                                   (700, 5000, 544), (1030, 4100, 288), (2500, 1900, 160)])
+                                   (700, 5000, 544), (1030, 4100, 288), (2500, 1900, 160), (2050, 4802, 1000), (2177, 4801, 96), (1500, 5120, 2080), (129, 12000, 320)])
 def test_matmul(m, n, k, dtype):
     g = gen(m + n + k)
     (qa, a), (qb, b) = packed((m, k), g), packed((n, k), g)
@@ -366,7 +366,7 @@ def test_matmul_is_exact_where_float32_is():
     """Whole numbers whose sums stay below 2^24: no rounding anywhere, so no bit may differ."""
     g = gen(12)
     grid = torch.tensor([0, 1, 2, 3, 4, 6, 8, 12, -1, -2, -3, -4, -6, -8, -12], device="cuda").float()
-    for m, n, k in ((5, 200, 700), (300, 260, 1000), (130, 4800, 512)):
+    for m, n, k in ((5, 200, 700), (300, 260, 1000), (130, 4800, 512), (2300, 2600, 700)):
         a = grid[torch.randint(15, (m, k), generator=g, device="cuda")]
         b = grid[torch.randint(15, (n, k), generator=g, device="cuda")]
         a[:, ::32], b[:, ::32] = 12.0, -12.0                                   # every block has the scale of 12: e2m1 x 2 holds the grid
@@ -375,7 +375,7 @@ def test_matmul_is_exact_where_float32_is():
         assert torch.equal(got.double(), a.double() @ b.double().t() + bias.double())
 
 
-@pytest.mark.parametrize("m", [4, 200])
+@pytest.mark.parametrize("m", [4, 200, 6000])
 def test_matmul_scales_far_apart_and_nan(m):
     g = gen(13)
     a, b = randn((m, 512), g), randn((300, 512), g)
@@ -393,7 +393,7 @@ def test_matmul_scales_far_apart_and_nan(m):
 
 def test_matmul_writes_nothing_else():
     g = gen(14)
-    for m, n, k in ((3, 100, 64), (130, 130, 300), (1000, 5000, 64)):
+    for m, n, k in ((3, 100, 64), (130, 130, 300), (1000, 5000, 64), (1001, 5001, 64)):
         (qa, _), (qb, _) = packed((m, k), g), packed((n, k), g)
         room = torch.full((2 * 4096 + m * n,), 5.0, device="cuda", dtype=F16)
         out = room[4096:4096 + m * n].view(m, n)
