@@ -389,19 +389,29 @@ def mx4_linear(x, weight, bias=None):
     4-bit products (dx and dw have the types of x and weight; differentiable once)."""
     op = "mx4_linear"
     rows, cols = _rows(x, op)
-    _code(x, op, "x")
+    code = _code(x, op, "x")
     packed = isinstance(weight, MX4Tensor)
     outs, k = weight.shape
     if k != cols:
         _fail(op, f"x has {cols} channels, the weight {k} columns")
+    _check_bias(op, bias, outs, x.device)
     grad = torch.is_grad_enabled() and (x.requires_grad or (bias is not None and bias.requires_grad) or (not packed and weight.requires_grad))
     if packed:
         if grad:
             _fail(op, "a packed weight is for inference: pass the unpacked weight to train, or call under torch.no_grad()")
-        return _unrows(mx4_matmul(_quantize(x, rows, cols, True, False)[0], weight, bias, x.dtype), x)
-    if not weight.is_contiguous() or weight.device != x.device or weight.dtype not in _CODES or outs == 0:
-        _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
-    _check_bias(op, bias, outs, x.device)
-    if grad:
-        return _MX4Linear.apply(x, weight, bias)
-    return _unrows(mx4_matmul(_quantize(x, rows, cols, True, False)[0], _quantize(weight, outs, cols, True, False)[0], bias, x.dtype), x)
+        if weight._data.device != x.device:
+            _fail(op, f"the weight must be on {x.device}")
+    else:
+        if not weight.is_contiguous() or weight.device != x.device or weight.dtype not in _CODES or outs == 0:
+            _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
+        if grad:
+            return _MX4Linear.apply(x, weight, bias)
+        weight = _quantize(weight, outs, cols, True, False)[0]
+    out = x.new_empty((rows, outs))
+    if rows > 0 and outs > 0:
+        with _device(x):
+            nbytes = lib.dc_mx4_linear_workspace_bytes(rows, outs, cols)
+        ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
+        _launch(op, lib.dc_mx4_linear, x, x.data_ptr(), *weight._ptrs(), _ptr(bias), out.data_ptr(), rows, outs, cols, code,
+                0 if bias is None else _CODES[bias.dtype], _ptr(ws), nbytes)
+    return _unrows(out, x)

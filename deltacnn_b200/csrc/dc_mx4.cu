@@ -16,40 +16,6 @@ namespace dc {
 
 int col_reduce(const float* partial, int n, int c, int64_t pitch, void* o0, void* o1, int dtype, cudaStream_t st);   // dc_norm.cu
 
-// Eight values of a row starting at column col (cols in all); zeros behind the end.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const T* row, int64_t col, int64_t cols) {
-    if constexpr (VEC) {
-        constexpr int N = 8 / VecTraits<T>::kVec;
-#pragma unroll
-        for (int k = 0; k < N; ++k) {
-            Pack<T, VecTraits<T>::kVec> p;
-            if (col + k * VecTraits<T>::kVec < cols) p.load(row + col + k * VecTraits<T>::kVec);
-            else p.zero();
-#pragma unroll
-            for (int i = 0; i < VecTraits<T>::kVec; ++i) v[k * VecTraits<T>::kVec + i] = p.get(i);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? to_f<T>(row[col + i]) : 0.f;
-    }
-}
-
-__device__ __forceinline__ uint32_t amax8_bits(const float (&v)[8]) {
-    uint32_t m = 0;      // as integers: a NaN is above every number, so it is not lost
-#pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    return m;
-}
-__device__ __forceinline__ uint32_t encode_scaled(const float (&v)[8], uint32_t s) {
-    if (s == 255u) return 0u;
-    const float f = mx4_factor(s);
-    float u[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = v[i] * f;
-    return mx4_encode8(u);
-}
-
 constexpr int kMxChunk = 256;          // values of a row that a warp takes at once (eight blocks)
 constexpr int kMxAhead = 4;            // chunks of a row whose reads a warp has in flight
 

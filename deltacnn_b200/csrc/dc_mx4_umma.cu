@@ -10,7 +10,10 @@
 // A step is 256 values of k: one TMA box per operand (rows of 128 bytes, 128-byte swizzle) and the step's two 512-byte scale
 // tiles per 128 rows, in one contiguous copy each; tcgen05.cp spreads a scale tile over the four lane quarters of tensor
 // memory. Roles: one thread issues the copies, one the scale copies and MMAs, four warps drain accumulators; persistent CTAs,
-// two accumulators where the tensor memory holds them.
+// two accumulators.
+//
+// dc_mx4_linear on few tokens packs them in the same kernel: eight warps, one per stage, quantise a step's rows straight into
+// it, in the swizzled layout that the TMA would have written, and arrive on the stage's barrier beside the copies.
 //
 // Bound: many tokens, the tensor core and the shared memory that feeds it; few tokens, the weight's bytes. Then the tiles
 // do not fill the GPU, and the CTAs of a cluster share a tile along k: each leaves its float32 sums in its own shared
@@ -24,25 +27,26 @@ namespace dc {
 __device__ int g_mx4_error = 0;
 
 constexpr int kMxThreads = 192;            // TMA warp, MMA warp, four epilogue warps
+constexpr int kMxQuantThreads = 320;       // with the tokens quantised on the way: eight warps for that, four of them drain
+constexpr int kMxQuantRows = 4;            // tokens that dc_mx4_linear packs inside the product
 constexpr int kMxStep = 256;               // values of k per step: one 128-byte row
 constexpr uint32_t kMxTmem = 512;
 
 // Columns (tokens) per tile -> stages of the ring, accumulators, tensor memory columns of a stage's scales.
 template <int NT> struct MxCfg {
-    static constexpr int kRowTiles = NT <= 128 ? 1 : 2;                 // 128-row scale tiles of the tokens
     static constexpr int kB = NT * 128;
-    static constexpr int kScB = kRowTiles * 1024;
-    static constexpr int kStage = kABytes + kB + 1024 + kScB;
-    static constexpr int kStages = NT == 256 ? 4 : NT == 128 ? 6 : 8;
-    static constexpr int kAcc = NT == 256 ? 1 : 2;
-    static constexpr int kScCols = 8 + 8 * kRowTiles;
+    static constexpr int kStage = kABytes + kB + 2048;
+    static constexpr int kStages = NT == 128 ? 6 : 8;
+    static constexpr int kScCols = 16;
     static constexpr int kSmem = kStages * kStage + 1024;
-    static_assert(kAcc * NT + kStages * kScCols <= (int)kMxTmem, "tensor memory");
+    static_assert(2 * NT + kStages * kScCols <= (int)kMxTmem, "tensor memory");
     static_assert(kSmem <= 227 * 1024 - 1024, "shared memory");
 };
 
 struct MxGemmParams {
     const uint8_t *a_sc, *b_sc;            // scales of the tokens, of the features
+    const void* x;                         // tokens in the result's type, where they are quantised on the way
+    int k, x_vec;                          // their width; rows allow 16-byte reads
     const void* bias;
     void* out;
     int64_t m;
@@ -50,6 +54,12 @@ struct MxGemmParams {
     int tiles_f, tiles;                    // feature tiles, all tiles
     int bias_dtype, out_dtype;
     int out_even;                          // out is 4-byte aligned (16-bit results)
+};
+
+struct MxPlan {
+    bool pair, quant;
+    int nt, split;
+    int64_t tiles;
 };
 
 __device__ __forceinline__ uint64_t mx_scale_desc(uint32_t smem_addr) {
@@ -96,8 +106,8 @@ __device__ __forceinline__ float mx_bias(const MxGemmParams& p, int f) {
     return __bfloat162float(((const __nv_bfloat16*)p.bias)[f]);
 }
 
-template <typename OT, int NT, bool SPLIT>
-__global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+template <typename OT, int NT, bool SPLIT, bool QUANT>
+__global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4_gemm(const MxGemmParams p, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     using Cfg = MxCfg<NT>;
     constexpr int S = Cfg::kStages;
     extern __shared__ uint8_t raw[];
@@ -112,7 +122,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
     auto acc_full = [&](int a) { return bar0 + 8u * (2 * S + a); };
     auto acc_empty = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) { mbar_init(full(s), 1); mbar_init(empty(s), 1); }
+        for (int s = 0; s < S; ++s) { mbar_init(full(s), QUANT ? 2 : 1); mbar_init(empty(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 4); }
         *ok_flag = 1;
         fence_barrier_init();
@@ -122,7 +132,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_u32[0];
-    const uint32_t tmem_sc = tmem + Cfg::kAcc * NT;
+    const uint32_t tmem_sc = tmem + 2 * NT;
     grid_dep_launch();
     grid_dep_wait();
 
@@ -143,14 +153,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
                     if (!mbar_wait(empty(s), phase ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 1); ok = false; break; }
                     const uint32_t at = ring + s * Cfg::kStage;
                     const int nsc = min(2, p.tiles_k - ks * 2);
-                    const int rt = Cfg::kRowTiles == 1 ? 1 : min(2, (int)((p.m - (int64_t)tt * NT + 127) >> 7));
-                    mbar_expect_tx(full(s), (uint32_t)(kABytes + Cfg::kB + nsc * 512 * (1 + rt)));
+                    mbar_expect_tx(full(s), (uint32_t)(kABytes + nsc * 512 + (QUANT ? 0 : Cfg::kB + nsc * 512)));
                     tma_load_rows(at, &map_b, ks * 128, tf * 128, full(s));
-                    tma_load_rows(at + kABytes, &map_a, ks * 128, tt * NT, full(s));
                     bulk_g2s(at + kABytes + Cfg::kB, p.b_sc + ((int64_t)tf * p.tiles_k + ks * 2) * 512, (uint32_t)nsc * 512u, full(s));
-                    for (int q = 0; q < rt; ++q)
-                        bulk_g2s(at + kABytes + Cfg::kB + 1024 + q * 1024,
-                                 p.a_sc + (((int64_t)tt * NT / 128 + q) * p.tiles_k + ks * 2) * 512, (uint32_t)nsc * 512u, full(s));
+                    if constexpr (!QUANT) {
+                        tma_load_rows(at + kABytes, &map_a, ks * 128, tt * NT, full(s));
+                        bulk_g2s(at + kABytes + Cfg::kB + 1024, p.a_sc + ((int64_t)tt * NT / 128 * p.tiles_k + ks * 2) * 512, (uint32_t)nsc * 512u, full(s));
+                    }
                     ++issued;
                     if (++s == S) { s = 0; phase ^= 1u; }
                 }
@@ -169,7 +178,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
             uint32_t phase = 0;
             bool ok = true;
             for (int tile = blockIdx.x; tile < p.tiles && ok; tile += gridDim.x, ++it) {
-                const int a = Cfg::kAcc == 2 ? it & 1 : 0, use = Cfg::kAcc == 2 ? it >> 1 : it;
+                const int a = it & 1, use = it >> 1;
                 if (!mbar_wait(acc_empty(a), (uint32_t)(use & 1) ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 2); break; }
                 tc_fence_after();
                 const uint32_t d = tmem + a * NT;
@@ -180,15 +189,13 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
                     const int nsc = min(2, p.tiles_k - ks * 2);
                     for (int q = 0; q < nsc; ++q) {
                         tmem_cp_scales(sc + q * 4, mx_scale_desc(at + kABytes + Cfg::kB + q * 512));
-#pragma unroll
-                        for (int t = 0; t < Cfg::kRowTiles; ++t)
-                            tmem_cp_scales(sc + 8 + (q * Cfg::kRowTiles + t) * 4, mx_scale_desc(at + kABytes + Cfg::kB + 1024 + t * 1024 + q * 512));
+                        tmem_cp_scales(sc + 8 + q * 4, mx_scale_desc(at + kABytes + Cfg::kB + 1024 + q * 512));
                     }
                     const uint64_t da = make_smem_desc(at), db = make_smem_desc(at + kABytes);
                     const int chunks = min(4, (p.nb - ks * 8 + 1) >> 1);          // 64 values of k each
                     for (int c = 0; c < chunks; ++c)
                         umma_mxf4(d, da + c * 2, db + c * 2, mx_idesc(NT) | mx_idesc_half(c & 1), sc + (c >> 1) * 4,
-                                  sc + 8 + (c >> 1) * 4 * Cfg::kRowTiles, (ks > k_lo || c > 0) ? 1u : 0u);
+                                  sc + 8 + (c >> 1) * 4, (ks > k_lo || c > 0) ? 1u : 0u);
                     umma_commit(empty(s));
                     if (++s == S) { s = 0; phase ^= 1u; }
                 }
@@ -200,9 +207,59 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
         // ---- accumulators out: warp w owns lanes 32 (w % 4) .. + 31, a lane is a feature
         const int quarter = warp & 3;
         int it = 0;
+        [[maybe_unused]] uint32_t seq = 0;         // steps so far
         for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, ++it) {
-            const int a = Cfg::kAcc == 2 ? it & 1 : 0, use = Cfg::kAcc == 2 ? it >> 1 : it;
+            const int a = it & 1, use = it >> 1;
             const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
+            if constexpr (QUANT) {
+                // Warp w packs the steps of stage w - 2, 256 values of every token, straight into the stage: a row at a time,
+                // four rows' reads in flight; eight values a lane, 16-byte pieces in the 128-byte swizzle, the scales of four
+                // blocks as one word of the scale tile.
+                static_assert(S == 8, "a stage per warp");
+                const int64_t row0 = (int64_t)tt * NT;
+                const int rows = (int)(p.m - row0 < NT ? p.m - row0 : NT);
+                uint8_t* codes = raw + (ring - smem_u32(raw)) + (warp - 2) * Cfg::kStage + kABytes;
+                bool ok = true;
+                for (int ks = k_lo; ks < k_hi; ++ks, ++seq) {
+                    if ((int)(seq & 7u) != warp - 2) continue;
+                    const int64_t col = (int64_t)ks * kMxStep + lane * 8;
+                    bool ready = false;
+                    for (int r0 = 0; r0 < rows; r0 += 4) {
+                        float v[4][8];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (r0 + j >= rows) break;
+                            const OT* row = (const OT*)p.x + (row0 + r0 + j) * p.k;
+                            if (p.x_vec) load8<OT, true>(v[j], row, col, p.k);
+                            else load8<OT, false>(v[j], row, col, p.k);
+                        }
+                        if (!ready) {
+                            if (!mbar_wait_warp(empty(warp - 2), ((uint32_t)(seq >> 3) & 1u) ^ 1u, ok_flag)) { ok = false; break; }
+                            ready = true;
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int r = r0 + j;
+                            if (r >= rows) break;
+                            uint32_t mx = amax8_bits(v[j]);
+                            mx = max(mx, __shfl_xor_sync(DC_FULL, mx, 1));
+                            mx = max(mx, __shfl_xor_sync(DC_FULL, mx, 2));
+                            const uint32_t sb = mx4_scale_byte(mx);
+                            *reinterpret_cast<uint32_t*>(codes + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = encode_scaled(v[j], sb);
+                            uint32_t word = sb << (8 * ((lane >> 2) & 3));
+                            word |= __shfl_xor_sync(DC_FULL, word, 4);
+                            word |= __shfl_xor_sync(DC_FULL, word, 8);
+                            if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(codes + Cfg::kB + 1024 + (lane >> 4) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
+                        }
+                    }
+                    if (!ok) { *ok_flag = 0; atomicExch(&g_mx4_error, 9); break; }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(full(warp - 2));
+                }
+                if (!ok) break;
+                if (warp >= 6) continue;
+            }
             const int f = tf * 128 + quarter * 32 + lane;
             const float bias = f < p.n && !SPLIT ? mx_bias(p, f) : 0.f;
             if (!mbar_wait_warp(acc_full(a), (uint32_t)(use & 1), ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 4); break; }
@@ -237,7 +294,7 @@ __global__ void __launch_bounds__(kMxThreads, 1) k_mx4_gemm(const MxGemmParams p
         const int64_t t0 = (int64_t)tt * NT;
         const int cols = (int)(p.m - t0 < NT ? p.m - t0 : NT);
         const bool good = *ok_flag != 0;
-        for (int i = threadIdx.x; i < 128 * ((cols - rank + ranks - 1) / ranks); i += kMxThreads) {
+        for (int i = threadIdx.x; i < 128 * ((cols - rank + ranks - 1) / ranks); i += blockDim.x) {
             const int col = rank + (i >> 7) * ranks, f = tf * 128 + (i & 127);
             if (f >= p.n || !good) continue;
             float v = 0.f;
@@ -521,7 +578,7 @@ static int launch_mx4_pair(const MxGemmParams& p, const CUtensorMap& ma, const C
     return launch_pdl(k_mx4_gemm2<OT>, dim3((unsigned)(2 * (p.tiles < pairs ? p.tiles : pairs))), dim3(kM2Threads), kM2Smem, st, p, ma, mb, msa, msb);
 }
 
-template <typename OT, int NT, bool SPLIT>
+template <typename OT, int NT, bool SPLIT, bool QUANT>
 static int launch_mx4(const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
     // a cluster's CTAs wait for one another: they take an SM's whole shared memory, so that no other kernel's CTA that waits in
     // a cluster too can hold tensor memory on the same SM
@@ -530,26 +587,88 @@ static int launch_mx4(const MxGemmParams& p, int split, const CUtensorMap& ma, c
     bool* set = once.slot();
     if (set == nullptr) return DC_ERR_LAUNCH;
     if (!*set) {
-        if (cudaFuncSetAttribute(k_mx4_gemm<OT, NT, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return check_launch();
+        if (cudaFuncSetAttribute(k_mx4_gemm<OT, NT, SPLIT, QUANT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return check_launch();
         *set = true;
     }
     const int sms = sm_count();
     const dim3 grid((unsigned)(SPLIT ? p.tiles : p.tiles < sms ? p.tiles : sms), (unsigned)split);
-    return launch_pdl_cluster(k_mx4_gemm<OT, NT, SPLIT>, grid, dim3(kMxThreads), smem, st, split, p, ma, mb);
+    return launch_pdl_cluster(k_mx4_gemm<OT, NT, SPLIT, QUANT>, grid, dim3(QUANT ? kMxQuantThreads : kMxThreads), smem, st, split, p, ma, mb);
 }
 
 template <typename OT, bool SPLIT>
 static int launch_mx4_nt(int nt, const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
+    if (p.x != nullptr) return launch_mx4<OT, 16, SPLIT, true>(p, split, ma, mb, st);      // kMxQuantRows <= 16
     switch (nt) {
-        case 16: return launch_mx4<OT, 16, SPLIT>(p, split, ma, mb, st);
-        case 32: return launch_mx4<OT, 32, SPLIT>(p, split, ma, mb, st);
-        case 64: return launch_mx4<OT, 64, SPLIT>(p, split, ma, mb, st);
-        default: return launch_mx4<OT, 128, SPLIT>(p, split, ma, mb, st);
+        case 16: return launch_mx4<OT, 16, SPLIT, false>(p, split, ma, mb, st);
+        case 32: return launch_mx4<OT, 32, SPLIT, false>(p, split, ma, mb, st);
+        case 64: return launch_mx4<OT, 64, SPLIT, false>(p, split, ma, mb, st);
+        default: return launch_mx4<OT, 128, SPLIT, false>(p, split, ma, mb, st);
     }
 }
 template <typename OT>
-static int launch_mx4_split(int nt, const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
-    return split > 1 ? launch_mx4_nt<OT, true>(nt, p, split, ma, mb, st) : launch_mx4_nt<OT, false>(nt, p, 1, ma, mb, st);
+static int launch_mx4_split(const MxPlan& pl, const MxGemmParams& p, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
+    return pl.split > 1 ? launch_mx4_nt<OT, true>(pl.nt, p, pl.split, ma, mb, st) : launch_mx4_nt<OT, false>(pl.nt, p, 1, ma, mb, st);
+}
+
+// How a product is cut: pairs of SMs, or tiles of nt tokens shared along k by `split` CTAs; quant: dc_mx4_linear quantises the
+// tokens inside the product.
+static MxPlan mx4_plan(int64_t m, int64_t n, int64_t k) {
+    const int sms = sm_count();
+    const int steps = (int)divup64(k, kMxStep);
+    const int64_t tiles_k = mx4_scale_tiles(k);
+    MxPlan pl{};
+    pl.split = 1;
+    // many tokens: pairs of SMs, where their tiles fill at least half of the GPU
+    const int64_t pair_tiles = divup64(n, 256) * divup64(m, kM2Tok);
+    pl.pair = m > 128 && pair_tiles * 4 >= sms && pair_tiles <= 0x7fffffffLL && (divup64(m > n ? m : n, 128) + 2) * tiles_k <= 0x7fffffffLL;
+    if (pl.pair) { pl.tiles = pair_tiles; return pl; }
+    // columns of a tile: no more than the tokens need
+    pl.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
+    pl.tiles = divup64(n, 128) * divup64(m, pl.nt);
+    // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each
+    while (pl.split < 8 && pl.tiles * pl.split * 2 <= sms && steps >= pl.split * 2) pl.split *= 2;
+    // Quantising inside makes every feature tile read the tokens unpacked and wait for a row's 1 us of latency per four rows and
+    // step: 4096 -> 14336 takes 9.7 us for one token (2.6 + 9.4 us with a launch of its own) 11.5 us for four, 15.6 us for eight (2.7 + 9.6).
+    pl.quant = m <= kMxQuantRows;
+    return pl;
+}
+
+// x != NULL: the tokens unpacked, in the result's type; a_data / a_scales otherwise.
+static int mx4_product(const void* x, const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m,
+                       int64_t n, int64_t k, int bias_dtype, int out_dtype, cudaStream_t st) {
+    const MxPlan pl = mx4_plan(m, n, k);
+    if (pl.tiles > 0x7fffffffLL) return DC_ERR_SHAPE;
+    MxGemmParams p{};
+    p.a_sc = (const uint8_t*)a_scales; p.b_sc = (const uint8_t*)b_scales; p.bias = bias; p.out = out;
+    p.m = m; p.n = (int)n; p.nb = (int)mx4_blocks(k); p.tiles_k = (int)mx4_scale_tiles(k); p.steps = (int)divup64(k, kMxStep);
+    p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
+    p.out_even = (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+    p.tiles_f = (int)divup64(n, pl.pair ? 256 : 128);
+    p.tiles = (int)pl.tiles;
+    p.x = x; p.k = (int)k;
+    p.x_vec = aligned16(x) && k % (out_dtype == DC_F32 ? 4 : 8) == 0;
+    alignas(64) CUtensorMap ma, mb;
+    if (!encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128)) return DC_ERR_UNSUPPORTED;
+    if (x != nullptr) ma = mb;          // not read
+    else if (!encode_mx4_map(&ma, a_data, m, (int64_t)p.nb * 16, pl.pair ? kM2Tok / 2 : pl.nt)) return DC_ERR_UNSUPPORTED;
+    if (pl.pair) {
+        alignas(64) CUtensorMap msa, msb;
+        if (!encode_mx4_scales(&msa, a_scales, divup64(m, 128) * p.tiles_k) || !encode_mx4_scales(&msb, b_scales, divup64(n, 128) * p.tiles_k)) return DC_ERR_UNSUPPORTED;
+        switch (out_dtype) {
+            case DC_F32: return launch_mx4_pair<float>(p, ma, mb, msa, msb, st);
+            case DC_F16: return launch_mx4_pair<__half>(p, ma, mb, msa, msb, st);
+            default: return launch_mx4_pair<__nv_bfloat16>(p, ma, mb, msa, msb, st);
+        }
+    }
+    switch (out_dtype) {
+        case DC_F32: return launch_mx4_split<float>(pl, p, ma, mb, st);
+        case DC_F16: return launch_mx4_split<__half>(pl, p, ma, mb, st);
+        default: return launch_mx4_split<__nv_bfloat16>(pl, p, ma, mb, st);
+    }
+}
+
+static bool mx4_sizes_ok(int64_t m, int64_t n, int64_t k) {
+    return m >= 0 && n >= 0 && k > 0 && m <= 0x7fffff00LL && n <= 0x7fffff00LL && k <= 0x7fffff00LL;
 }
 
 int mx4_error_code() {
@@ -562,49 +681,39 @@ int mx4_error_code() {
 
 using namespace dc;
 
-extern "C" int dc_mx4_matmul(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m,
-                             int64_t n, int64_t k, int32_t bias_dtype, int32_t out_dtype, void* stream) {
-    if (m < 0 || n < 0 || k <= 0 || m > 0x7fffff00LL || n > 0x7fffff00LL || k > 0x7fffff00LL) return DC_ERR_SHAPE;
+extern "C" {
+
+int dc_mx4_matmul(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m, int64_t n,
+                  int64_t k, int32_t bias_dtype, int32_t out_dtype, void* stream) {
+    if (!mx4_sizes_ok(m, n, k)) return DC_ERR_SHAPE;
     if (out_dtype < DC_F32 || out_dtype > DC_BF16 || (bias != nullptr && (bias_dtype < DC_F32 || bias_dtype > DC_BF16))) return DC_ERR_DTYPE;
     if (m == 0 || n == 0) return DC_OK;
     if (a_data == nullptr || a_scales == nullptr || b_data == nullptr || b_scales == nullptr || out == nullptr) return DC_ERR_NULL_POINTER;
     if (!aligned16(a_data) || !aligned16(a_scales) || !aligned16(b_data) || !aligned16(b_scales)) return DC_ERR_ALIGNMENT;
-    const int sms = sm_count();
-    MxGemmParams p{};
-    p.a_sc = (const uint8_t*)a_scales; p.b_sc = (const uint8_t*)b_scales; p.bias = bias; p.out = out;
-    p.m = m; p.n = (int)n; p.nb = (int)mx4_blocks(k); p.tiles_k = (int)mx4_scale_tiles(k); p.steps = (int)divup64(k, kMxStep);
-    p.bias_dtype = bias_dtype; p.out_dtype = out_dtype;
-    p.out_even = (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
-    cudaStream_t st = (cudaStream_t)stream;
-    alignas(64) CUtensorMap ma, mb;
-    // many tokens: pairs of SMs, where their tiles fill most of the GPU
-    const int64_t pair_tiles = divup64(n, 256) * divup64(m, kM2Tok);
-    const int64_t scale_tiles_max = divup64(m > n ? m : n, 128) * p.tiles_k;
-    if (m > 128 && pair_tiles * 4 >= sms && pair_tiles <= 0x7fffffffLL && scale_tiles_max + 256 <= 0x7fffffffLL) {
-        alignas(64) CUtensorMap msa, msb;
-        p.tiles_f = (int)divup64(n, 256); p.tiles = (int)pair_tiles;
-        if (!encode_mx4_map(&ma, a_data, m, (int64_t)p.nb * 16, 128) || !encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128) ||
-            !encode_mx4_scales(&msa, a_scales, divup64(m, 128) * p.tiles_k) || !encode_mx4_scales(&msb, b_scales, divup64(n, 128) * p.tiles_k))
-            return DC_ERR_UNSUPPORTED;
-        switch (out_dtype) {
-            case DC_F32: return launch_mx4_pair<float>(p, ma, mb, msa, msb, st);
-            case DC_F16: return launch_mx4_pair<__half>(p, ma, mb, msa, msb, st);
-            default: return launch_mx4_pair<__nv_bfloat16>(p, ma, mb, msa, msb, st);
-        }
-    }
-    // columns of a tile: no more than the tokens need
-    const int nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
-    const int64_t tiles_f = divup64(n, 128);
-    const int64_t tiles = tiles_f * divup64(m, nt);
-    if (tiles > 0x7fffffffLL) return DC_ERR_SHAPE;
-    p.tiles_f = (int)tiles_f; p.tiles = (int)tiles;
-    // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each
-    int split = 1;
-    while (split < 8 && tiles * split * 2 <= sms && p.steps >= split * 2) split *= 2;
-    if (!encode_mx4_map(&ma, a_data, m, (int64_t)p.nb * 16, nt) || !encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128)) return DC_ERR_UNSUPPORTED;
-    switch (out_dtype) {
-        case DC_F32: return launch_mx4_split<float>(nt, p, split, ma, mb, st);
-        case DC_F16: return launch_mx4_split<__half>(nt, p, split, ma, mb, st);
-        default: return launch_mx4_split<__nv_bfloat16>(nt, p, split, ma, mb, st);
-    }
+    return mx4_product(nullptr, a_data, a_scales, b_data, b_scales, bias, out, m, n, k, bias_dtype, out_dtype, (cudaStream_t)stream);
 }
+
+size_t dc_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!mx4_sizes_ok(m, n, k) || m == 0 || n == 0 || mx4_plan(m, n, k).quant) return 0;
+    return dc_mx4_data_bytes(m, k) + dc_mx4_scale_bytes(m, k);
+}
+
+int dc_mx4_linear(const void* x, const void* w_data, const void* w_scales, const void* bias, void* out, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                  int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!mx4_sizes_ok(m, n, k)) return DC_ERR_SHAPE;
+    if (dtype < DC_F32 || dtype > DC_BF16 || (bias != nullptr && (bias_dtype < DC_F32 || bias_dtype > DC_BF16))) return DC_ERR_DTYPE;
+    if (m == 0 || n == 0) return DC_OK;
+    if (x == nullptr || w_data == nullptr || w_scales == nullptr || out == nullptr) return DC_ERR_NULL_POINTER;
+    if (!aligned16(w_data) || !aligned16(w_scales) || !aligned16(workspace)) return DC_ERR_ALIGNMENT;
+    if (mx4_plan(m, n, k).quant)
+        return mx4_product(x, nullptr, nullptr, w_data, w_scales, bias, out, m, n, k, bias_dtype, dtype, (cudaStream_t)stream);
+    if (workspace == nullptr) return DC_ERR_NULL_POINTER;
+    const size_t data = dc_mx4_data_bytes(m, k);
+    if (workspace_bytes < data + dc_mx4_scale_bytes(m, k)) return DC_ERR_WORKSPACE;
+    uint8_t* ws = (uint8_t*)workspace;
+    const int rc = dc_mx4_quantize(x, ws, ws + data, nullptr, nullptr, nullptr, m, k, dtype, 0, nullptr, 0, stream);
+    if (rc != DC_OK) return rc;
+    return mx4_product(nullptr, ws, ws + data, w_data, w_scales, bias, out, m, n, k, bias_dtype, dtype, (cudaStream_t)stream);
+}
+
+}  // extern "C"

@@ -379,6 +379,13 @@ int dc_mx4_dequantize(const void* data, const void* scales, void* out, int64_t r
 int dc_mx4_matmul(const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m,
                   int64_t n, int64_t k, int32_t bias_dtype, int32_t out_dtype, void* stream);
 
+/* dc_mx4_quantize of x (m x k in dtype, contiguous) followed by dc_mx4_matmul with a packed weight (n x k), the result in
+ * dtype; few rows of x are packed inside the product (one launch). workspace: dc_mx4_linear_workspace_bytes of device
+ * memory, 16-byte aligned, only meaningful during the call (0 bytes, NULL: none wanted). Same bits as the two calls. */
+size_t dc_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int dc_mx4_linear(const void* x, const void* w_data, const void* w_scales, const void* bias, void* out, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                  int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

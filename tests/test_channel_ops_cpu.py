@@ -69,6 +69,13 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.dc_mx4_matmul(p, p, p, p, None, None, 1, 1, 32, 0, f32, None) == null
     assert lib.dc_mx4_matmul(p + 4, p, p, p, None, p, 1, 1, 32, 0, f32, None) == align
     assert lib.dc_mx4_matmul(None, None, None, None, None, None, 0, 5, 32, 0, f32, None) == 0
+    assert lib.dc_mx4_linear(p, p, p, None, p, 1, 1, 0, f32, f32, None, 0, None) == shape
+    assert lib.dc_mx4_linear(p, p, p, None, p, 1, 1, 32, 5, f32, None, 0, None) == dtype
+    assert lib.dc_mx4_linear(p, p, None, None, p, 1, 1, 32, f32, f32, None, 0, None) == null
+    assert lib.dc_mx4_linear(p, p + 8, p, None, p, 1, 1, 32, f32, f32, None, 0, None) == align
+    assert lib.dc_mx4_linear(p, p, p, None, p, 500, 500, 32, f32, f32, p, 64, None) == space
+    assert lib.dc_mx4_linear(p, p, p, None, p, 500, 500, 32, f32, f32, None, 0, None) == null
+    assert lib.dc_mx4_linear_workspace_bytes(1, 500, 64) == 0 and lib.dc_mx4_linear_workspace_bytes(500, 500, 64) == 500 * 32 + 4 * 512
     assert lib.dc_mx4_data_bytes(3, 33) == 3 * 32 and lib.dc_mx4_scale_bytes(129, 129) == 2 * 2 * 512
 
 

@@ -434,6 +434,25 @@ def test_linear_gradients(m, n, k, dtype):
     assert torch.equal(dc().mx4_linear(x, dc().mx4_quantize(w), b), y.detach())
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,n,k", [(1, 100, 40), (1, 14000, 1024), (2, 1000, 1281), (5, 130, 2052), (16, 1000, 4096), (17, 300, 31), (31, 5000, 500), (33, 1000, 1280), (64, 1000, 700),
+                                   (64, 9000, 2048), (65, 100, 260)])
+def test_linear_with_packed_weight_is_quantize_and_matmul(m, n, k, dtype):
+    """Few tokens are packed inside the product: the same bits as the two calls, hard values and odd widths included."""
+    g = gen(m + n)
+    x, b = randn((m, k), g, dtype, 2.0), randn((n,), g, dtype)
+    x[0, :32] = 0
+    x[-1, -1] = float("nan") if m > 2 else 7.0
+    qw = dc().mx4_quantize(randn((n, k), g))
+    got = dc().mx4_linear(x, qw, b)
+    want = dc().mx4_matmul(dc().mx4_quantize(x), qw, b, dtype)
+    assert torch.equal(torch.nan_to_num(got, nan=77.0), torch.nan_to_num(want, nan=77.0))
+    if m > 2:
+        assert got[-1].isnan().all() and not got[:-1].isnan().any()
+    off = torch.empty(m * k + 1, device="cuda", dtype=dtype)[1:].view(m, k).copy_(x)         # rows off 16 bytes
+    assert torch.equal(torch.nan_to_num(dc().mx4_linear(off, qw, b), nan=77.0), torch.nan_to_num(want, nan=77.0))
+
+
 def test_linear_gradient_against_differences():
     """Where every rounding is exact (whole numbers that e2m1 holds) the layer is linear: differences are the gradient."""
     g = gen(17)
