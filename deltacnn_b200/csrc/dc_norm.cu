@@ -11,6 +11,7 @@
 // registers, and the next row is requested before the sums of the current one are taken, so the memory system always has a
 // row per team in flight. Rows whose width or address does not allow 16-byte accesses take the same code with single
 // elements; rows beyond the registers of a CTA are read three times by a plain loop.
+#include <type_traits>
 #include "dc_common.cuh"
 
 namespace dc {
@@ -45,7 +46,71 @@ template <typename T, int W> struct Frag {
     }
 };
 
+// Float32 values in twos (packed instructions, half the issue slots) for 16-byte packs, singly for single elements.
+struct V2 {
+    uint64_t v;
+    static __device__ __forceinline__ V2 make(float a, float b) { V2 r; asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b)); return r; }
+    static __device__ __forceinline__ V2 all(float a) { return make(a, a); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+    __device__ __forceinline__ float sum() const { float a, b; get(a, b); return a + b; }
+};
+__device__ __forceinline__ V2 add(V2 a, V2 b) { V2 r; asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ V2 mul(V2 a, V2 b) { V2 r; asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v)); return r; }
+__device__ __forceinline__ V2 fma(V2 a, V2 b, V2 c) { V2 r; asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v)); return r; }
+struct V1 {
+    float v;
+    static __device__ __forceinline__ V1 all(float a) { return V1{a}; }
+    __device__ __forceinline__ float sum() const { return v; }
+};
+__device__ __forceinline__ V1 add(V1 a, V1 b) { return V1{a.v + b.v}; }
+__device__ __forceinline__ V1 mul(V1 a, V1 b) { return V1{a.v * b.v}; }
+__device__ __forceinline__ V1 fma(V1 a, V1 b, V1 c) { return V1{fmaf(a.v, b.v, c.v)}; }
+
+// The values of a Frag in float32.
+template <int W> struct Vals {
+    using V = V2;
+    static constexpr int N = W / 2;
+    V2 v[N];
+    template <typename T> __device__ __forceinline__ void from(const Frag<T, W>& f) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = V2::make(f.s[2 * i], f.s[2 * i + 1]);
+            else if constexpr (std::is_same_v<T, __half>) {
+                const float2 h = __half22float2(reinterpret_cast<const __half2*>(f.s)[i]);
+                v[i] = V2::make(h.x, h.y);
+            } else {
+                const uint32_t u = reinterpret_cast<const uint32_t*>(f.s)[i];
+                v[i] = V2::make(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+            }
+        }
+    }
+    template <typename T> __device__ __forceinline__ void to(Frag<T, W>& f) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float a, b;
+            v[i].get(a, b);
+            if constexpr (sizeof(T) == 4) { f.s[2 * i] = a; f.s[2 * i + 1] = b; }
+            else if constexpr (std::is_same_v<T, __half>) reinterpret_cast<__half2*>(f.s)[i] = __floats2half2_rn(a, b);
+            else reinterpret_cast<__nv_bfloat162*>(f.s)[i] = __floats2bfloat162_rn(a, b);
+        }
+    }
+    __device__ __forceinline__ void put(float* p) const {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i].get(p[2 * i], p[2 * i + 1]);
+    }
+};
+template <> struct Vals<1> {
+    using V = V1;
+    static constexpr int N = 1;
+    V1 v[1];
+    template <typename T> __device__ __forceinline__ void from(const Frag<T, 1>& f) { v[0].v = to_f<T>(f.s[0]); }
+    template <typename T> __device__ __forceinline__ void to(Frag<T, 1>& f) const { f.s[0] = from_f<T>(v[0].v); }
+    __device__ __forceinline__ void put(float* p) const { p[0] = v[0].v; }
+};
+
 constexpr int kLnCta = 512;         // most threads of a CTA that holds a row: 128 registers a thread
+// Threads of a CTA at most for a row split into so many packs per thread.
+__host__ __device__ constexpr int row_threads(int w, int p) { return (w == 1 ? p > 8 : p > 1) ? kLnCta : 256; }
 constexpr int kMaxWarps = 32;
 
 // A row's team: g lanes of a warp (BLOCK false) or the whole CTA (BLOCK true).
@@ -80,12 +145,95 @@ __device__ __forceinline__ void load_row(Frag<T, W> (&v)[P], const T* p, int ran
     for (int k = 0; k < P; ++k)
         if (rank + k * size < nvec) v[k].load(p + (int64_t)(rank + k * size) * W);
 }
+// The rows ahead of the one at hand. 16-byte packs: every thread copies its own packs of the next rows of N arrays into its own
+// slots of a ring in shared memory (cp.async: no registers, no barrier, a wait for the thread's own copies). Three rows, or one
+// where a row alone is 64 KB or more of a CTA's shared memory. Single elements: the next row in registers.
+__host__ __device__ constexpr int rows_ahead(int packs) { return packs > 4 ? 1 : 3; }
+__device__ __forceinline__ void cp16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
+}
+// Packs behind the end of a row (rank + k size >= nvec) read as zeros, so that the arithmetic needs no branch for them.
+template <typename T, int W, int P, int N> struct RowPipe {
+    static constexpr bool kRing = W > 1;
+    static constexpr int kAhead = rows_ahead(N * P);
+    Frag<T, W> next[kRing ? 1 : N][kRing ? 1 : P];
+    uint8_t* mine;
+    const T* at[N];                        // this thread's first pack of the next row to ask for
+    int64_t step, left;                    // elements between the team's rows; rows it still has to ask for
+    int size, in, out;                     // slots to fill, to read
+    unsigned valid;                        // bit k: pack k is inside the row
+
+    __device__ __forceinline__ void ask() {
+        if (left > 0) {
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+#pragma unroll
+                for (int k = 0; k < P; ++k)
+                    if (valid >> k & 1u) {
+                        if constexpr (kRing) cp16(mine + (size_t)((in * N + n) * P + k) * blockDim.x * 16, at[n] + k * size * W);
+                        else next[n][k].load(at[n] + k * size * W);
+                    }
+                at[n] += step;
+            }
+        }
+        if constexpr (kRing) {
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            in = in == kAhead ? 0 : in + 1;
+        }
+        --left;
+    }
+    template <bool BLOCK>
+    __device__ __forceinline__ void start(const Team<BLOCK>& t, const void* const (&src)[N], int64_t rows, int c, int nvec, uint8_t* smem) {
+        mine = smem + threadIdx.x * 16;
+        size = t.size;
+        step = t.stride * c;
+        left = t.row < rows ? (rows - t.row + t.stride - 1) / t.stride : 0;
+        in = out = 0;
+        valid = 0;
+#pragma unroll
+        for (int k = 0; k < P; ++k) valid |= t.rank + k * t.size < nvec ? 1u << k : 0u;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            at[n] = (const T*)src[n] + t.row * c + t.rank * W;
+#pragma unroll
+            for (int k = 0; k < P; ++k) {
+                if constexpr (kRing) {
+                    if (!(valid >> k & 1u))
+                        for (int i = 0; i <= kAhead; ++i)
+                            *reinterpret_cast<uint4*>(mine + (size_t)((i * N + n) * P + k) * blockDim.x * 16) = make_uint4(0u, 0u, 0u, 0u);
+                } else {
+                    next[n][k].fill(0.f);
+                }
+            }
+        }
+        for (int i = 0; i < (kRing ? kAhead : 1); ++i) ask();
+    }
+    // The current row's packs, with the next request on its way.
+    __device__ __forceinline__ void take(Frag<T, W> (&v)[N][P]) {
+        if constexpr (kRing) {
+            ask();
+            asm volatile("cp.async.wait_group %0;" ::"n"(kAhead) : "memory");
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < P; ++k) v[n][k].load(reinterpret_cast<const T*>(mine + (size_t)((out * N + n) * P + k) * blockDim.x * 16));
+            out = out == kAhead ? 0 : out + 1;
+        } else {
+#pragma unroll
+            for (int n = 0; n < N; ++n)
+#pragma unroll
+                for (int k = 0; k < P; ++k) v[n][k] = next[n][k];
+            ask();
+        }
+    }
+};
+
 template <typename T, int W, int P>
 __device__ __forceinline__ void load_param(Frag<T, W> (&v)[P], const T* p, int rank, int size, int nvec, float neutral) {
 #pragma unroll
     for (int k = 0; k < P; ++k) {
-        if (p == nullptr) v[k].fill(neutral);
-        else if (rank + k * size < nvec) v[k].load(p + (rank + k * size) * W);
+        v[k].fill(rank + k * size < nvec ? neutral : 0.f);
+        if (p != nullptr && rank + k * size < nvec) v[k].load(p + (rank + k * size) * W);
     }
 }
 
@@ -102,72 +250,93 @@ struct LnParams {
 };
 
 template <typename T, typename WT, int W, int P, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? kLnCta : 256) k_ln_fwd(LnParams p) {
+__global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnParams p) {
     __shared__ float red[2][kMaxWarps];
+    extern __shared__ __align__(16) uint8_t ring[];
     grid_dep_launch();
     grid_dep_wait();
     const Team<BLOCK> t(p.g);
-    const T* x = (const T*)p.x;
-    T* y = (T*)p.y;
+    RowPipe<T, W, P, 1> pipe;
+    pipe.start(t, {p.x}, p.rows, p.c, p.nvec, ring);
+    T* y = (T*)p.y + t.row * p.c + t.rank * W;
     Frag<WT, W> w[P], b[P];
     load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
     load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
-    Frag<T, W> nx[P];
-    if (t.row < p.rows) load_row<T, W, P>(nx, x + t.row * p.c, t.rank, t.size, p.nvec);
+    using V = typename Vals<W>::V;
+    constexpr int N = Vals<W>::N;
     // lanes of a warp whose own rows have run out still take part in its shuffles
-    for (int64_t base = t.row - (BLOCK ? 0 : (threadIdx.x & 31) / p.g); base < p.rows; base += t.stride) {
-        const int64_t row = BLOCK ? base : base + (threadIdx.x & 31) / p.g;
-        const bool on = row < p.rows;
-        Frag<T, W> v[P];
+    for (int64_t base = t.row - (BLOCK ? 0 : (threadIdx.x & 31) / p.g), row = t.row; base < p.rows; base += t.stride, row += t.stride, y += pipe.step) {
+        const bool on = BLOCK || row < p.rows;
+        Frag<T, W> in[1][P];
+        pipe.take(in);
+        Vals<W> x[P];
+        V s = V::all(0.f), q = V::all(0.f);
 #pragma unroll
-        for (int k = 0; k < P; ++k) v[k] = nx[k];
-        if (row + t.stride < p.rows) load_row<T, W, P>(nx, x + (row + t.stride) * p.c, t.rank, t.size, p.nvec);
-        float s = 0.f;
+        for (int k = 0; k < P; ++k) {
+            x[k].from(in[0][k]);
 #pragma unroll
-        for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec)
-#pragma unroll
-                for (int i = 0; i < W; ++i) s += v[k].get(i);
-        const float m = t.sum(s, red[0]) * p.inv_c;
-        float q = 0.f;
-#pragma unroll
-        for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec)
-#pragma unroll
-                for (int i = 0; i < W; ++i) { const float d = v[k].get(i) - m; q += d * d; }
-        const float r = __frsqrt_rn(t.sum(q, red[1]) * p.inv_c + p.eps);
-        if (on) {
-#pragma unroll
-            for (int k = 0; k < P; ++k)
-                if (t.rank + k * t.size < p.nvec) {
-#pragma unroll
-                    for (int i = 0; i < W; ++i) v[k].set(i, (v[k].get(i) - m) * r * w[k].get(i) + b[k].get(i));
-                    v[k].store(y + row * p.c + (int64_t)(t.rank + k * t.size) * W);
-                }
-            if (t.rank == 0 && p.mean != nullptr) { p.mean[row] = m; p.rstd[row] = r; }
+            for (int i = 0; i < N; ++i) s = add(s, x[k].v[i]);
         }
+        const float m = t.sum(s.sum(), red[0]) * p.inv_c;
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            const V neg = V::all(pipe.valid >> k & 1u ? -m : 0.f);
+#pragma unroll
+            for (int i = 0; i < N; ++i) { x[k].v[i] = add(x[k].v[i], neg); q = fma(x[k].v[i], x[k].v[i], q); }
+        }
+        const float r = __frsqrt_rn(t.sum(q.sum(), red[1]) * p.inv_c + p.eps);
+        const V rr = V::all(r);
+#pragma unroll
+        for (int k = 0; k < P; ++k) {
+            Vals<W> ww, bb;
+            ww.from(w[k]);
+            bb.from(b[k]);
+#pragma unroll
+            for (int i = 0; i < N; ++i) x[k].v[i] = fma(mul(x[k].v[i], rr), ww.v[i], bb.v[i]);
+            x[k].to(in[0][k]);
+            if (on && (pipe.valid >> k & 1u)) in[0][k].store(y + k * t.size * W);
+        }
+        if (on && t.rank == 0 && p.mean != nullptr) { p.mean[row] = m; p.rstd[row] = r; }
     }
 }
 
-// Rows beyond the registers of a CTA: three reads (the second and third mostly from L2).
-template <typename T, typename WT>
+// Rows beyond the registers of a CTA: three reads, the second and third mostly from L2.
+template <typename T, typename WT, int W>
 __global__ void __launch_bounds__(1024) k_ln_fwd_long(LnParams p) {
     __shared__ float red[2][kMaxWarps];
     grid_dep_launch();
     grid_dep_wait();
     const Team<true> t(0);
-    const WT *w = (const WT*)p.w, *b = (const WT*)p.b;
     for (int64_t row = t.row; row < p.rows; row += t.stride) {
         const T* x = (const T*)p.x + row * p.c;
         T* y = (T*)p.y + row * p.c;
-        float s = 0.f;
-        for (int i = t.rank; i < p.c; i += t.size) s += to_f<T>(x[i]);
+        float s = 0.f, q = 0.f;
+        Frag<T, W> v;
+#pragma unroll 4
+        for (int i = t.rank; i < p.nvec; i += t.size) {
+            v.load(x + (int64_t)i * W);
+#pragma unroll
+            for (int j = 0; j < W; ++j) s += v.get(j);
+        }
         const float m = t.sum(s, red[0]) * p.inv_c;
-        float q = 0.f;
-        for (int i = t.rank; i < p.c; i += t.size) { const float d = to_f<T>(x[i]) - m; q += d * d; }
+#pragma unroll 4
+        for (int i = t.rank; i < p.nvec; i += t.size) {
+            v.load(x + (int64_t)i * W);
+#pragma unroll
+            for (int j = 0; j < W; ++j) { const float d = v.get(j) - m; q += d * d; }
+        }
         const float r = __frsqrt_rn(t.sum(q, red[1]) * p.inv_c + p.eps);
-        for (int i = t.rank; i < p.c; i += t.size)
-            y[i] = from_f<T>((to_f<T>(x[i]) - m) * r * (w != nullptr ? to_f<WT>(w[i]) : 1.f) + (b != nullptr ? to_f<WT>(b[i]) : 0.f));
+        for (int i = t.rank; i < p.nvec; i += t.size) {
+            Frag<WT, W> w, b;
+            w.fill(1.f);
+            b.fill(0.f);
+            v.load(x + (int64_t)i * W);
+            if (p.w != nullptr) w.load((const WT*)p.w + (int64_t)i * W);
+            if (p.b != nullptr) b.load((const WT*)p.b + (int64_t)i * W);
+#pragma unroll
+            for (int j = 0; j < W; ++j) v.set(j, (v.get(j) - m) * r * w.get(j) + b.get(j));
+            v.store(y + (int64_t)i * W);
+        }
         if (t.rank == 0 && p.mean != nullptr) { p.mean[row] = m; p.rstd[row] = r; }
     }
 }
@@ -185,90 +354,92 @@ struct LnBwdParams {
     float inv_c;
 };
 
+// CTAs of so many threads whose registers an SM holds: the accumulators alone are 2 P W registers.
+__host__ __device__ constexpr int bwd_ctas(int w, int p) { return row_threads(w, p) == kLnCta ? 1 : w == 1 && p > 2 ? 2 : 3; }
+
 template <typename T, typename WT, int W, int P, bool BLOCK>
-__global__ void __launch_bounds__(BLOCK ? kLnCta : 256) k_ln_bwd(LnBwdParams p) {
+__global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(LnBwdParams p) {
     __shared__ float red[2][2][kMaxWarps];
-    extern __shared__ float cols[];            // [2][c]: the CTA's column sums (teams within a CTA only)
+    extern __shared__ __align__(16) uint8_t ring[];      // the rows ahead; at the end [2][c] column sums of the CTA's teams
     grid_dep_launch();
     grid_dep_wait();
     const Team<BLOCK> t(p.g);
-    const T *x = (const T*)p.x, *dy = (const T*)p.dy;
-    T* dx = (T*)p.dx;
+    RowPipe<T, W, P, 2> pipe;
+    pipe.start(t, {p.x, p.dy}, p.rows, p.c, p.nvec, ring);
+    T* dx = (T*)p.dx + t.row * p.c + t.rank * W;
     Frag<WT, W> w[P];
     load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
-    float dw[P][W], db[P][W];
+    using V = typename Vals<W>::V;
+    constexpr int N = Vals<W>::N;
+    Vals<W> dw[P], db[P];
 #pragma unroll
     for (int k = 0; k < P; ++k)
 #pragma unroll
-        for (int i = 0; i < W; ++i) dw[k][i] = db[k][i] = 0.f;
-    // four packs a thread leave no registers for the next row; the CTA that holds such a row has 64 KB of it in flight anyway
-    constexpr bool kAhead = P * W < 32;
-    Frag<T, W> nx[P], nd[P];
+        for (int i = 0; i < N; ++i) dw[k].v[i] = db[k].v[i] = V::all(0.f);
     float nm = 0.f, nr = 0.f;
     [[maybe_unused]] int par = 0;
-    if (kAhead && t.row < p.rows) {
-        load_row<T, W, P>(nx, x + t.row * p.c, t.rank, t.size, p.nvec);
-        load_row<T, W, P>(nd, dy + t.row * p.c, t.rank, t.size, p.nvec);
-        nm = p.mean[t.row]; nr = p.rstd[t.row];
-    }
-    for (int64_t base = t.row - (BLOCK ? 0 : (threadIdx.x & 31) / p.g); base < p.rows; base += t.stride) {
-        const int64_t row = BLOCK ? base : base + (threadIdx.x & 31) / p.g;
-        const bool on = row < p.rows;
-        Frag<T, W> v[P], d[P];
-        if (!kAhead && on) {
-            load_row<T, W, P>(nx, x + row * p.c, t.rank, t.size, p.nvec);
-            load_row<T, W, P>(nd, dy + row * p.c, t.rank, t.size, p.nvec);
-            nm = p.mean[row]; nr = p.rstd[row];
-        }
+    if (t.row < p.rows) { nm = p.mean[t.row]; nr = p.rstd[t.row]; }
+    for (int64_t base = t.row - (BLOCK ? 0 : (threadIdx.x & 31) / p.g), row = t.row; base < p.rows; base += t.stride, row += t.stride, dx += pipe.step) {
+        const bool on = BLOCK || row < p.rows;
         const float m = nm, r = nr;
+        Frag<T, W> in[2][P];
+        pipe.take(in);
+        if (row + t.stride < p.rows) { nm = p.mean[row + t.stride]; nr = p.rstd[row + t.stride]; }
+        // n and g stay in registers between the two sums and dx, or are formed again where a thread has too many of them
+        constexpr bool kKeep = P * W <= 16 && P < 16;
+        Vals<W> n[kKeep ? P : 1], g[kKeep ? P : 1];
+        V sg = V::all(0.f), sgn = V::all(0.f);
+        const V rr = V::all(r);
+        auto form = [&](int k, Vals<W>& nn, Vals<W>& ee, Vals<W>& gg) {
+            Vals<W> ww;
+            nn.from(in[0][k]);
+            ee.from(in[1][k]);
+            ww.from(w[k]);
+            const V shift = V::all(pipe.valid >> k & 1u ? -m : 0.f);
 #pragma unroll
-        for (int k = 0; k < P; ++k) { v[k] = nx[k]; d[k] = nd[k]; }
-        if (kAhead && row + t.stride < p.rows) {
-            load_row<T, W, P>(nx, x + (row + t.stride) * p.c, t.rank, t.size, p.nvec);
-            load_row<T, W, P>(nd, dy + (row + t.stride) * p.c, t.rank, t.size, p.nvec);
-            nm = p.mean[row + t.stride]; nr = p.rstd[row + t.stride];
-        }
-        float sg = 0.f, sgn = 0.f;
+            for (int i = 0; i < N; ++i) { nn.v[i] = mul(add(nn.v[i], shift), rr); gg.v[i] = mul(ee.v[i], ww.v[i]); }
+        };
         if (on) {
 #pragma unroll
-            for (int k = 0; k < P; ++k)
-                if (t.rank + k * t.size < p.nvec)
+            for (int k = 0; k < P; ++k) {
+                Vals<W> nn, ee, gg;
+                form(k, nn, ee, gg);
 #pragma unroll
-                    for (int i = 0; i < W; ++i) {
-                        const float n = (v[k].get(i) - m) * r, e = d[k].get(i), g = e * w[k].get(i);
-                        dw[k][i] += e * n;
-                        db[k][i] += e;
-                        sg += g;
-                        sgn += g * n;
-                    }
+                for (int i = 0; i < N; ++i) {
+                    dw[k].v[i] = fma(ee.v[i], nn.v[i], dw[k].v[i]);
+                    db[k].v[i] = add(db[k].v[i], ee.v[i]);
+                    sg = add(sg, gg.v[i]);
+                    sgn = fma(gg.v[i], nn.v[i], sgn);
+                }
+                if constexpr (kKeep) { n[k] = nn; g[k] = gg; }
+            }
         }
-        if (dx != nullptr) {
+        if (p.dx != nullptr) {
             float a, c;
             if constexpr (BLOCK) {             // both sums behind one barrier
                 const int lane = threadIdx.x & 31;
                 par ^= 1;
-                sg = group_sum(sg, 32);
-                sgn = group_sum(sgn, 32);
-                if (lane == 0) { red[par][0][threadIdx.x >> 5] = sg; red[par][1][threadIdx.x >> 5] = sgn; }
+                a = group_sum(sg.sum(), 32);
+                c = group_sum(sgn.sum(), 32);
+                if (lane == 0) { red[par][0][threadIdx.x >> 5] = a; red[par][1][threadIdx.x >> 5] = c; }
                 __syncthreads();
-                const bool in = lane < (int)(blockDim.x >> 5);
-                a = group_sum(in ? red[par][0][lane] : 0.f, 32) * p.inv_c;
-                c = group_sum(in ? red[par][1][lane] : 0.f, 32) * p.inv_c;
+                const bool in_cta = lane < (int)(blockDim.x >> 5);
+                a = group_sum(in_cta ? red[par][0][lane] : 0.f, 32) * p.inv_c;
+                c = group_sum(in_cta ? red[par][1][lane] : 0.f, 32) * p.inv_c;
             } else {
-                a = group_sum(sg, t.size) * p.inv_c;
-                c = group_sum(sgn, t.size) * p.inv_c;
+                a = group_sum(sg.sum(), t.size) * p.inv_c;
+                c = group_sum(sgn.sum(), t.size) * p.inv_c;
             }
-            if (on) {
+            const V na = V::all(-a), nc = V::all(-c);
 #pragma unroll
-                for (int k = 0; k < P; ++k)
-                    if (t.rank + k * t.size < p.nvec) {
+            for (int k = 0; k < P; ++k) {
+                Vals<W> nn, ee, gg;
+                if constexpr (kKeep) { nn = n[k]; gg = g[k]; }
+                else form(k, nn, ee, gg);
 #pragma unroll
-                        for (int i = 0; i < W; ++i) {
-                            const float n = (v[k].get(i) - m) * r;
-                            d[k].set(i, r * (d[k].get(i) * w[k].get(i) - a - n * c));
-                        }
-                        d[k].store(dx + row * p.c + (int64_t)(t.rank + k * t.size) * W);
-                    }
+                for (int i = 0; i < N; ++i) gg.v[i] = mul(rr, fma(nn.v[i], nc, add(gg.v[i], na)));
+                gg.to(in[0][k]);
+                if (on && (pipe.valid >> k & 1u)) in[0][k].store(dx + k * t.size * W);
             }
         }
     }
@@ -277,23 +448,30 @@ __global__ void __launch_bounds__(BLOCK ? kLnCta : 256) k_ln_bwd(LnBwdParams p) 
     if constexpr (BLOCK) {
 #pragma unroll
         for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec)
-#pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    const int col = (t.rank + k * t.size) * W + i;
-                    out[col] = dw[k][i];
-                    out[p.c + col] = db[k][i];
-                }
+            if (t.rank + k * t.size < p.nvec) {
+                const int col = (t.rank + k * t.size) * W;
+                Frag<float, W> f;
+                dw[k].put(f.s);
+                f.store(out + col);
+                db[k].put(f.s);
+                f.store(out + p.c + col);
+            }
     } else {
         // teams of a warp by shuffles, warps of the CTA one after the other: a fixed order
+        float* cols = reinterpret_cast<float*>(ring);
+        __syncthreads();                       // every thread has read its last row
+        float sums[2][P][W];
 #pragma unroll
-        for (int k = 0; k < P; ++k)
+        for (int k = 0; k < P; ++k) {
+            dw[k].put(sums[0][k]);
+            db[k].put(sums[1][k]);
 #pragma unroll
             for (int i = 0; i < W; ++i)
                 for (int o = p.g; o < 32; o <<= 1) {
-                    dw[k][i] += __shfl_xor_sync(DC_FULL, dw[k][i], o);
-                    db[k][i] += __shfl_xor_sync(DC_FULL, db[k][i], o);
+                    sums[0][k][i] += __shfl_xor_sync(DC_FULL, sums[0][k][i], o);
+                    sums[1][k][i] += __shfl_xor_sync(DC_FULL, sums[1][k][i], o);
                 }
+        }
         const int warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
         for (int q = 0; q < warps; ++q) {
             if (warp == q && (threadIdx.x & 31) < p.g) {
@@ -303,8 +481,8 @@ __global__ void __launch_bounds__(BLOCK ? kLnCta : 256) k_ln_bwd(LnBwdParams p) 
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
                             const int col = (t.rank + k * t.size) * W + i;
-                            cols[col] = (q == 0 ? 0.f : cols[col]) + dw[k][i];
-                            cols[p.c + col] = (q == 0 ? 0.f : cols[p.c + col]) + db[k][i];
+                            cols[col] = (q == 0 ? 0.f : cols[col]) + sums[0][k][i];
+                            cols[p.c + col] = (q == 0 ? 0.f : cols[p.c + col]) + sums[1][k][i];
                         }
             }
             __syncthreads();
@@ -313,41 +491,68 @@ __global__ void __launch_bounds__(BLOCK ? kLnCta : 256) k_ln_bwd(LnBwdParams p) 
     }
 }
 
-// Long rows: the row's two sums in a first loop, dx in a second; the column sums go through the CTA's own slice of the
-// workspace, whose columns belong to one thread each.
-template <typename T, typename WT>
+// Long rows: the row's two sums in a first loop, dx in a second. A column belongs to one thread, which adds its sums in shared
+// memory, or in the CTA's own slice of the workspace where they do not fit there.
+constexpr int kLongSmem = 200 * 1024;
+template <typename T, typename WT, int W>
 __global__ void __launch_bounds__(1024) k_ln_bwd_long(LnBwdParams p) {
     __shared__ float red[2][kMaxWarps];
+    extern __shared__ __align__(16) uint8_t ring[];
     grid_dep_launch();
     grid_dep_wait();
     const Team<true> t(0);
-    const WT* w = (const WT*)p.w;
+    const bool inside = (size_t)p.c * 8 <= (size_t)kLongSmem;
     float* out = p.partial == nullptr ? nullptr : p.partial + (int64_t)blockIdx.x * 2 * p.c;
+    float* cols = inside ? reinterpret_cast<float*>(ring) : out;
     if (out != nullptr)
-        for (int i = t.rank; i < p.c; i += t.size) out[i] = out[p.c + i] = 0.f;
+        for (int i = t.rank; i < p.nvec; i += t.size)
+#pragma unroll
+            for (int j = 0; j < W; ++j) cols[(int64_t)i * W + j] = cols[p.c + (int64_t)i * W + j] = 0.f;
     for (int64_t row = t.row; row < p.rows; row += t.stride) {
         const T *x = (const T*)p.x + row * p.c, *dy = (const T*)p.dy + row * p.c;
         const float m = p.mean[row], r = p.rstd[row];
         float sg = 0.f, sgn = 0.f;
-        for (int i = t.rank; i < p.c; i += t.size) {
-            const float n = (to_f<T>(x[i]) - m) * r, e = to_f<T>(dy[i]), g = e * (w != nullptr ? to_f<WT>(w[i]) : 1.f);
-            if (out != nullptr) { out[i] += e * n; out[p.c + i] += e; }
-            sg += g;
-            sgn += g * n;
-        }
-        const float a = t.sum(sg, red[0]) * p.inv_c, c = t.sum(sgn, red[1]) * p.inv_c;
-        if (p.dx != nullptr) {
-            T* dx = (T*)p.dx + row * p.c;
-            for (int i = t.rank; i < p.c; i += t.size) {
-                const float n = (to_f<T>(x[i]) - m) * r;
-                dx[i] = from_f<T>(r * (to_f<T>(dy[i]) * (w != nullptr ? to_f<WT>(w[i]) : 1.f) - a - n * c));
+#pragma unroll 2
+        for (int i = t.rank; i < p.nvec; i += t.size) {
+            Frag<T, W> v, d;
+            Frag<WT, W> w;
+            w.fill(1.f);
+            v.load(x + (int64_t)i * W);
+            d.load(dy + (int64_t)i * W);
+            if (p.w != nullptr) w.load((const WT*)p.w + (int64_t)i * W);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const float n = (v.get(j) - m) * r, e = d.get(j), g = e * w.get(j);
+                if (out != nullptr) { cols[(int64_t)i * W + j] += e * n; cols[p.c + (int64_t)i * W + j] += e; }
+                sg += g;
+                sgn += g * n;
             }
         }
+        if (p.dx == nullptr) continue;
+        const float a = t.sum(sg, red[0]) * p.inv_c, c = t.sum(sgn, red[1]) * p.inv_c;
+        T* dx = (T*)p.dx + row * p.c;
+#pragma unroll 2
+        for (int i = t.rank; i < p.nvec; i += t.size) {
+            Frag<T, W> v, d;
+            Frag<WT, W> w;
+            w.fill(1.f);
+            v.load(x + (int64_t)i * W);
+            d.load(dy + (int64_t)i * W);
+            if (p.w != nullptr) w.load((const WT*)p.w + (int64_t)i * W);
+#pragma unroll
+            for (int j = 0; j < W; ++j) d.set(j, r * (d.get(j) * w.get(j) - a - (v.get(j) - m) * r * c));
+            d.store(dx + (int64_t)i * W);
+        }
     }
+    if (out != nullptr && inside)
+        for (int i = t.rank; i < p.nvec; i += t.size)
+#pragma unroll
+            for (int j = 0; j < W; ++j) { out[(int64_t)i * W + j] = cols[(int64_t)i * W + j]; out[p.c + (int64_t)i * W + j] = cols[p.c + (int64_t)i * W + j]; }
 }
 
-// Column sums of the CTAs' partial rows, in a fixed order: 32 columns per CTA, 16 threads share a column's rows.
-constexpr int kRedRows = 16;
+// Column sums of the CTAs' partial rows, in a fixed order: 32 columns per CTA, 32 threads share a column's rows and have four
+// of them in flight each (16 threads and one row at a time: 17 us for 296 x 4096, all of it latency).
+constexpr int kRedRows = 32;
 template <typename OT>
 __global__ void __launch_bounds__(32 * kRedRows) k_col_reduce(const float* __restrict__ partial, int n, int c, int64_t pitch, OT* __restrict__ o0,
                                                               OT* __restrict__ o1) {
@@ -357,17 +562,21 @@ __global__ void __launch_bounds__(32 * kRedRows) k_col_reduce(const float* __res
     const int col = blockIdx.x * 32 + threadIdx.x;
     OT* o = blockIdx.y == 0 ? o0 : o1;
     if (o == nullptr) return;
-    float a = 0.f;
-    if (col < c)
-        for (int i = threadIdx.y; i < n; i += kRedRows) a += partial[i * pitch + (int64_t)blockIdx.y * c + col];
-    s[threadIdx.y][threadIdx.x] = a;
-    __syncthreads();
-    if (threadIdx.y == 0 && col < c) {
-        a = 0.f;
+    float a[4] = {0.f, 0.f, 0.f, 0.f};
+    if (col < c) {
+        const float* src = partial + (int64_t)blockIdx.y * c + col;
+        for (int i = threadIdx.y; i < n; i += 4 * kRedRows) {
 #pragma unroll
-        for (int i = 0; i < kRedRows; ++i) a += s[i][threadIdx.x];
-        o[col] = from_f<OT>(a);
+            for (int j = 0; j < 4; ++j)
+                if (i + j * kRedRows < n) a[j] += src[(i + j * kRedRows) * pitch];
+        }
     }
+    s[threadIdx.y][threadIdx.x] = (a[0] + a[1]) + (a[2] + a[3]);
+    __syncthreads();
+    // a warp takes a column: its 32 sums by shuffles
+    const float v = group_sum(s[threadIdx.x][threadIdx.y], 32);
+    const int mine = blockIdx.x * 32 + threadIdx.y;
+    if (threadIdx.x == 0 && mine < c) o[mine] = from_f<OT>(v);
 }
 
 int col_reduce(const float* partial, int n, int c, int64_t pitch, void* o0, void* o1, int dtype, cudaStream_t st) {
@@ -391,27 +600,32 @@ struct LnDeltaParams {
     int64_t npix;
     int c, nvec, g;
     float thr, eps, inv_c;
+    int chunk;                 // pixels that a warp takes at once (teams of lanes)
 };
 
+// What a team reads of a pixel: the delta, the accumulated input, the accumulated output.
+template <typename T, int W, int P> struct DeltaPixel {
+    Frag<T, W> d[P], u[P], o[P];
+    __device__ __forceinline__ void load(const LnDeltaParams& p, int64_t px, int rank, int size) {
+        const int64_t off = px * p.c;
+        load_row<T, W, P>(d, (const T*)p.delta + off, rank, size, p.nvec);
+        load_row<T, W, P>(u, (const T*)p.prev_in + off, rank, size, p.nvec);
+        load_row<T, W, P>(o, (const T*)p.prev_out + off, rank, size, p.nvec);
+    }
+};
 // One pixel by its team; returns whether any channel's change is above the threshold (the same answer in the whole team).
 template <typename T, typename WT, int W, int P, bool BLOCK>
-__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, Frag<WT, W> (&w)[P], Frag<WT, W> (&b)[P],
-                                               float* red0, float* red1) {
+__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, DeltaPixel<T, W, P>& v, Frag<WT, W> (&w)[P],
+                                               Frag<WT, W> (&b)[P], float* red0, float* red1) {
     const int64_t off = px * p.c;
-    Frag<T, W> u[P], d[P], o[P];
-    if (on) {
-        load_row<T, W, P>(d, (const T*)p.delta + off, t.rank, t.size, p.nvec);
-        load_row<T, W, P>(u, (const T*)p.prev_in + off, t.rank, t.size, p.nvec);
-        load_row<T, W, P>(o, (const T*)p.prev_out + off, t.rank, t.size, p.nvec);
-    }
     float s = 0.f;
     if (on) {
 #pragma unroll
         for (int k = 0; k < P; ++k)
             if (t.rank + k * t.size < p.nvec) {
 #pragma unroll
-                for (int i = 0; i < W; ++i) { u[k].set(i, u[k].get(i) + d[k].get(i)); s += u[k].get(i); }
-                u[k].store((T*)p.prev_in + off + (int64_t)(t.rank + k * t.size) * W);
+                for (int i = 0; i < W; ++i) { v.u[k].set(i, v.u[k].get(i) + v.d[k].get(i)); s += v.u[k].get(i); }
+                v.u[k].store((T*)p.prev_in + off + (int64_t)(t.rank + k * t.size) * W);
             }
     }
     const float m = t.sum(s, red0) * p.inv_c;
@@ -421,7 +635,7 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
         for (int k = 0; k < P; ++k)
             if (t.rank + k * t.size < p.nvec)
 #pragma unroll
-                for (int i = 0; i < W; ++i) { const float e = u[k].get(i) - m; q += e * e; }
+                for (int i = 0; i < W; ++i) { const float e = v.u[k].get(i) - m; q += e * e; }
     }
     const float r = __frsqrt_rn(t.sum(q, red1) * p.inv_c + p.eps);
     bool hit = false;
@@ -432,9 +646,9 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
 #pragma unroll
                 for (int i = 0; i < W; ++i) {
                     // the norm is rounded to the storage type first, then the difference: e = 0 exactly where nothing changed
-                    const float y = rnd<T>((u[k].get(i) - m) * r * w[k].get(i) + b[k].get(i));
-                    d[k].set(i, y - o[k].get(i));
-                    hit |= fabsf(d[k].get(i)) > p.thr;
+                    const float y = rnd<T>((v.u[k].get(i) - m) * r * w[k].get(i) + b[k].get(i));
+                    v.d[k].set(i, y - v.o[k].get(i));
+                    hit |= fabsf(v.d[k].get(i)) > p.thr;
                 }
     }
     bool keep;
@@ -446,29 +660,33 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
             if (t.rank + k * t.size < p.nvec) {
                 const int64_t at = off + (int64_t)(t.rank + k * t.size) * W;
 #pragma unroll
-                for (int i = 0; i < W; ++i) o[k].set(i, o[k].get(i) + d[k].get(i));
-                d[k].store((T*)p.out + at);
-                o[k].store((T*)p.prev_out + at);
+                for (int i = 0; i < W; ++i) v.o[k].set(i, v.o[k].get(i) + v.d[k].get(i));
+                v.d[k].store((T*)p.out + at);
+                v.o[k].store((T*)p.prev_out + at);
             }
     }
     return keep;
 }
 
-// Teams of lanes: a warp reads the mask of 32 pixels at once, lists the active ones and hands them to its teams, so that
-// sparse maps cost one coalesced mask read and no idle teams.
+// Teams of lanes: a warp reads the mask of `chunk` pixels at once, lists the active ones and hands them to its teams, so that
+// sparse maps cost one coalesced mask read and no idle teams. The next chunk's mask is on its way meanwhile.
 template <typename T, typename WT, int W, int P>
-__global__ void __launch_bounds__(256) k_ln_delta(LnDeltaParams p) {
+__global__ void __launch_bounds__(256, P == 1 ? 5 : 1) k_ln_delta(LnDeltaParams p) {
     __shared__ uint8_t list[8][32], kept[8][32];
     grid_dep_launch();
     grid_dep_wait();
     Team<false> t(p.g);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, teams = 32 / p.g;
+    const int64_t step = (int64_t)gridDim.x * 8 * p.chunk;
+    int64_t base = ((int64_t)blockIdx.x * 8 + warp) * p.chunk;
+    const bool mine = lane < p.chunk;
+    int32_t next = mine && base + lane < p.npix ? p.mask[base + lane] : 0;
     Frag<WT, W> w[P], b[P];
     load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
     load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
-    const int64_t step = (int64_t)gridDim.x * 8 * 32;
-    for (int64_t base = ((int64_t)blockIdx.x * 8 + warp) * 32; base < p.npix; base += step) {
-        const bool act = base + lane < p.npix && p.mask[base + lane] != 0;
+    for (; base < p.npix; base += step) {
+        const bool act = next != 0;
+        next = mine && base + step + lane < p.npix ? p.mask[base + step + lane] : 0;
         const unsigned m = __ballot_sync(DC_FULL, act);
         if (act) list[warp][__popc(m & ((1u << lane) - 1u))] = (uint8_t)lane;
         kept[warp][lane] = 0;
@@ -478,11 +696,13 @@ __global__ void __launch_bounds__(256) k_ln_delta(LnDeltaParams p) {
             const int at = k + lane / p.g;
             const bool on = at < n;
             const int px = on ? list[warp][at] : 0;
-            const bool keep = ln_delta_pixel<T, WT, W, P, false>(p, t, base + px, on, w, b, nullptr, nullptr);
+            DeltaPixel<T, W, P> v;
+            if (on) v.load(p, base + px, t.rank, t.size);
+            const bool keep = ln_delta_pixel<T, WT, W, P, false>(p, t, base + px, on, v, w, b, nullptr, nullptr);
             if (on && t.rank == 0 && keep) kept[warp][px] = 1;
         }
         __syncwarp();
-        if (base + lane < p.npix) p.mask_out[base + lane] = kept[warp][lane];
+        if (mine && base + lane < p.npix) p.mask_out[base + lane] = kept[warp][lane];
         __syncwarp();
     }
 }
@@ -498,7 +718,12 @@ __global__ void __launch_bounds__(kLnCta) k_ln_delta_cta(LnDeltaParams p) {
     load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
     for (int64_t px = t.row; px < p.npix; px += t.stride) {
         const bool act = p.mask[px] != 0;      // the same word in every thread
-        const bool keep = act && ln_delta_pixel<T, WT, W, P, true>(p, t, px, true, w, b, red[0], red[1]);
+        bool keep = false;
+        if (act) {
+            DeltaPixel<T, W, P> v;
+            v.load(p, px, t.rank, t.size);
+            keep = ln_delta_pixel<T, WT, W, P, true>(p, t, px, true, v, w, b, red[0], red[1]);
+        }
         __syncthreads();                       // mask_out may be mask: everybody has read it
         if (t.rank == 0) p.mask_out[px] = keep ? 1 : 0;
     }
@@ -512,91 +737,124 @@ struct LnShape {
     int w, p, g, threads;      // g > 0: lanes of a warp; g == 0: a CTA of `threads`; p == 0: the long loop
 };
 
-static LnShape ln_shape(int c, int elem_bytes, bool aligned) {
+// warp_packs: most packs per lane of a row that a group of lanes takes (more registers per lane than a CTA's threads need, but
+// no barriers).
+static LnShape ln_shape(int c, int elem_bytes, bool aligned, int warp_packs) {
     LnShape s{};
     const int vec = 16 / elem_bytes;
     s.w = aligned && c % vec == 0 ? vec : 1;
     const int n = c / s.w;
     // single elements: eight per thread, so that a thread has as many bytes in flight as a packed one
-    const int warp_max = s.w > 1 ? 4 : 8;
-    if (n <= 32 * warp_max) {
+    if (n <= 32 * (s.w > 1 ? warp_packs : 8)) {
         s.g = lanes_per_pixel(n);
         const int need = divup(n, s.g);
         s.p = s.w == 1 ? (need <= 2 ? 2 : 8) : need <= 1 ? 1 : need <= 2 ? 2 : 4;
         s.threads = 256;
         return s;
     }
-    s.p = s.w == 1 ? 8 : n <= 256 ? 1 : n <= 2 * kLnCta ? 2 : 4;
+    s.p = s.w == 1 ? (n <= 2048 ? 8 : 16) : n <= 256 ? 1 : n <= 2 * kLnCta ? 2 : 4;
     const int threads = divup(divup(n, s.p), 32) * 32;
     if (threads <= kLnCta) { s.threads = threads; return s; }
-    s.w = 1; s.p = 0; s.threads = 1024;
+    s.p = 0; s.threads = 1024;
     return s;
 }
 
-static int64_t ln_grid(const LnShape& s, int64_t rows, int per_sm_threads) {
+// CTAs of a kernel that an SM holds; the grid is sized by it, so that every CTA's rows, and its one read of the parameters, start at once.
+template <auto KERNEL>
+static int resident_ctas(int threads, size_t smem) {
+    static int known[64][33] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 1;
+    int& n = known[dev][threads / 32];
+    if (n == 0) {
+        int v = 0;
+        if (smem > 48 * 1024) (void)cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem);
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, KERNEL, threads, smem) != cudaSuccess) (void)cudaGetLastError();
+        n = v > 0 ? v : 1;
+    }
+    return n;
+}
+
+static int64_t ln_ctas(const LnShape& s, int64_t rows, int per_sm) {
     const int64_t want = s.g > 0 ? divup64(rows, s.threads / s.g) : rows;
-    int per_sm = per_sm_threads / s.threads;
-    if (per_sm < 1) per_sm = 1;
     const int64_t cap = (int64_t)sm_count() * per_sm;
     return want < cap ? (want < 1 ? 1 : want) : cap;
 }
 
-#define DC_LN_P(KERNEL, T, WT, W, BLOCK)                                                  \
-    switch (s.p) {                                                                        \
-        case 1: DC_LN_RUN((KERNEL<T, WT, W, 1 DC_LN_TAIL(BLOCK)>)); break;                \
-        case 2: DC_LN_RUN((KERNEL<T, WT, W, 2 DC_LN_TAIL(BLOCK)>)); break;                \
-        case 4: DC_LN_RUN((KERNEL<T, WT, W, 4 DC_LN_TAIL(BLOCK)>)); break;                \
-        default: break;                                                                   \
-    }
-#define DC_LN_P1(KERNEL, T, WT, BLOCK)                                                    \
-    switch (s.p) {                                                                        \
-        case 2: DC_LN_RUN((KERNEL<T, WT, 1, 2 DC_LN_TAIL(BLOCK)>)); break;                \
-        case 8: DC_LN_RUN((KERNEL<T, WT, 1, 8 DC_LN_TAIL(BLOCK)>)); break;                \
-        default: break;                                                                   \
-    }
+// DC_LN_RUN for the instantiation that a shape names, of those that ln_shape can give.
+#define DC_LN_CASE(N, KERNEL, T, WT, W, BLOCK) case N: DC_LN_RUN((KERNEL<T, WT, W, N DC_LN_TAIL(BLOCK)>)); break;
+#define DC_LN_PACKS2(KERNEL, T, WT, W, BLOCK) switch (s.p) { DC_LN_CASE(1, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(2, KERNEL, T, WT, W, BLOCK) default: break; }
+#define DC_LN_PACKS4(KERNEL, T, WT, W, BLOCK) \
+    switch (s.p) { DC_LN_CASE(1, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(2, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(4, KERNEL, T, WT, W, BLOCK) default: break; }
+// Single elements, and the delta kernels have no BLOCK parameter.
+#define DC_LN_SINGLE_WARP(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(2, KERNEL, T, WT, 1, false) DC_LN_CASE(8, KERNEL, T, WT, 1, false) default: break; }
+#define DC_LN_SINGLE_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
 
 #define DC_LN_TAIL(BLOCK) , BLOCK
+template <auto KERNEL>
+static int ln_forward_run(const LnShape& s, LnParams& p, size_t smem, cudaStream_t st) {
+    const int64_t ctas = ln_ctas(s, p.rows, resident_ctas<KERNEL>(s.threads, smem));
+    return launch_pdl(KERNEL, dim3((unsigned)ctas), dim3(s.threads), smem, st, p);
+}
 template <typename T, typename WT>
 static int ln_forward_t(const LnShape& s, LnParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
-    // 2048 threads a SM is the most it holds; a team prefetches one row, so more resident threads are more rows in flight
-    const dim3 grid((unsigned)ln_grid(s, p.rows, 2048)), block(s.threads);
+    const size_t smem = s.w > 1 ? (size_t)s.threads * s.p * (rows_ahead(s.p) + 1) * 16 : 0;
     int rc = DC_ERR_UNSUPPORTED;
-#define DC_LN_RUN(K) rc = launch_pdl(K, grid, block, 0, st, p)
-    if (s.p == 0) return launch_pdl(k_ln_fwd_long<T, WT>, grid, block, 0, st, p);
-    if (s.w > 1) { if (s.g > 0) { DC_LN_P(k_ln_fwd, T, WT, V, false) } else { DC_LN_P(k_ln_fwd, T, WT, V, true) } }
-    else { if (s.g > 0) { DC_LN_P1(k_ln_fwd, T, WT, false) } else { DC_LN_P1(k_ln_fwd, T, WT, true) } }
+#define DC_LN_RUN(K) rc = ln_forward_run<K>(s, p, smem, st)
+    if (s.p == 0) return s.w > 1 ? ln_forward_run<k_ln_fwd_long<T, WT, V>>(s, p, 0, st) : ln_forward_run<k_ln_fwd_long<T, WT, 1>>(s, p, 0, st);
+    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS4(k_ln_fwd, T, WT, V, false) } else { DC_LN_PACKS4(k_ln_fwd, T, WT, V, true) } }
+    else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_fwd, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_fwd, T, WT) } }
 #undef DC_LN_RUN
     return rc;
 }
 
+// CTAs of the backward kernel; each owns a slice of the workspace, so the count depends on nothing but the sizes and the GPU: what
+// an SM holds at the kernels' register bounds.
+static int64_t ln_backward_ctas(const LnShape& s, int64_t rows) {
+    const int per_sm = s.p == 0 ? 1 : bwd_ctas(s.w, s.p) * row_threads(s.w, s.p) / s.threads;
+    return ln_ctas(s, rows, per_sm < 1 ? 1 : per_sm);
+}
+template <auto KERNEL>
+static int ln_backward_run(const LnShape& s, LnBwdParams& p, int64_t ctas, size_t smem, cudaStream_t st) {
+    (void)resident_ctas<KERNEL>(s.threads, smem);          // sets the shared memory limit once per device
+    return launch_pdl(KERNEL, dim3((unsigned)ctas), dim3(s.threads), smem, st, p);
+}
 template <typename T, typename WT>
 static int ln_backward_t(const LnShape& s, LnBwdParams& p, int64_t ctas, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
-    const dim3 grid((unsigned)ctas), block(s.threads);
-    const size_t smem = s.g > 0 ? (size_t)2 * p.c * sizeof(float) : 0;     // at most 2 * 1024 floats
+    size_t smem = s.w > 1 ? (size_t)s.threads * s.p * 2 * (rows_ahead(2 * s.p) + 1) * 16 : 0;
+    if (s.g > 0 && smem < (size_t)8 * p.c) smem = (size_t)8 * p.c;
     int rc = DC_ERR_UNSUPPORTED;
-#define DC_LN_RUN(K) rc = launch_pdl(K, grid, block, smem, st, p)
-    if (s.p == 0) return launch_pdl(k_ln_bwd_long<T, WT>, grid, block, 0, st, p);
-    if (s.w > 1) { if (s.g > 0) { DC_LN_P(k_ln_bwd, T, WT, V, false) } else { DC_LN_P(k_ln_bwd, T, WT, V, true) } }
-    else { if (s.g > 0) { DC_LN_P1(k_ln_bwd, T, WT, false) } else { DC_LN_P1(k_ln_bwd, T, WT, true) } }
+#define DC_LN_RUN(K) rc = ln_backward_run<K>(s, p, ctas, smem, st)
+    if (s.p == 0) {
+        smem = (size_t)p.c * 8 <= (size_t)kLongSmem ? (size_t)kLongSmem : 0;
+        return s.w > 1 ? ln_backward_run<k_ln_bwd_long<T, WT, V>>(s, p, ctas, smem, st) : ln_backward_run<k_ln_bwd_long<T, WT, 1>>(s, p, ctas, smem, st);
+    }
+    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS2(k_ln_bwd, T, WT, V, false) } else { DC_LN_PACKS4(k_ln_bwd, T, WT, V, true) } }
+    else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_bwd, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_bwd, T, WT) } }
 #undef DC_LN_RUN
     return rc;
 }
 #undef DC_LN_TAIL
 
 #define DC_LN_TAIL(BLOCK)
+template <auto KERNEL>
+static int ln_delta_run(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
+    const int64_t resident = (int64_t)sm_count() * resident_ctas<KERNEL>(s.threads, 0);
+    // teams of lanes: pixels that a warp takes at once, as many as leave every resident warp some
+    p.chunk = 32;
+    while (p.chunk > 8 && divup64(p.npix, p.chunk) < resident * 8) p.chunk >>= 1;
+    const int64_t want = s.g > 0 ? divup64(p.npix, p.chunk * 8) : p.npix;
+    return launch_pdl(KERNEL, dim3((unsigned)(want < resident ? want : resident)), dim3(s.threads), 0, st, p);
+}
 template <typename T, typename WT>
 static int ln_delta_t(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
-    int64_t ctas = s.g > 0 ? divup64(p.npix, 256) : p.npix;
-    const int64_t cap = (int64_t)sm_count() * (2048 / s.threads > 0 ? 2048 / s.threads : 1);
-    if (ctas > cap) ctas = cap;
-    const dim3 grid((unsigned)ctas), block(s.threads);
     int rc = DC_ERR_UNSUPPORTED;
-#define DC_LN_RUN(K) rc = launch_pdl(K, grid, block, 0, st, p)
-    if (s.w > 1) { if (s.g > 0) { DC_LN_P(k_ln_delta, T, WT, V, ) } else { DC_LN_P(k_ln_delta_cta, T, WT, V, ) } }
-    else { if (s.g > 0) { DC_LN_P1(k_ln_delta, T, WT, ) } else { DC_LN_P1(k_ln_delta_cta, T, WT, ) } }
+#define DC_LN_RUN(K) rc = ln_delta_run<K>(s, p, st)
+    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS4(k_ln_delta, T, WT, V, ) } else { DC_LN_PACKS4(k_ln_delta_cta, T, WT, V, ) } }
+    else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_delta, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_delta_cta, T, WT) } }
 #undef DC_LN_RUN
     return rc;
 }
@@ -617,8 +875,7 @@ static bool ln_dtypes_ok(int dtype, int weight_dtype) {
 }
 static int ln_elem(int dtype) { return dtype == DC_F32 ? 4 : 2; }
 
-// CTAs of the backward kernel; each owns a slice of the workspace, so the count depends on nothing but the sizes and the GPU.
-static int64_t ln_backward_ctas(const LnShape& s, int64_t rows) { return ln_grid(s, rows, 1024); }
+constexpr int kFwdWarpPacks = 4, kBwdWarpPacks = 2, kDeltaWarpPacks = 4;
 
 }  // namespace dc
 
@@ -632,7 +889,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
     if (rows < 0 || c <= 0) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     if (rows == 0) return DC_OK;
-    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias));
+    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias), kFwdWarpPacks);
     LnParams p{x, weight, bias, y, mean, rstd, rows, c, c / s.w, s.g, eps, 1.f / (float)c};
     DC_LN_TYPES(ln_forward_t, s, p, (cudaStream_t)stream)
 }
@@ -640,7 +897,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype) {
     if (rows <= 0 || c <= 0 || dtype < DC_F32 || dtype > DC_BF16) return 0;
     // the split may differ with the pointers' alignment: room for either
-    const int64_t a = ln_backward_ctas(ln_shape(c, ln_elem(dtype), true), rows), b = ln_backward_ctas(ln_shape(c, ln_elem(dtype), false), rows);
+    const int64_t a = ln_backward_ctas(ln_shape(c, ln_elem(dtype), true, kBwdWarpPacks), rows), b = ln_backward_ctas(ln_shape(c, ln_elem(dtype), false, kBwdWarpPacks), rows);
     return (size_t)((a > b ? a : b) * 2 * c) * sizeof(float);
 }
 
@@ -655,7 +912,7 @@ int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (sums && workspace == nullptr)) return DC_ERR_NULL_POINTER;
     if (dx == nullptr && !sums) return DC_OK;
     if (sums && (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0) return DC_ERR_ALIGNMENT;
-    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(weight));
+    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(weight), kBwdWarpPacks);
     const int64_t ctas = ln_backward_ctas(s, rows);
     if (sums && workspace_bytes < (size_t)(ctas * 2 * c) * sizeof(float)) return DC_ERR_WORKSPACE;
     LnBwdParams p{dy, x, weight, mean, rstd, dx, sums ? (float*)workspace : nullptr, rows, c, c / s.w, s.g, 1.f / (float)c};
@@ -673,10 +930,10 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
     if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;      // the caches are those of the delta path
     if (npix == 0) return DC_OK;
     const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(delta) && aligned16(prev_in) && aligned16(prev_out) && aligned16(out) &&
-                                                      aligned16(weight) && aligned16(bias));
+                                                      aligned16(weight) && aligned16(bias), kDeltaWarpPacks);
     if (s.p == 0) return DC_ERR_UNSUPPORTED;      // more channels than the registers of a CTA hold
     const float thr = dtype == DC_F16 ? host_round_threshold<__half>(threshold) : threshold;
-    LnDeltaParams p{delta, weight, bias, mask, prev_in, prev_out, out, mask_out, npix, c, c / s.w, s.g, thr, eps, 1.f / (float)c};
+    LnDeltaParams p{delta, weight, bias, mask, prev_in, prev_out, out, mask_out, npix, c, c / s.w, s.g, thr, eps, 1.f / (float)c, 32};
     cudaStream_t st = (cudaStream_t)stream;
     if (dtype == DC_F32) return ln_delta_t<float, float>(s, p, st);
     return weight_dtype == DC_F32 ? ln_delta_t<__half, float>(s, p, st) : ln_delta_t<__half, __half>(s, p, st);
