@@ -113,6 +113,16 @@ constexpr int kLnCta = 512;         // most threads of a CTA that holds a row: 1
 __host__ __device__ constexpr int row_threads(int w, int p) { return (w == 1 ? p > 8 : p > 1) ? kLnCta : 256; }
 constexpr int kMaxWarps = 32;
 
+// Sum over an aligned group of g lanes, g the same in the whole grid: five predicated steps instead of a loop.
+__device__ __forceinline__ float lanes_sum(float x, int g) {
+    if (g > 16) x += __shfl_xor_sync(DC_FULL, x, 16);
+    if (g > 8) x += __shfl_xor_sync(DC_FULL, x, 8);
+    if (g > 4) x += __shfl_xor_sync(DC_FULL, x, 4);
+    if (g > 2) x += __shfl_xor_sync(DC_FULL, x, 2);
+    if (g > 1) x += __shfl_xor_sync(DC_FULL, x, 1);
+    return x;
+}
+
 // A row's team: g lanes of a warp (BLOCK false) or the whole CTA (BLOCK true).
 template <bool BLOCK> struct Team {
     int rank, size;            // this thread's place in the team, the team's threads
@@ -130,7 +140,7 @@ template <bool BLOCK> struct Team {
     // Sum over the team, the same bits in every thread. red: kMaxWarps floats per call site (BLOCK); a site is used again
     // only after another site's barrier.
     __device__ __forceinline__ float sum(float x, float* red) const {
-        if constexpr (!BLOCK) return group_sum(x, size);
+        if constexpr (!BLOCK) return lanes_sum(x, size);
         x = group_sum(x, 32);
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = x;
         __syncthreads();
@@ -139,12 +149,6 @@ template <bool BLOCK> struct Team {
     }
 };
 
-template <typename T, int W, int P>
-__device__ __forceinline__ void load_row(Frag<T, W> (&v)[P], const T* p, int rank, int size, int nvec) {
-#pragma unroll
-    for (int k = 0; k < P; ++k)
-        if (rank + k * size < nvec) v[k].load(p + (int64_t)(rank + k * size) * W);
-}
 // The rows ahead of the one at hand. 16-byte packs: every thread copies its own packs of the next rows of N arrays into its own
 // slots of a ring in shared memory (cp.async: no registers, no barrier, a wait for the thread's own copies). Three rows, or one
 // where a row alone is 64 KB or more of a CTA's shared memory. Single elements: the next row in registers.
@@ -259,9 +263,14 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
     RowPipe<T, W, P, 1> pipe;
     pipe.start(t, {p.x}, p.rows, p.c, p.nvec, ring);
     T* y = (T*)p.y + t.row * p.c + t.rank * W;
-    Frag<WT, W> w[P], b[P];
-    load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
-    load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
+    // weight and bias stay in registers; lanes with three packs and more read them from L1 for every row instead and have the
+    // registers for twice the warps (12544 x 576: 12.3 -> 8.9 us)
+    constexpr bool kHeld = BLOCK || P < 3 || W == 1;
+    Frag<WT, W> w[kHeld ? P : 1], b[kHeld ? P : 1];
+    if constexpr (kHeld) {
+        load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
+        load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
+    }
     using V = typename Vals<W>::V;
     constexpr int N = Vals<W>::N;
     // lanes of a warp whose own rows have run out still take part in its shuffles
@@ -284,13 +293,24 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
 #pragma unroll
             for (int i = 0; i < N; ++i) { x[k].v[i] = add(x[k].v[i], neg); q = fma(x[k].v[i], x[k].v[i], q); }
         }
-        const float r = __frsqrt_rn(t.sum(q.sum(), red[1]) * p.inv_c + p.eps);
+        const float r = rsqrtf(t.sum(q.sum(), red[1]) * p.inv_c + p.eps);
         const V rr = V::all(r);
 #pragma unroll
         for (int k = 0; k < P; ++k) {
             Vals<W> ww, bb;
-            ww.from(w[k]);
-            bb.from(b[k]);
+            if constexpr (kHeld) {
+                ww.from(w[k]);
+                bb.from(b[k]);
+            } else {
+                Frag<WT, W> f[2];
+                f[0].fill(1.f);
+                f[1].fill(0.f);
+                const int col = (t.rank + k * t.size) * W;
+                if (p.w != nullptr && (pipe.valid >> k & 1u)) f[0].load((const WT*)p.w + col);
+                if (p.b != nullptr && (pipe.valid >> k & 1u)) f[1].load((const WT*)p.b + col);
+                ww.from(f[0]);
+                bb.from(f[1]);
+            }
 #pragma unroll
             for (int i = 0; i < N; ++i) x[k].v[i] = fma(mul(x[k].v[i], rr), ww.v[i], bb.v[i]);
             x[k].to(in[0][k]);
@@ -325,7 +345,7 @@ __global__ void __launch_bounds__(1024) k_ln_fwd_long(LnParams p) {
 #pragma unroll
             for (int j = 0; j < W; ++j) { const float d = v.get(j) - m; q += d * d; }
         }
-        const float r = __frsqrt_rn(t.sum(q, red[1]) * p.inv_c + p.eps);
+        const float r = rsqrtf(t.sum(q, red[1]) * p.inv_c + p.eps);
         for (int i = t.rank; i < p.nvec; i += t.size) {
             Frag<WT, W> w, b;
             w.fill(1.f);
@@ -427,8 +447,8 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
                 a = group_sum(in_cta ? red[par][0][lane] : 0.f, 32) * p.inv_c;
                 c = group_sum(in_cta ? red[par][1][lane] : 0.f, 32) * p.inv_c;
             } else {
-                a = group_sum(sg.sum(), t.size) * p.inv_c;
-                c = group_sum(sgn.sum(), t.size) * p.inv_c;
+                a = lanes_sum(sg.sum(), t.size) * p.inv_c;
+                c = lanes_sum(sgn.sum(), t.size) * p.inv_c;
             }
             const V na = V::all(-a), nc = V::all(-c);
 #pragma unroll
@@ -603,66 +623,103 @@ struct LnDeltaParams {
     int chunk;                 // pixels that a warp takes at once (teams of lanes)
 };
 
-// What a team reads of a pixel: the delta, the accumulated input, the accumulated output.
-template <typename T, int W, int P> struct DeltaPixel {
-    Frag<T, W> d[P], u[P], o[P];
-    __device__ __forceinline__ void load(const LnDeltaParams& p, int64_t px, int rank, int size) {
-        const int64_t off = px * p.c;
-        load_row<T, W, P>(d, (const T*)p.delta + off, rank, size, p.nvec);
-        load_row<T, W, P>(u, (const T*)p.prev_in + off, rank, size, p.nvec);
-        load_row<T, W, P>(o, (const T*)p.prev_out + off, rank, size, p.nvec);
+// Sums and differences in the storage type, each rounded once. Two halves added in packed half arithmetic give the correctly
+// rounded half, as float32 and one rounding do (24 >= 2 * 11 + 2 bits).
+template <typename T, int W> __device__ __forceinline__ void frag_add(Frag<T, W>& a, const Frag<T, W>& b) {
+    if constexpr (std::is_same_v<T, __half> && W > 1) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) reinterpret_cast<__half2*>(a.s)[i] = __hadd2(reinterpret_cast<__half2*>(a.s)[i], reinterpret_cast<const __half2*>(b.s)[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) a.set(i, a.get(i) + b.get(i));
     }
-};
+}
+template <typename T, int W> __device__ __forceinline__ void frag_sub(Frag<T, W>& a, const Frag<T, W>& b) {
+    if constexpr (std::is_same_v<T, __half> && W > 1) {
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) reinterpret_cast<__half2*>(a.s)[i] = __hsub2(reinterpret_cast<__half2*>(a.s)[i], reinterpret_cast<const __half2*>(b.s)[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < W; ++i) a.set(i, a.get(i) - b.get(i));
+    }
+}
+template <typename T, int W> __device__ __forceinline__ bool frag_any_above(const Frag<T, W>& a, float thr) {
+    if constexpr (std::is_same_v<T, __half> && W > 1) {      // thr is a half already
+        const __half2 t = __float2half2_rn(thr);
+        unsigned any = 0;
+#pragma unroll
+        for (int i = 0; i < W / 2; ++i) any |= __hgt2_mask(__habs2(reinterpret_cast<const __half2*>(a.s)[i]), t);
+        return any != 0;
+    } else {
+        bool any = false;
+#pragma unroll
+        for (int i = 0; i < W; ++i) any |= fabsf(a.get(i)) > thr;
+        return any;
+    }
+}
+
 // One pixel by its team; returns whether any channel's change is above the threshold (the same answer in the whole team).
+// Packs behind the last channel hold zeros all along.
 template <typename T, typename WT, int W, int P, bool BLOCK>
-__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, DeltaPixel<T, W, P>& v, Frag<WT, W> (&w)[P],
-                                               Frag<WT, W> (&b)[P], float* red0, float* red1) {
-    const int64_t off = px * p.c;
-    float s = 0.f;
-    if (on) {
+__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, Frag<WT, W> (&w)[P], Frag<WT, W> (&b)[P],
+                                               float* red0, float* red1) {
+    const int64_t off = px * p.c + t.rank * W;
+    Frag<T, W> d[P], u[P], o[P];
+    bool valid[P];
 #pragma unroll
-        for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec) {
-#pragma unroll
-                for (int i = 0; i < W; ++i) { v.u[k].set(i, v.u[k].get(i) + v.d[k].get(i)); s += v.u[k].get(i); }
-                v.u[k].store((T*)p.prev_in + off + (int64_t)(t.rank + k * t.size) * W);
-            }
+    for (int k = 0; k < P; ++k) {
+        valid[k] = t.rank + k * t.size < p.nvec;
+        d[k].fill(0.f); u[k].fill(0.f); o[k].fill(0.f);
+        if (on && valid[k]) {
+            const int64_t at = off + k * t.size * W;
+            d[k].load((const T*)p.delta + at);
+            u[k].load((const T*)p.prev_in + at);
+            o[k].load((const T*)p.prev_out + at);
+        }
     }
-    const float m = t.sum(s, red0) * p.inv_c;
-    float q = 0.f;
-    if (on) {
+    using V = typename Vals<W>::V;
+    constexpr int N = Vals<W>::N;
+    Vals<W> x[P];
+    V s = V::all(0.f), q = V::all(0.f);
 #pragma unroll
-        for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec)
+    for (int k = 0; k < P; ++k) {
+        frag_add(u[k], d[k]);
+        if (on && valid[k]) u[k].store((T*)p.prev_in + off + k * t.size * W);
+        x[k].from(u[k]);
 #pragma unroll
-                for (int i = 0; i < W; ++i) { const float e = v.u[k].get(i) - m; q += e * e; }
+        for (int i = 0; i < N; ++i) s = add(s, x[k].v[i]);
     }
-    const float r = __frsqrt_rn(t.sum(q, red1) * p.inv_c + p.eps);
+    const float m = t.sum(s.sum(), red0) * p.inv_c;
+#pragma unroll
+    for (int k = 0; k < P; ++k) {
+        const V neg = V::all(valid[k] ? -m : 0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) { x[k].v[i] = add(x[k].v[i], neg); q = fma(x[k].v[i], x[k].v[i], q); }
+    }
+    const float r = rsqrtf(t.sum(q.sum(), red1) * p.inv_c + p.eps);
+    const V rr = V::all(r);
     bool hit = false;
-    if (on) {
 #pragma unroll
-        for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec)
+    for (int k = 0; k < P; ++k) {
+        Vals<W> ww, bb;
+        ww.from(w[k]);
+        bb.from(b[k]);
 #pragma unroll
-                for (int i = 0; i < W; ++i) {
-                    // the norm is rounded to the storage type first, then the difference: e = 0 exactly where nothing changed
-                    const float y = rnd<T>((v.u[k].get(i) - m) * r * w[k].get(i) + b[k].get(i));
-                    v.d[k].set(i, y - v.o[k].get(i));
-                    hit |= fabsf(v.d[k].get(i)) > p.thr;
-                }
+        for (int i = 0; i < N; ++i) x[k].v[i] = fma(mul(x[k].v[i], rr), ww.v[i], bb.v[i]);
+        x[k].to(d[k]);               // the norm is rounded to the storage type first, then the difference: e = 0 exactly where nothing changed
+        frag_sub(d[k], o[k]);
+        hit |= frag_any_above(d[k], p.thr);
     }
     bool keep;
     if constexpr (BLOCK) keep = __syncthreads_or(hit) != 0;
-    else keep = group_any(hit, t.size, threadIdx.x & 31);
+    else keep = group_any(hit && on, t.size, threadIdx.x & 31);
     if (on && keep) {
 #pragma unroll
         for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec) {
-                const int64_t at = off + (int64_t)(t.rank + k * t.size) * W;
-#pragma unroll
-                for (int i = 0; i < W; ++i) v.o[k].set(i, v.o[k].get(i) + v.d[k].get(i));
-                v.d[k].store((T*)p.out + at);
-                v.o[k].store((T*)p.prev_out + at);
+            if (valid[k]) {
+                frag_add(o[k], d[k]);
+                d[k].store((T*)p.out + off + k * t.size * W);
+                o[k].store((T*)p.prev_out + off + k * t.size * W);
             }
     }
     return keep;
@@ -696,9 +753,7 @@ __global__ void __launch_bounds__(256, P == 1 ? 5 : 1) k_ln_delta(LnDeltaParams 
             const int at = k + lane / p.g;
             const bool on = at < n;
             const int px = on ? list[warp][at] : 0;
-            DeltaPixel<T, W, P> v;
-            if (on) v.load(p, base + px, t.rank, t.size);
-            const bool keep = ln_delta_pixel<T, WT, W, P, false>(p, t, base + px, on, v, w, b, nullptr, nullptr);
+            const bool keep = ln_delta_pixel<T, WT, W, P, false>(p, t, base + px, on, w, b, nullptr, nullptr);
             if (on && t.rank == 0 && keep) kept[warp][px] = 1;
         }
         __syncwarp();
@@ -718,12 +773,7 @@ __global__ void __launch_bounds__(kLnCta) k_ln_delta_cta(LnDeltaParams p) {
     load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
     for (int64_t px = t.row; px < p.npix; px += t.stride) {
         const bool act = p.mask[px] != 0;      // the same word in every thread
-        bool keep = false;
-        if (act) {
-            DeltaPixel<T, W, P> v;
-            v.load(p, px, t.rank, t.size);
-            keep = ln_delta_pixel<T, WT, W, P, true>(p, t, px, true, v, w, b, red[0], red[1]);
-        }
+        const bool keep = act && ln_delta_pixel<T, WT, W, P, true>(p, t, px, true, w, b, red[0], red[1]);
         __syncthreads();                       // mask_out may be mask: everybody has read it
         if (t.rank == 0) p.mask_out[px] = keep ? 1 : 0;
     }
@@ -739,7 +789,7 @@ struct LnShape {
 
 // warp_packs: most packs per lane of a row that a group of lanes takes (more registers per lane than a CTA's threads need, but
 // no barriers).
-static LnShape ln_shape(int c, int elem_bytes, bool aligned, int warp_packs) {
+static LnShape ln_shape(int c, int64_t rows, int elem_bytes, bool aligned, int warp_packs) {
     LnShape s{};
     const int vec = 16 / elem_bytes;
     s.w = aligned && c % vec == 0 ? vec : 1;
@@ -747,8 +797,11 @@ static LnShape ln_shape(int c, int elem_bytes, bool aligned, int warp_packs) {
     // single elements: eight per thread, so that a thread has as many bytes in flight as a packed one
     if (n <= 32 * (s.w > 1 ? warp_packs : 8)) {
         s.g = lanes_per_pixel(n);
+        // Rows enough for every SM's threads all the same: fewer lanes with more packs each shuffle less per element (96 channels
+        // in fp16, 200000 rows: 16 lanes of one pack 25 us, 4 lanes of three 20 us).
+        while (s.w > 1 && s.g > 1 && divup(n, s.g / 2) <= warp_packs && rows * (s.g / 2) >= (int64_t)sm_count() * 1024) s.g /= 2;
         const int need = divup(n, s.g);
-        s.p = s.w == 1 ? (need <= 2 ? 2 : 8) : need <= 1 ? 1 : need <= 2 ? 2 : 4;
+        s.p = s.w == 1 ? (need <= 2 ? 2 : 8) : need;
         s.threads = 256;
         return s;
     }
@@ -786,6 +839,11 @@ static int64_t ln_ctas(const LnShape& s, int64_t rows, int per_sm) {
 #define DC_LN_PACKS2(KERNEL, T, WT, W, BLOCK) switch (s.p) { DC_LN_CASE(1, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(2, KERNEL, T, WT, W, BLOCK) default: break; }
 #define DC_LN_PACKS4(KERNEL, T, WT, W, BLOCK) \
     switch (s.p) { DC_LN_CASE(1, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(2, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(4, KERNEL, T, WT, W, BLOCK) default: break; }
+#define DC_LN_PACKS1234(KERNEL, T, WT, W, BLOCK)                                                               \
+    switch (s.p) {                                                                                             \
+        DC_LN_CASE(1, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(2, KERNEL, T, WT, W, BLOCK)                          \
+        DC_LN_CASE(3, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(4, KERNEL, T, WT, W, BLOCK) default: break;          \
+    }
 // Single elements, and the delta kernels have no BLOCK parameter.
 #define DC_LN_SINGLE_WARP(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(2, KERNEL, T, WT, 1, false) DC_LN_CASE(8, KERNEL, T, WT, 1, false) default: break; }
 #define DC_LN_SINGLE_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
@@ -803,7 +861,7 @@ static int ln_forward_t(const LnShape& s, LnParams& p, cudaStream_t st) {
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_forward_run<K>(s, p, smem, st)
     if (s.p == 0) return s.w > 1 ? ln_forward_run<k_ln_fwd_long<T, WT, V>>(s, p, 0, st) : ln_forward_run<k_ln_fwd_long<T, WT, 1>>(s, p, 0, st);
-    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS4(k_ln_fwd, T, WT, V, false) } else { DC_LN_PACKS4(k_ln_fwd, T, WT, V, true) } }
+    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS1234(k_ln_fwd, T, WT, V, false) } else { DC_LN_PACKS4(k_ln_fwd, T, WT, V, true) } }
     else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_fwd, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_fwd, T, WT) } }
 #undef DC_LN_RUN
     return rc;
@@ -853,7 +911,7 @@ static int ln_delta_t(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_delta_run<K>(s, p, st)
-    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS4(k_ln_delta, T, WT, V, ) } else { DC_LN_PACKS4(k_ln_delta_cta, T, WT, V, ) } }
+    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS1234(k_ln_delta, T, WT, V, ) } else { DC_LN_PACKS4(k_ln_delta_cta, T, WT, V, ) } }
     else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_delta, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_delta_cta, T, WT) } }
 #undef DC_LN_RUN
     return rc;
@@ -889,7 +947,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
     if (rows < 0 || c <= 0) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     if (rows == 0) return DC_OK;
-    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias), kFwdWarpPacks);
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias), kFwdWarpPacks);
     LnParams p{x, weight, bias, y, mean, rstd, rows, c, c / s.w, s.g, eps, 1.f / (float)c};
     DC_LN_TYPES(ln_forward_t, s, p, (cudaStream_t)stream)
 }
@@ -897,7 +955,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype) {
     if (rows <= 0 || c <= 0 || dtype < DC_F32 || dtype > DC_BF16) return 0;
     // the split may differ with the pointers' alignment: room for either
-    const int64_t a = ln_backward_ctas(ln_shape(c, ln_elem(dtype), true, kBwdWarpPacks), rows), b = ln_backward_ctas(ln_shape(c, ln_elem(dtype), false, kBwdWarpPacks), rows);
+    const int64_t a = ln_backward_ctas(ln_shape(c, rows, ln_elem(dtype), true, kBwdWarpPacks), rows), b = ln_backward_ctas(ln_shape(c, rows, ln_elem(dtype), false, kBwdWarpPacks), rows);
     return (size_t)((a > b ? a : b) * 2 * c) * sizeof(float);
 }
 
@@ -912,7 +970,7 @@ int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (sums && workspace == nullptr)) return DC_ERR_NULL_POINTER;
     if (dx == nullptr && !sums) return DC_OK;
     if (sums && (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0) return DC_ERR_ALIGNMENT;
-    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(weight), kBwdWarpPacks);
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(weight), kBwdWarpPacks);
     const int64_t ctas = ln_backward_ctas(s, rows);
     if (sums && workspace_bytes < (size_t)(ctas * 2 * c) * sizeof(float)) return DC_ERR_WORKSPACE;
     LnBwdParams p{dy, x, weight, mean, rstd, dx, sums ? (float*)workspace : nullptr, rows, c, c / s.w, s.g, 1.f / (float)c};
@@ -929,7 +987,7 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
     if (npix < 0 || c <= 0) return DC_ERR_SHAPE;
     if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;      // the caches are those of the delta path
     if (npix == 0) return DC_OK;
-    const LnShape s = ln_shape(c, ln_elem(dtype), aligned16(delta) && aligned16(prev_in) && aligned16(prev_out) && aligned16(out) &&
+    const LnShape s = ln_shape(c, 0, ln_elem(dtype), aligned16(delta) && aligned16(prev_in) && aligned16(prev_out) && aligned16(out) &&
                                                       aligned16(weight) && aligned16(bias), kDeltaWarpPacks);
     if (s.p == 0) return DC_ERR_UNSUPPORTED;      // more channels than the registers of a CTA hold
     const float thr = dtype == DC_F16 ? host_round_threshold<__half>(threshold) : threshold;
