@@ -31,21 +31,17 @@ __global__ void __launch_bounds__(256) k_mx4_rows(const T* __restrict__ x, uint8
         const int64_t r = it / segments;
         const int64_t c0 = (it - r * segments) * (kMxChunk * kMxAhead) + lane * 8;
         const T* row = x + r * cols;
-        float v[kMxAhead][8];
+        Eight<T> v[kMxAhead];
 #pragma unroll
-        for (int a = 0; a < kMxAhead; ++a) load8<T, VEC>(v[a], row, c0 + a * kMxChunk, cols);
+        for (int a = 0; a < kMxAhead; ++a) v[a].template load<VEC>(row, c0 + a * kMxChunk, cols);
 #pragma unroll
         for (int a = 0; a < kMxAhead; ++a) {
             const int64_t col = c0 + a * kMxChunk, b = col >> 5;
-            uint32_t m = amax8_bits(v[a]);
-            m = max(m, __shfl_xor_sync(DC_FULL, m, 1));
-            m = max(m, __shfl_xor_sync(DC_FULL, m, 2));
-            const uint32_t s = mx4_scale_byte(m);
-            if (b < nb) *reinterpret_cast<uint32_t*>(data + r * nb * 16 + (col >> 1)) = encode_scaled(v[a], s);
+            uint32_t s;
+            const uint32_t code = mx4_encode_lane<T>(v[a], s);
+            if (b < nb) *reinterpret_cast<uint32_t*>(data + r * nb * 16 + (col >> 1)) = code;
             // the scale bytes of four blocks as one word, written by the first lane of every sixteen
-            uint32_t word = s << (8 * ((lane >> 2) & 3));
-            word |= __shfl_xor_sync(DC_FULL, word, 4);
-            word |= __shfl_xor_sync(DC_FULL, word, 8);
+            const uint32_t word = mx4_scale_quad(s, lane);
             if ((lane & 15) == 0 && (b >> 2) < tiles) *reinterpret_cast<uint32_t*>(scales + mx4_scale_word(r, b >> 2, tiles)) = word;
         }
     }
@@ -77,29 +73,15 @@ __global__ void __launch_bounds__(256) k_mx4_tile(MxTileParams p) {
     for (int q = 0; q < kTile / 16; ++q) {
         const int tr = q * 16 + lr;
         const int64_t r = r0 + tr;
-        float v[8];
-        if (r < p.rows) load8<T, VEC>(v, (const T*)p.x + r * p.cols, c0 + lc, p.cols);
-        else {
+        Eight<T> v;
+        v.template load<VEC>((const T*)p.x + r * p.cols, c0 + lc, r < p.rows ? p.cols : 0);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = 0.f;
-        }
-        T* at = reinterpret_cast<T*>(tile + tile_at<T>(tr, lc));
-#pragma unroll
-        for (int k = 0; k < 8 / VecTraits<T>::kVec; ++k) {
-            Pack<T, VecTraits<T>::kVec> o;
-#pragma unroll
-            for (int i = 0; i < VecTraits<T>::kVec; ++i) o.set(i, v[k * VecTraits<T>::kVec + i]);
-            o.store(at + k * VecTraits<T>::kVec);
-        }
+        for (int k = 0; k < Eight<T>::kWords / 4; ++k) reinterpret_cast<uint4*>(tile + tile_at<T>(tr, lc))[k] = reinterpret_cast<const uint4*>(v.w)[k];
         if (p.data != nullptr) {
-            uint32_t m = amax8_bits(v);
-            m = max(m, __shfl_xor_sync(DC_FULL, m, 1));
-            m = max(m, __shfl_xor_sync(DC_FULL, m, 2));
-            const uint32_t s = mx4_scale_byte(m);
-            if (r < p.rows && (c0 + lc) >> 5 < nb) *reinterpret_cast<uint32_t*>(p.data + r * nb * 16 + ((c0 + lc) >> 1)) = encode_scaled(v, s);
-            uint32_t word = s << (8 * ((lane >> 2) & 3));
-            word |= __shfl_xor_sync(DC_FULL, word, 4);
-            word |= __shfl_xor_sync(DC_FULL, word, 8);
+            uint32_t s;
+            const uint32_t code = mx4_encode_lane<T>(v, s);
+            if (r < p.rows && (c0 + lc) >> 5 < nb) *reinterpret_cast<uint32_t*>(p.data + r * nb * 16 + ((c0 + lc) >> 1)) = code;
+            const uint32_t word = mx4_scale_quad(s, lane);
             if ((lane & 15) == 0 && r < p.rows) *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_word(r, blockIdx.x, tiles)) = word;
         }
     }
@@ -107,33 +89,47 @@ __global__ void __launch_bounds__(256) k_mx4_tile(MxTileParams p) {
     // phase 2: a thread takes two columns of a 32-row block; a warp 8 column pairs x the 4 blocks
     const int pair = warp * 8 + (lane & 7), blk = lane >> 3;
     const int64_t nbt = mx4_blocks(p.rows), tiles_t = mx4_scale_tiles(p.rows);
-    float u[2][8];
-    float sum[2] = {0.f, 0.f};
+    const uint8_t* col = tile + tile_at<T>(blk * 32, pair * 2);
     uint32_t m[2] = {0u, 0u};
+    float sum[2] = {0.f, 0.f};
+    uint32_t code[2][4], s[2];
+    auto values = [&](int i) {           // row i of the block: both columns
+        if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float2*>(col + i * kTile * 4);
+        else return word_values<T>(*reinterpret_cast<const uint32_t*>(col + i * kTile * 2));
+    };
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll 8
-    for (int i = 0; i < 32; ++i) {
-        const T* at = reinterpret_cast<const T*>(tile + tile_at<T>(blk * 32 + i, pair * 2));
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float f = to_f<T>(at[k]);
-            sum[k] += f;
-            m[k] = max(m[k], __float_as_uint(f) & 0x7fffffffu);
+        for (int i = 0; i < 32; ++i) {
+            const float2 f = values(i);
+            m[0] = amax_word<float>(m[0], __float_as_uint(f.x));
+            m[1] = amax_word<float>(m[1], __float_as_uint(f.y));
         }
+    } else {
+        uint32_t both = 0u;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) both = amax_word<T>(both, *reinterpret_cast<const uint32_t*>(col + i * kTile * 2));
+        const float2 f = word_values<T>(both);
+        m[0] = __float_as_uint(f.x);
+        m[1] = __float_as_uint(f.y);
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) s[k] = mx4_scale_byte(m[k]);
+    const float f0 = mx4_factor(s[0]), f1 = mx4_factor(s[1]);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float u[2][8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float2 f = values(j * 8 + i);
+            if (p.colsum != nullptr) { sum[0] += f.x; sum[1] += f.y; }
+            mul2(f.x, f.y, f0, f1);
+            u[0][i] = f.x;
+            u[1][i] = f.y;
+        }
+        code[0][j] = s[0] == 255u ? 0u : mx4_encode8(u[0]);
+        code[1][j] = s[1] == 255u ? 0u : mx4_encode8(u[1]);
     }
     if (p.data_t != nullptr) {
-        uint32_t code[2][4];
-        const uint32_t s[2] = {mx4_scale_byte(m[0]), mx4_scale_byte(m[1])};
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const T* at = reinterpret_cast<const T*>(tile + tile_at<T>(blk * 32 + j * 8 + i, pair * 2));
-                u[0][i] = to_f<T>(at[0]);
-                u[1][i] = to_f<T>(at[1]);
-            }
-            code[0][j] = encode_scaled(u[0], s[0]);
-            code[1][j] = encode_scaled(u[1], s[1]);
-        }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             const int64_t c = c0 + pair * 2 + k, b = (int64_t)blockIdx.y * 4 + blk;
@@ -153,34 +149,50 @@ __global__ void __launch_bounds__(256) k_mx4_tile(MxTileParams p) {
     }
 }
 
-// A lane takes eight codes and their scale byte; 16 (or 32) bytes leave.
+// The way of k_mx4_rows back: a warp takes four chunks of 256 values of a row, a lane eight codes of each.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, T* __restrict__ out,
-                                                        int64_t rows, int64_t cols, int packs) {
+                                                        int64_t rows, int64_t cols, int segments) {
     grid_dep_launch();
     grid_dep_wait();
+    const int lane = threadIdx.x & 31;
     const int64_t nb = mx4_blocks(cols), tiles = mx4_scale_tiles(cols);
-    const int64_t n = rows * packs;
-    for (int64_t it = (int64_t)blockIdx.x * 256 + threadIdx.x; it < n; it += (int64_t)gridDim.x * 256) {
-        const int64_t r = it / packs, c = (it - r * packs) * 8, b = c >> 5;
-        const uint32_t code = *reinterpret_cast<const uint32_t*>(data + r * nb * 16 + (c >> 1));
-        const float s = mx4_scale_value(scales[mx4_scale_word(r, b >> 2, tiles) + (b & 3)]);
-        T* o = out + r * cols + c;
-        float v[8];
+    const int64_t items = rows * segments, nwarps = (int64_t)gridDim.x * 8;
+    for (int64_t it = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); it < items; it += nwarps) {
+        const int64_t r = it / segments;
+        const int64_t c0 = (it - r * segments) * (kMxChunk * kMxAhead) + lane * 8;
+        const uint8_t* row = data + r * nb * 16;
+        const uint8_t* srow = scales + mx4_scale_word(r, 0, tiles);
+        uint32_t code[kMxAhead], s[kMxAhead];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = mx4_decode(code >> (4 * i)) * s;
-        if constexpr (VEC) {
+        for (int a = 0; a < kMxAhead; ++a) {
+            const int64_t col = c0 + a * kMxChunk, b = col >> 5;
+            code[a] = b < nb ? *reinterpret_cast<const uint32_t*>(row + (col >> 1)) : 0u;
+            s[a] = b < nb ? srow[(b >> 2) * 512 + (b & 3)] : 0u;
+        }
 #pragma unroll
-            for (int k = 0; k < 8 / VecTraits<T>::kVec; ++k) {
-                Pack<T, VecTraits<T>::kVec> q;
+        for (int a = 0; a < kMxAhead; ++a) {
+            const int64_t col = c0 + a * kMxChunk;
+            const float f = mx4_scale_value(s[a]);
+            T* o = out + r * cols + col;
+            float v[8];
+            mx4_decode8(code[a], v);
 #pragma unroll
-                for (int i = 0; i < VecTraits<T>::kVec; ++i) q.set(i, v[k * VecTraits<T>::kVec + i]);
-                if (c + k * VecTraits<T>::kVec < cols) q.store(o + k * VecTraits<T>::kVec);
+            for (int i = 0; i < 4; ++i) mul2(v[2 * i], v[2 * i + 1], f, f);
+            if constexpr (VEC) {
+                constexpr int N = VecTraits<T>::kVec;
+#pragma unroll
+                for (int k = 0; k < 8 / N; ++k) {
+                    Pack<T, N> q;
+#pragma unroll
+                    for (int i = 0; i < N; ++i) q.set(i, v[k * N + i]);
+                    if (col + k * N < cols) q.store(o + k * N);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (col + i < cols) o[i] = from_f<T>(v[i]);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                if (c + i < cols) o[i] = from_f<T>(v[i]);
         }
     }
 }
@@ -214,13 +226,13 @@ static int quantize_t(const void* x, void* data, void* scales, void* data_t, voi
 
 template <typename T>
 static int dequantize_t(const void* data, const void* scales, void* out, int64_t rows, int64_t cols, cudaStream_t st) {
-    const int packs = (int)divup64(cols, 8);
-    int64_t ctas = divup64(rows * packs, 256);
-    const int64_t cap = (int64_t)sm_count() * 16;
+    const int segments = (int)divup64(cols, kMxChunk * kMxAhead);
+    int64_t ctas = divup64(rows * segments, 8);
+    const int64_t cap = (int64_t)sm_count() * 8;
     if (ctas > cap) ctas = cap;
     if (aligned16(out) && cols % VecTraits<T>::kVec == 0)
-        return launch_pdl(k_mx4_dequantize<T, true>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scales, (T*)out, rows, cols, packs);
-    return launch_pdl(k_mx4_dequantize<T, false>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scales, (T*)out, rows, cols, packs);
+        return launch_pdl(k_mx4_dequantize<T, true>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scales, (T*)out, rows, cols, segments);
+    return launch_pdl(k_mx4_dequantize<T, false>, dim3((unsigned)ctas), dim3(256), 0, st, (const uint8_t*)data, (const uint8_t*)scales, (T*)out, rows, cols, segments);
 }
 
 }  // namespace dc

@@ -46,45 +46,114 @@ __device__ __forceinline__ uint32_t mx4_encode8(const float* v) {
         : "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]));
     return r;
 }
-// The value of one code: sign, two exponent bits (bias 1), one mantissa bit.
-__device__ __forceinline__ float mx4_decode(uint32_t code) {
-    const uint32_t e = (code >> 1) & 3u, m = code & 1u;
-    const float a = e == 0u ? 0.5f * (float)m : (float)((2u + m) << (e - 1u)) * 0.5f;
-    return (code & 8u) ? -a : a;
-}
-
-// Eight values of a row starting at column col (cols in all); zeros behind the end.
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(float (&v)[8], const T* row, int64_t col, int64_t cols) {
-    if constexpr (VEC) {
-        constexpr int N = 8 / VecTraits<T>::kVec;
+// The values of eight codes.
+__device__ __forceinline__ void mx4_decode8(uint32_t codes, float* v) {
+    uint32_t h[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+        "mov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %1, b;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %2, c;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
+        : "r"(codes));
 #pragma unroll
-        for (int k = 0; k < N; ++k) {
-            Pack<T, VecTraits<T>::kVec> p;
-            if (col + k * VecTraits<T>::kVec < cols) p.load(row + col + k * VecTraits<T>::kVec);
-            else p.zero();
-#pragma unroll
-            for (int i = 0; i < VecTraits<T>::kVec; ++i) v[k * VecTraits<T>::kVec + i] = p.get(i);
-        }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? to_f<T>(row[col + i]) : 0.f;
+    for (int i = 0; i < 4; ++i) {
+        const float2 x = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+        v[2 * i] = x.x;
+        v[2 * i + 1] = x.y;
     }
 }
 
-__device__ __forceinline__ uint32_t amax8_bits(const float (&v)[8]) {
-    uint32_t m = 0;      // as integers: a NaN is above every number, so it is not lost
+// Eight neighbouring values of a row as they are stored, zeros behind the end.
+template <typename T> struct Eight {
+    static constexpr int kWords = 8 * (int)sizeof(T) / 4;
+    alignas(16) uint32_t w[kWords];
+
+    template <bool VEC> __device__ __forceinline__ void load(const T* row, int64_t col, int64_t cols) {
+        if constexpr (VEC) {
+            constexpr int N = VecTraits<T>::kVec;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-    return m;
+            for (int k = 0; k < 8 / N; ++k)
+                reinterpret_cast<uint4*>(w)[k] = col + k * N < cols ? *reinterpret_cast<const uint4*>(row + col + k * N) : make_uint4(0u, 0u, 0u, 0u);
+        } else {
+            T v[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = col + i < cols ? row[col + i] : from_f<T>(0.f);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) {
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(v[i]);
+                else w[i] = (uint32_t)*reinterpret_cast<const uint16_t*>(&v[2 * i]) | (uint32_t)*reinterpret_cast<const uint16_t*>(&v[2 * i + 1]) << 16;
+            }
+        }
+    }
+};
+
+// Largest magnitudes. 16-bit types: packed maxima of two values at once (a NaN stays a NaN); float32: as integers, where a NaN is
+// above every number. amax_bits gives the float32 bits.
+template <typename T> __device__ __forceinline__ uint32_t amax_word(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t amax_word<float>(uint32_t a, uint32_t b) { return max(a, b & 0x7fffffffu); }
+template <> __device__ __forceinline__ uint32_t amax_word<__half>(uint32_t a, uint32_t b) {
+    b &= 0x7fff7fffu;
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
 }
-__device__ __forceinline__ uint32_t encode_scaled(const float (&v)[8], uint32_t s) {
-    if (s == 255u) return 0u;
-    const float f = mx4_factor(s);
-    float u[8];
+template <> __device__ __forceinline__ uint32_t amax_word<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    b &= 0x7fff7fffu;
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&r);
+}
+// A word's two values (or its one) in float32.
+template <typename T> __device__ __forceinline__ float2 word_values(uint32_t w);
+template <> __device__ __forceinline__ float2 word_values<__half>(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+template <> __device__ __forceinline__ float2 word_values<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+// float32 bits of the larger of a word's two magnitudes.
+template <typename T> __device__ __forceinline__ uint32_t amax_bits(uint32_t w) {
+    if constexpr (sizeof(T) == 4) return w;
+    else {
+        const float2 v = word_values<T>(w);
+        return max(__float_as_uint(v.x), __float_as_uint(v.y));
+    }
+}
+
+// Products of two float32 at once.
+__device__ __forceinline__ void mul2(float& a, float& b, float f, float g) {
+    uint64_t x, y;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(x) : "f"(a), "f"(b));
+    asm("mov.b64 %0, {%1, %2};" : "=l"(y) : "f"(f), "f"(g));
+    asm("mul.rn.f32x2 %0, %0, %1;" : "+l"(x) : "l"(y));
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x));
+}
+
+// The scale byte of the block that a lane shares with its three neighbours, and the codes of its eight values.
+template <typename T> __device__ __forceinline__ uint32_t mx4_encode_lane(const Eight<T>& v, uint32_t& scale) {
+    uint32_t m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = v[i] * f;
-    return mx4_encode8(u);
+    for (int i = 0; i < Eight<T>::kWords; ++i) m = amax_word<T>(m, v.w[i]);
+    m = amax_word<T>(m, __shfl_xor_sync(DC_FULL, m, 1));
+    m = amax_word<T>(m, __shfl_xor_sync(DC_FULL, m, 2));
+    scale = mx4_scale_byte(amax_bits<T>(m));
+    const float f = mx4_factor(scale);
+    float u[8];
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) u[i] = __uint_as_float(v.w[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) { const float2 x = word_values<T>(v.w[i]); u[2 * i] = x.x; u[2 * i + 1] = x.y; }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mul2(u[2 * i], u[2 * i + 1], f, f);
+    const uint32_t code = mx4_encode8(u);
+    return scale == 255u ? 0u : code;
+}
+// The scale bytes of the four blocks of sixteen lanes as one word (in every lane).
+__device__ __forceinline__ uint32_t mx4_scale_quad(uint32_t scale, int lane) {
+    uint32_t word = scale << (8 * ((lane >> 2) & 3));
+    word |= __shfl_xor_sync(DC_FULL, word, 4);
+    return word | __shfl_xor_sync(DC_FULL, word, 8);
 }
 
 }  // namespace dc

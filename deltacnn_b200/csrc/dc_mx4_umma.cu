@@ -225,13 +225,13 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
                     const int64_t col = (int64_t)ks * kMxStep + lane * 8;
                     bool ready = false;
                     for (int r0 = 0; r0 < rows; r0 += 4) {
-                        float v[4][8];
+                        Eight<OT> v[4];
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
-                            if (r0 + j >= rows) break;
                             const OT* row = (const OT*)p.x + (row0 + r0 + j) * p.k;
-                            if (p.x_vec) load8<OT, true>(v[j], row, col, p.k);
-                            else load8<OT, false>(v[j], row, col, p.k);
+                            const int64_t end = r0 + j < rows ? p.k : 0;
+                            if (p.x_vec) v[j].template load<true>(row, col, end);
+                            else v[j].template load<false>(row, col, end);
                         }
                         if (!ready) {
                             if (!mbar_wait_warp(empty(warp - 2), ((uint32_t)(seq >> 3) & 1u) ^ 1u, ok_flag)) { ok = false; break; }
@@ -241,14 +241,9 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
                         for (int j = 0; j < 4; ++j) {
                             const int r = r0 + j;
                             if (r >= rows) break;
-                            uint32_t mx = amax8_bits(v[j]);
-                            mx = max(mx, __shfl_xor_sync(DC_FULL, mx, 1));
-                            mx = max(mx, __shfl_xor_sync(DC_FULL, mx, 2));
-                            const uint32_t sb = mx4_scale_byte(mx);
-                            *reinterpret_cast<uint32_t*>(codes + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = encode_scaled(v[j], sb);
-                            uint32_t word = sb << (8 * ((lane >> 2) & 3));
-                            word |= __shfl_xor_sync(DC_FULL, word, 4);
-                            word |= __shfl_xor_sync(DC_FULL, word, 8);
+                            uint32_t sb;
+                            *reinterpret_cast<uint32_t*>(codes + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = mx4_encode_lane<OT>(v[j], sb);
+                            const uint32_t word = mx4_scale_quad(sb, lane);
                             if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(codes + Cfg::kB + 1024 + (lane >> 4) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
                         }
                     }
