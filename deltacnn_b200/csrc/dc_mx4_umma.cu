@@ -663,7 +663,7 @@ static int mx4_product(const void* x, const void* a_data, const void* a_scales, 
 }
 
 static bool mx4_sizes_ok(int64_t m, int64_t n, int64_t k) {
-    return m >= 0 && n >= 0 && k > 0 && m <= 0x7fffff00LL && n <= 0x7fffff00LL && k <= 0x7fffff00LL;
+    return m >= 0 && n >= 0 && k > 0 && m <= 0x7ffff000LL && n <= 0x7ffff000LL && k <= 0x7ffff000LL;
 }
 
 int mx4_error_code() {
