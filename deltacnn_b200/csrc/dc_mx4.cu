@@ -69,8 +69,16 @@ __global__ void __launch_bounds__(256) k_mx4_rows(const T* __restrict__ x, uint8
 }
 
 constexpr int kTile = 128;             // rows and columns of a tile
+// Where a value of the tile stands: rows in 16-byte pieces, the pieces of a row exchanged so that eight lanes that read the
+// same piece of four blocks of two rows, and the eight column pairs x four 32-row blocks of a warp (the rows' skew of 16
+// values per 32 rows), meet in no bank.
 template <typename T> __host__ __device__ constexpr int tile_bytes() { return (kTile * kTile + 3 * 16) * (int)sizeof(T); }
-template <typename T> __device__ __forceinline__ int tile_at(int r, int c) { return (r * kTile + (r >> 5) * 16 + c) * (int)sizeof(T); }
+template <typename T> __device__ __forceinline__ int tile_at(int r, int c) {
+    constexpr int N = VecTraits<T>::kVec;
+    const int piece = c / N, block = c >> 5;
+    const int moved = sizeof(T) == 4 ? piece ^ block ^ ((r & 1) << 2) : piece ^ (block >> 1) ^ ((r & 1) << 1);
+    return (r * kTile + (r >> 5) * 16) * (int)sizeof(T) + moved * 16 + (c % N) * (int)sizeof(T);
+}
 
 struct MxTileParams {
     const void* x;
@@ -80,127 +88,161 @@ struct MxTileParams {
     int tiles_x, tiles_y;
 };
 
-// One tile into shared memory, zeros outside the matrix. VEC: asynchronous copies (the caller commits and waits).
-template <typename T, bool VEC>
-__device__ __forceinline__ void mx4_fetch(const MxTileParams& p, uint8_t* tile, int64_t r0, int64_t c0) {
-    constexpr int N = VecTraits<T>::kVec, kPacks = kTile / N;
-#pragma unroll 4
-    for (int i = threadIdx.x; i < kTile * kPacks; i += 256) {
-        const int r = i / kPacks, c = (i % kPacks) * N;
-        const T* src = (const T*)p.x + (r0 + r) * p.cols + c0 + c;
+// One tile into shared memory, zeros outside the matrix, in asynchronous copies of 16 bytes or of 4 (rows that only allow
+// that), which the caller commits and waits for, or (COPY 0) element by element.
+template <typename T, int COPY>
+__device__ __forceinline__ void mx4_fetch(const MxTileParams& p, uint8_t* tile, int it) {
+    constexpr int N = COPY > 0 ? COPY / (int)sizeof(T) : VecTraits<T>::kVec, kPacks = kTile / N;
+    const int ty = it / p.tiles_x;
+    const int64_t r0 = (int64_t)ty * kTile;
+    const int c0 = (it - ty * p.tiles_x) * kTile;
+    // a thread's column is the same in every round
+    const int c = (int)(threadIdx.x % kPacks) * N, rows = (int)(p.rows - r0 < kTile ? p.rows - r0 : kTile), cols = (int)p.cols - c0;
+    const T* src = (const T*)p.x + (r0 + threadIdx.x / kPacks) * p.cols + c0 + c;
+    const int64_t step = (int64_t)(256 / kPacks) * p.cols;
+#pragma unroll 8
+    for (int r = threadIdx.x / kPacks; r < kTile; r += 256 / kPacks, src += step) {
         uint8_t* dst = tile + tile_at<T>(r, c);
-        if constexpr (VEC) {
-            const bool in = r0 + r < p.rows && c0 + c < p.cols;
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(in ? src : (const T*)p.x),
-                         "r"(in ? 16 : 0) : "memory");
+        if constexpr (COPY > 0) {
+            const bool in = r < rows && c < cols;
+            const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+            if constexpr (COPY == 16)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(in ? src : (const T*)p.x), "r"(in ? 16 : 0) : "memory");
+            else
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(in ? src : (const T*)p.x), "r"(in ? 4 : 0) : "memory");
         } else {
             Pack<T, N> v;
 #pragma unroll
-            for (int j = 0; j < N; ++j) v.s[j] = r0 + r < p.rows && c0 + c + j < p.cols ? src[j] : from_f<T>(0.f);
+            for (int j = 0; j < N; ++j) v.s[j] = r < rows && c + j < cols ? src[j] : from_f<T>(0.f);
             v.store(reinterpret_cast<T*>(dst));
         }
     }
 }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(256) k_mx4_tile(MxTileParams p) {
+// Thirty-two values (already multiplied by the factor, two at a time) as 16 bytes of codes; f(i) gives values i and i + 1.
+template <typename F> __device__ __forceinline__ uint4 mx4_encode32(F&& f) {
+    uint32_t c[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float u[8];
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) { const float2 x = f(j * 8 + i); u[i] = x.x; u[i + 1] = x.y; }
+        c[j] = mx4_encode8(u);
+    }
+    return make_uint4(c[0], c[1], c[2], c[3]);
+}
+
+template <typename T, int COPY, bool SUMS>
+__global__ void __launch_bounds__(256, sizeof(T) == 4 ? 1 : 3) k_mx4_tile(MxTileParams p) {
     extern __shared__ __align__(16) uint8_t tiles_smem[];
     __shared__ float sums[4][kTile];
     grid_dep_launch();
     grid_dep_wait();
+    constexpr int N = VecTraits<T>::kVec, kWords = 32 * (int)sizeof(T) / 4;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t nb = mx4_blocks(p.cols), tiles = mx4_scale_tiles(p.cols), nbt = mx4_blocks(p.rows), tiles_t = mx4_scale_tiles(p.rows);
+    const int nb = (int)mx4_blocks(p.cols), tiles = (int)mx4_scale_tiles(p.cols), nbt = (int)mx4_blocks(p.rows), tiles_t = (int)mx4_scale_tiles(p.rows);
     const int count = p.tiles_x * p.tiles_y;
-    if constexpr (VEC) {
-        mx4_fetch<T, VEC>(p, tiles_smem, (int64_t)(blockIdx.x / p.tiles_x) * kTile, (int64_t)(blockIdx.x % p.tiles_x) * kTile);
+    if constexpr (COPY > 0) {
+        mx4_fetch<T, COPY>(p, tiles_smem, blockIdx.x);
         asm volatile("cp.async.commit_group;" ::: "memory");
     }
-    for (int it = blockIdx.x, buf = 0; it < count; it += gridDim.x, buf ^= VEC ? 1 : 0) {
+    for (int it = blockIdx.x, buf = 0; it < count; it += gridDim.x, buf ^= COPY > 0 ? 1 : 0) {
         const int ty = it / p.tiles_x, tx = it - ty * p.tiles_x;
-        const int64_t r0 = (int64_t)ty * kTile, c0 = (int64_t)tx * kTile;
+        const int64_t r0 = (int64_t)ty * kTile;
+        const int c0 = tx * kTile;
         uint8_t* tile = tiles_smem + buf * tile_bytes<T>();
-        if constexpr (VEC) {
-            const int nt = it + gridDim.x;
-            if (nt < count) mx4_fetch<T, VEC>(p, tiles_smem + (buf ^ 1) * tile_bytes<T>(), (int64_t)(nt / p.tiles_x) * kTile, (int64_t)(nt % p.tiles_x) * kTile);
+        if constexpr (COPY > 0) {
+            if (it + (int)gridDim.x < count) mx4_fetch<T, COPY>(p, tiles_smem + (buf ^ 1) * tile_bytes<T>(), it + gridDim.x);
             asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 1;" ::: "memory");
         } else {
-            mx4_fetch<T, VEC>(p, tile, r0, c0);
+            mx4_fetch<T, COPY>(p, tile, it);
         }
         __syncthreads();
-        // the rows: sixteen lanes a row (eight values each), so a warp takes two rows at a time
+        // the rows: a lane takes a block, a warp the four blocks of eight rows, twice
         if (p.data != nullptr) {
-            const int lc = (lane & 15) * 8;
-#pragma unroll 4
-            for (int q = 0; q < kTile / 16; ++q) {
-                const int tr = q * 16 + warp * 2 + (lane >> 4);
-                const int64_t r = r0 + tr;
-                Eight<T> v;
+#pragma unroll 1
+            for (int q = 0; q < 2; ++q) {
+                const int tr = q * 64 + warp * 8 + (lane >> 2), blk = lane & 3;
+                uint32_t w[kWords], m = 0u;
 #pragma unroll
-                for (int k = 0; k < Eight<T>::kWords / 4; ++k) reinterpret_cast<uint4*>(v.w)[k] = reinterpret_cast<const uint4*>(tile + tile_at<T>(tr, lc))[k];
-                uint32_t s;
-                const uint32_t code = mx4_encode_lane<T>(v, s);
-                if (r < p.rows && (c0 + lc) >> 5 < nb) *reinterpret_cast<uint32_t*>(p.data + r * nb * 16 + ((c0 + lc) >> 1)) = code;
-                const uint32_t word = mx4_scale_quad(s, lane);
-                if ((lane & 15) == 0 && r < p.rows) *reinterpret_cast<uint32_t*>(p.scales + mx4_scale_word(r, tx, tiles)) = word;
+                for (int k = 0; k < kWords / 4; ++k) reinterpret_cast<uint4*>(w)[k] = *reinterpret_cast<const uint4*>(tile + tile_at<T>(tr, blk * 32 + k * N));
+#pragma unroll
+                for (int k = 0; k < kWords; ++k) m = amax_word<T>(m, w[k]);
+                const uint32_t s = mx4_scale_byte(amax_bits<T>(m));
+                const float f = mx4_factor(s);
+                uint4 code = mx4_encode32([&](int i) {
+                    float2 x;
+                    if constexpr (sizeof(T) == 4) x = make_float2(__uint_as_float(w[i]), __uint_as_float(w[i + 1]));
+                    else x = word_values<T>(w[i / 2]);
+                    mul2(x.x, x.y, f, f);
+                    return x;
+                });
+                if (s == 255u) code = make_uint4(0u, 0u, 0u, 0u);
+                const int64_t r = r0 + tr;
+                if (tr < p.rows - r0) {
+                    if (tx * 4 + blk < nb) *reinterpret_cast<uint4*>(p.data + (r * nb + tx * 4 + blk) * 16) = code;
+                    p.scales[mx4_scale_word(r, tx, tiles) + blk] = (uint8_t)s;
+                }
             }
         }
         // the columns: a thread takes two columns of a 32-row block; a warp 8 column pairs x the 4 blocks
         const int pair = warp * 8 + (lane & 7), blk = lane >> 3;
-        const uint8_t* col = tile + tile_at<T>(blk * 32, pair * 2);
         uint32_t m[2] = {0u, 0u};
+        uint32_t w[sizeof(T) == 4 ? 64 : 32];          // both columns, row by row
         float sum[2] = {0.f, 0.f};
-        uint32_t code[2][4], s[2];
-        auto values = [&](int i) {           // row i of the block: both columns
-            if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float2*>(col + i * kTile * 4);
-            else return word_values<T>(*reinterpret_cast<const uint32_t*>(col + i * kTile * 2));
-        };
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll 8
-            for (int i = 0; i < 32; ++i) {
-                const float2 f = values(i);
-                m[0] = amax_word<float>(m[0], __float_as_uint(f.x));
-                m[1] = amax_word<float>(m[1], __float_as_uint(f.y));
-            }
-        } else {
-            uint32_t both = 0u;
 #pragma unroll
-            for (int i = 0; i < 32; ++i) both = amax_word<T>(both, *reinterpret_cast<const uint32_t*>(col + i * kTile * 2));
-            const float2 f = word_values<T>(both);
+        for (int i = 0; i < 32; ++i) {
+            const uint8_t* at = tile + tile_at<T>(blk * 32 + i, pair * 2);
+            if constexpr (sizeof(T) == 4) {
+                *reinterpret_cast<uint2*>(&w[2 * i]) = *reinterpret_cast<const uint2*>(at);
+                m[0] = amax_word<float>(m[0], w[2 * i]);
+                m[1] = amax_word<float>(m[1], w[2 * i + 1]);
+            } else {
+                w[i] = *reinterpret_cast<const uint32_t*>(at);
+                m[0] = amax_word<T>(m[0], w[i]);
+            }
+        }
+        if constexpr (sizeof(T) == 2) {
+            const float2 f = word_values<T>(m[0]);
             m[0] = __float_as_uint(f.x);
             m[1] = __float_as_uint(f.y);
         }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) s[k] = mx4_scale_byte(m[k]);
+        const uint32_t s[2] = {mx4_scale_byte(m[0]), mx4_scale_byte(m[1])};
         const float f0 = mx4_factor(s[0]), f1 = mx4_factor(s[1]);
+        uint32_t code[2][4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             float u[2][8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                float2 f = values(j * 8 + i);
-                if (p.colsum != nullptr) { sum[0] += f.x; sum[1] += f.y; }
+                float2 f;
+                if constexpr (sizeof(T) == 4) f = make_float2(__uint_as_float(w[2 * (j * 8 + i)]), __uint_as_float(w[2 * (j * 8 + i) + 1]));
+                else f = word_values<T>(w[j * 8 + i]);
+                if constexpr (SUMS) { sum[0] += f.x; sum[1] += f.y; }
                 mul2(f.x, f.y, f0, f1);
                 u[0][i] = f.x;
                 u[1][i] = f.y;
             }
-            code[0][j] = s[0] == 255u ? 0u : mx4_encode8(u[0]);
-            code[1][j] = s[1] == 255u ? 0u : mx4_encode8(u[1]);
+            code[0][j] = mx4_encode8(u[0]);
+            code[1][j] = mx4_encode8(u[1]);
         }
         if (p.data_t != nullptr) {
+            const int b = ty * 4 + blk;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const int64_t c = c0 + pair * 2 + k, b = (int64_t)ty * 4 + blk;
+                const int c = c0 + pair * 2 + k;
                 if (c < p.cols) {
-                    if (b < nbt) *reinterpret_cast<uint4*>(p.data_t + (c * nbt + b) * 16) = make_uint4(code[k][0], code[k][1], code[k][2], code[k][3]);
+                    const uint4 v = s[k] == 255u ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(code[k][0], code[k][1], code[k][2], code[k][3]);
+                    if (b < nbt) *reinterpret_cast<uint4*>(p.data_t + ((int64_t)c * nbt + b) * 16) = v;
                     p.scales_t[mx4_scale_word(c, ty, tiles_t) + blk] = (uint8_t)s[k];
                 }
             }
         }
-        if (p.colsum != nullptr) {
+        if constexpr (SUMS) {
             sums[blk][pair * 2] = sum[0];
             sums[blk][pair * 2 + 1] = sum[1];
             __syncthreads();
-            if (threadIdx.x < kTile && c0 + threadIdx.x < p.cols)
+            if (threadIdx.x < kTile && c0 + (int)threadIdx.x < p.cols)
                 p.colsum[ty * p.cols + c0 + threadIdx.x] =
                     (sums[0][threadIdx.x] + sums[1][threadIdx.x]) + (sums[2][threadIdx.x] + sums[3][threadIdx.x]);
         }
@@ -208,14 +250,18 @@ __global__ void __launch_bounds__(256) k_mx4_tile(MxTileParams p) {
     }
 }
 
-// The way of k_mx4_rows back: a warp takes four chunks of 256 values of a row, a lane eight codes of each.
+// The way of k_mx4_rows back: a warp takes four chunks of 256 values of a row, a lane eight codes of each. Rows that do not
+// allow 16-byte stores go through shared memory, so that neighbouring lanes store neighbouring words (rows of an even number of
+// bytes over 4) or elements.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restrict__ data, const uint8_t* __restrict__ scales, T* __restrict__ out,
                                                         int cols, MxWalk w) {
     grid_dep_launch();
     grid_dep_wait();
+    __shared__ __align__(16) T turn[VEC ? 1 : 8][VEC ? 1 : kMxChunk];
     const int lane = threadIdx.x & 31;
     const int nb = (int)mx4_blocks(cols), tiles = (int)mx4_scale_tiles(cols);
+    const bool words = sizeof(T) == 4 || (((reinterpret_cast<uintptr_t>(out) & 3u) == 0) && (cols & 1) == 0);
     for (MxPlace at(w); at.row < w.rows; at.next(w)) {
         const int c0 = at.seg * (kMxChunk * kMxAhead) + lane * 8;
         const uint8_t* row = data + at.row * nb * 16;
@@ -237,28 +283,64 @@ __global__ void __launch_bounds__(256) k_mx4_dequantize(const uint8_t* __restric
             mx4_decode8(code[a], v);
 #pragma unroll
             for (int i = 0; i < 4; ++i) mul2(v[2 * i], v[2 * i + 1], f, f);
-            if constexpr (VEC) {
-                constexpr int N = VecTraits<T>::kVec;
+            constexpr int N = VecTraits<T>::kVec;
 #pragma unroll
-                for (int k = 0; k < 8 / N; ++k) {
-                    Pack<T, N> q;
+            for (int k = 0; k < 8 / N; ++k) {
+                Pack<T, N> q;
 #pragma unroll
-                    for (int i = 0; i < N; ++i) q.set(i, v[k * N + i]);
-                    if (col + k * N < cols) q.store(o + k * N);
+                for (int i = 0; i < N; ++i) q.set(i, v[k * N + i]);
+                if constexpr (VEC) { if (col + k * N < cols) q.store(o + k * N); }
+                else q.store(&turn[threadIdx.x >> 5][lane * 8 + k * N]);
+            }
+            if constexpr (!VEC) {
+                const T* mine = turn[threadIdx.x >> 5];
+                T* start = o - lane * 8;
+                const int left = cols - (col - lane * 8);          // values of the row from this chunk on
+                __syncwarp();
+                if (words) {
+                    constexpr int M = 4 / (int)sizeof(T);
+#pragma unroll
+                    for (int i = 0; i < kMxChunk / M; i += 32)
+                        if ((i + lane) * M < left) reinterpret_cast<uint32_t*>(start)[i + lane] = reinterpret_cast<const uint32_t*>(mine)[i + lane];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kMxChunk; i += 32)
+                        if (i + lane < left) start[i + lane] = mine[i + lane];
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (col + i < cols) o[i] = from_f<T>(v[i]);
+                __syncwarp();
             }
         }
     }
 }
 
+template <typename T, int COPY, bool SUMS>
+static int launch_tile(const MxTileParams& p, cudaStream_t st) {
+    // two tiles of shared memory per CTA where the next one is on its way while a tile is encoded
+    constexpr int smem = (COPY > 0 ? 2 : 1) * tile_bytes<T>();
+    static PerDeviceOnce once;
+    bool* set = once.slot();
+    if (set == nullptr) return DC_ERR_LAUNCH;
+    if (!*set) {
+        if (cudaFuncSetAttribute(k_mx4_tile<T, COPY, SUMS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return check_launch();
+        *set = true;
+    }
+    const int cap = sm_count() * (sizeof(T) == 4 ? 1 : 3), count = p.tiles_x * p.tiles_y;
+    return launch_pdl(k_mx4_tile<T, COPY, SUMS>, dim3((unsigned)(count < cap ? count : cap)), dim3(256), smem, st, p);
+}
+template <typename T, bool SUMS>
+static int launch_tile_copy(const MxTileParams& p, cudaStream_t st) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(p.x);
+    const int64_t pitch = p.cols * (int64_t)sizeof(T);
+    if ((x & 15u) == 0 && pitch % 16 == 0) return launch_tile<T, 16, SUMS>(p, st);
+    if ((x & 3u) == 0 && pitch % 4 == 0) return launch_tile<T, 4, SUMS>(p, st);
+    if constexpr (sizeof(T) == 2) return launch_tile<T, 0, SUMS>(p, st);
+    return DC_ERR_ALIGNMENT;          // float32 off 4 bytes
+}
+
 template <typename T>
 static int quantize_t(const void* x, void* data, void* scales, void* data_t, void* scales_t, float* colsum, int64_t rows, int64_t cols, cudaStream_t st) {
-    const bool vec = aligned16(x) && cols % VecTraits<T>::kVec == 0;
     if (data_t == nullptr && colsum == nullptr) {
+        const bool vec = aligned16(x) && cols % VecTraits<T>::kVec == 0;
         const int segments = (int)divup64(mx4_scale_tiles(cols) * 128, kMxChunk * kMxAhead);
         int64_t ctas = divup64(rows * segments, 8);
         const int64_t cap = (int64_t)sm_count() * 5;
@@ -268,22 +350,9 @@ static int quantize_t(const void* x, void* data, void* scales, void* data_t, voi
         return launch_pdl(k_mx4_rows<T, false>, dim3((unsigned)ctas), dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, (int)cols, w);
     }
     const int64_t tx = divup64(cols, kTile), ty = divup64(rows, kTile);
-    if (tx * ty > 0x3fffffffLL) return DC_ERR_SHAPE;
-    MxTileParams p{x, (uint8_t*)data, (uint8_t*)scales, (uint8_t*)data_t, (uint8_t*)scales_t, colsum, rows, cols, (int)tx, (int)ty};
-    static PerDeviceOnce once;
-    bool* set = once.slot();
-    if (set == nullptr) return DC_ERR_LAUNCH;
-    if (!*set) {
-        if (cudaFuncSetAttribute(k_mx4_tile<T, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 2 * tile_bytes<T>()) != cudaSuccess ||
-            cudaFuncSetAttribute(k_mx4_tile<T, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, tile_bytes<T>()) != cudaSuccess)
-            return check_launch();
-        *set = true;
-    }
-    // VEC: two tiles of shared memory per CTA, the next one on its way while a tile is encoded
-    const int64_t cap = (int64_t)sm_count() * (sizeof(T) == 4 ? (vec ? 1 : 3) : (vec ? 3 : 4));
-    const dim3 grid((unsigned)(tx * ty < cap ? tx * ty : cap));
-    if (vec) return launch_pdl(k_mx4_tile<T, true>, grid, dim3(256), 2 * tile_bytes<T>(), st, p);
-    return launch_pdl(k_mx4_tile<T, false>, grid, dim3(256), tile_bytes<T>(), st, p);
+    if (tx * ty > 0x3fffffffLL || rows > 0x7ffff000LL) return DC_ERR_SHAPE;
+    const MxTileParams p{x, (uint8_t*)data, (uint8_t*)scales, (uint8_t*)data_t, (uint8_t*)scales_t, colsum, rows, cols, (int)tx, (int)ty};
+    return colsum != nullptr ? launch_tile_copy<T, true>(p, st) : launch_tile_copy<T, false>(p, st);
 }
 
 template <typename T>
