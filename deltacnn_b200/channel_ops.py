@@ -7,6 +7,8 @@ the delta path, float32 and float16). As everywhere in this package there is no 
 memory format raises before a launch, and launches go to torch's current stream on the tensor's device; an argument is never
 copied to make it fit, except an incoming gradient, whose layout the caller cannot choose.
 """
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -32,20 +34,11 @@ def _launch(op, fn, t, *args):
         check(status, op)
 
 
-class _device:
-    """Makes a tensor's device the current one (nothing to do on the usual path)."""
-    __slots__ = ("guard",)
-
-    def __init__(self, t):
-        self.guard = torch.cuda.device(t.device) if t.get_device() != torch.cuda.current_device() else None
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+@functools.lru_cache(maxsize=4096)
+def _bytes_wanted(query, index, *sizes):
+    """A workspace query of the library (its answer depends on the sizes and on the device's SMs)."""
+    with torch.cuda.device(index):
+        return getattr(lib, query)(*sizes)
 
 
 def _fail(op, text):
@@ -111,7 +104,7 @@ def _ln_forward(x, rows, c, weight, bias, eps, keep):
     y = torch.empty_like(x)
     stats = mean = rstd = None
     if keep:
-        stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        stats = x.new_empty((2, rows), dtype=torch.float32)
         mean = stats.data_ptr()
         rstd = mean + 4 * rows
     if rows > 0:
@@ -143,14 +136,13 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty_like(x) if need_x else None
         dw = x.new_empty(c, dtype=wtype) if need_w else None
         db = x.new_empty(c, dtype=wtype) if need_b else None
-        ws, floats = None, 0
+        ws, nbytes = None, 0
         if need_w or need_b:
-            with _device(x):
-                floats = lib.dc_layer_norm_backward_workspace_bytes(rows, c, code) // 4
-            ws = x.new_empty(floats, dtype=torch.float32)
+            nbytes = _bytes_wanted("dc_layer_norm_backward_workspace_bytes", x.get_device(), rows, c, code)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
         mean = stats.data_ptr()
         _launch("layer_norm_backward", lib.dc_layer_norm_backward, x, dy.data_ptr(), x.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw),
-                _ptr(db), rows, c, code, _CODES[wtype], _ptr(ws), 4 * floats)
+                _ptr(db), rows, c, code, _CODES[wtype], _ptr(ws), nbytes)
         return dx, dw, db, None
 
     @staticmethod
@@ -261,7 +253,7 @@ def _quantize(x, rows, cols, along_rows, along_cols, colsum=None):
     ws, nbytes, sum_code = None, 0, 0
     if colsum is not None:
         nbytes, sum_code = lib.dc_mx4_colsum_workspace_bytes(rows, cols), _CODES[colsum.dtype]
-        ws = x.new_empty(nbytes // 4, dtype=torch.float32)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
     if rows > 0 or colsum is not None:
         _launch("mx4_quantize", lib.dc_mx4_quantize, x, x.data_ptr(), *(q._ptrs() if q is not None else _NONE), *(qt._ptrs() if qt is not None else _NONE),
                 _ptr(colsum), rows, cols, code, sum_code, _ptr(ws), nbytes)
@@ -409,8 +401,7 @@ def mx4_linear(x, weight, bias=None):
         weight = _quantize(weight, outs, cols, True, False)[0]
     out = x.new_empty((rows, outs))
     if rows > 0 and outs > 0:
-        with _device(x):
-            nbytes = lib.dc_mx4_linear_workspace_bytes(rows, outs, cols)
+        nbytes = _bytes_wanted("dc_mx4_linear_workspace_bytes", x.get_device(), rows, outs, cols)
         ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _launch(op, lib.dc_mx4_linear, x, x.data_ptr(), *weight._ptrs(), _ptr(bias), out.data_ptr(), rows, outs, cols, code,
                 0 if bias is None else _CODES[bias.dtype], _ptr(ws), nbytes)
