@@ -12,8 +12,8 @@
 // memory. Roles: one thread issues the copies, one the scale copies and MMAs, four warps drain accumulators; persistent CTAs,
 // two accumulators.
 //
-// dc_mx4_linear on few tokens packs them in the same kernel: eight warps, one per stage, quantise a step's rows straight into
-// it, in the swizzled layout that the TMA would have written, and arrive on the stage's barrier beside the copies.
+// dc_mx4_linear on few tokens packs them in the same kernel: eight warps quantise a step's rows straight into the stage, in the
+// swizzled layout that the TMA would have written, and arrive on the stage's barrier beside the copies.
 //
 // Bound: many tokens, the tensor core and the shared memory that feeds it; few tokens, the weight's bytes. Then the tiles
 // do not fill the GPU, and the CTAs of a cluster share a tile along k: each leaves its float32 sums in its own shared
@@ -28,7 +28,7 @@ __device__ int g_mx4_error = 0;
 
 constexpr int kMxThreads = 192;            // TMA warp, MMA warp, four epilogue warps
 constexpr int kMxQuantThreads = 320;       // with the tokens quantised on the way: eight warps for that, four of them drain
-constexpr int kMxQuantRows = 4;            // tokens that dc_mx4_linear packs inside the product
+constexpr int kMxQuantRounds = 2;          // rounds of eight warps that dc_mx4_linear spends on packing inside the product, at most
 constexpr int kMxStep = 256;               // values of k per step: one 128-byte row
 constexpr uint32_t kMxTmem = 512;
 
@@ -46,7 +46,7 @@ template <int NT> struct MxCfg {
 struct MxGemmParams {
     const uint8_t *a_sc, *b_sc;            // scales of the tokens, of the features
     const void* x;                         // tokens in the result's type, where they are quantised on the way
-    int k, x_vec;                          // their width; rows allow 16-byte reads
+    int k, x_vec, groups;                  // their width; rows allow 16-byte reads; groups of eight rows
     const void* bias;
     void* out;
     int64_t m;
@@ -122,7 +122,7 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
     auto acc_full = [&](int a) { return bar0 + 8u * (2 * S + a); };
     auto acc_empty = [&](int a) { return bar0 + 8u * (2 * S + 2 + a); };
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S; ++s) { mbar_init(full(s), QUANT ? 2 : 1); mbar_init(empty(s), 1); }
+        for (int s = 0; s < S; ++s) { mbar_init(full(s), QUANT ? 1 + p.groups : 1); mbar_init(empty(s), 1); }
         for (int a = 0; a < 2; ++a) { mbar_init(acc_full(a), 1); mbar_init(acc_empty(a), 4); }
         *ok_flag = 1;
         fence_barrier_init();
@@ -212,45 +212,41 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
             const int a = it & 1, use = it >> 1;
             const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
             if constexpr (QUANT) {
-                // Warp w packs the steps of stage w - 2, 256 values of every token, straight into the stage: a row at a time,
-                // four rows' reads in flight; eight values a lane, 16-byte pieces in the 128-byte swizzle, the scales of four
-                // blocks as one word of the scale tile.
-                static_assert(S == 8, "a stage per warp");
+                // A step's 256 values of every token, straight into the stage, in groups of eight rows; groups of a step and
+                // steps go round the eight warps. A warp has the eight rows' reads in flight; a lane takes eight values of a
+                // row, 16-byte pieces in the 128-byte swizzle, the scales of four blocks as one word of the scale tile.
                 const int64_t row0 = (int64_t)tt * NT;
                 const int rows = (int)(p.m - row0 < NT ? p.m - row0 : NT);
-                uint8_t* codes = raw + (ring - smem_u32(raw)) + (warp - 2) * Cfg::kStage + kABytes;
                 bool ok = true;
-                for (int ks = k_lo; ks < k_hi; ++ks, ++seq) {
-                    if ((int)(seq & 7u) != warp - 2) continue;
-                    const int64_t col = (int64_t)ks * kMxStep + lane * 8;
-                    bool ready = false;
-                    for (int r0 = 0; r0 < rows; r0 += 4) {
-                        Eight<OT> v[4];
+                for (int ks = k_lo; ks < k_hi && ok; ++ks, ++seq) {
+                    const int s = (int)(seq % S);
+                    uint8_t* codes = raw + (ring - smem_u32(raw)) + s * Cfg::kStage + kABytes;
+                    for (int g = 0; g < p.groups; ++g) {
+                        if ((int)((seq * p.groups + g) & 7u) != warp - 2) continue;
+                        const int64_t col = (int64_t)ks * kMxStep + lane * 8;
+                        Eight<OT> v[8];
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const OT* row = (const OT*)p.x + (row0 + r0 + j) * p.k;
-                            const int64_t end = r0 + j < rows ? p.k : 0;
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = g * 8 + j;
+                            const OT* row = (const OT*)p.x + (row0 + r) * p.k;
+                            const int64_t end = r < rows ? p.k : 0;
                             if (p.x_vec) v[j].template load<true>(row, col, end);
                             else v[j].template load<false>(row, col, end);
                         }
-                        if (!ready) {
-                            if (!mbar_wait_warp(empty(warp - 2), ((uint32_t)(seq >> 3) & 1u) ^ 1u, ok_flag)) { ok = false; break; }
-                            ready = true;
-                        }
+                        if (!mbar_wait_warp(empty(s), ((uint32_t)(seq / S) & 1u) ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 9); ok = false; break; }
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int r = r0 + j;
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = g * 8 + j;
                             if (r >= rows) break;
                             uint32_t sb;
                             *reinterpret_cast<uint32_t*>(codes + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) = mx4_encode_lane<OT>(v[j], sb);
                             const uint32_t word = mx4_scale_quad(sb, lane);
                             if ((lane & 15) == 0) *reinterpret_cast<uint32_t*>(codes + Cfg::kB + 1024 + (lane >> 4) * 512 + (r & 31) * 16 + (r >> 5) * 4) = word;
                         }
+                        fence_proxy_async();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(full(s));
                     }
-                    if (!ok) { *ok_flag = 0; atomicExch(&g_mx4_error, 9); break; }
-                    fence_proxy_async();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(full(warp - 2));
                 }
                 if (!ok) break;
                 if (warp >= 6) continue;
@@ -592,7 +588,13 @@ static int launch_mx4(const MxGemmParams& p, int split, const CUtensorMap& ma, c
 
 template <typename OT, bool SPLIT>
 static int launch_mx4_nt(int nt, const MxGemmParams& p, int split, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
-    if (p.x != nullptr) return launch_mx4<OT, 16, SPLIT, true>(p, split, ma, mb, st);      // kMxQuantRows <= 16
+    if (p.x != nullptr) {
+        switch (nt) {
+            case 16: return launch_mx4<OT, 16, SPLIT, true>(p, split, ma, mb, st);
+            case 32: return launch_mx4<OT, 32, SPLIT, true>(p, split, ma, mb, st);
+            default: return launch_mx4<OT, 64, SPLIT, true>(p, split, ma, mb, st);
+        }
+    }
     switch (nt) {
         case 16: return launch_mx4<OT, 16, SPLIT, false>(p, split, ma, mb, st);
         case 32: return launch_mx4<OT, 32, SPLIT, false>(p, split, ma, mb, st);
@@ -622,9 +624,12 @@ static MxPlan mx4_plan(int64_t m, int64_t n, int64_t k) {
     pl.tiles = divup64(n, 128) * divup64(m, pl.nt);
     // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each
     while (pl.split < 8 && pl.tiles * pl.split * 2 <= sms && steps >= pl.split * 2) pl.split *= 2;
-    // Quantising inside makes every feature tile read the tokens unpacked and wait for a row's 1 us of latency per four rows and
-    // step: 4096 -> 14336 takes 9.7 us for one token (2.6 + 9.4 us with a launch of its own) 11.5 us for four, 15.6 us for eight (2.7 + 9.6).
-    pl.quant = m <= kMxQuantRows;
+    // Quantising inside makes every feature tile's CTA read the tokens unpacked: eight rows of a step and warp at a time, which
+    // waits for their 1 us of latency in every round of the eight warps. Device time inside / with a launch of its own (2.2 us of
+    // it), bf16: one round, 1 x 4096 -> 14336, 10.0 / 11.8 us; two, 8 x 4096 -> 14336, 11.4 / 11.7, and 64 x 1280 -> 1000, 12.3 /
+    // 11.5 (but a call of the host costs 5 us less); four, 16 x 4096 -> 14336, 16.4 / 12.1.
+    const int64_t rounds = divup64(divup64(pl.tiles, sms) * divup(steps, pl.split) * divup64(m, 8), 8);
+    pl.quant = m <= 64 && rounds <= kMxQuantRounds;
     return pl;
 }
 
@@ -640,7 +645,7 @@ static int mx4_product(const void* x, const void* a_data, const void* a_scales, 
     p.out_even = (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
     p.tiles_f = (int)divup64(n, pl.pair ? 256 : 128);
     p.tiles = (int)pl.tiles;
-    p.x = x; p.k = (int)k;
+    p.x = x; p.k = (int)k; p.groups = (int)divup64(m < 64 ? m : 64, 8);
     p.x_vec = aligned16(x) && k % (out_dtype == DC_F32 ? 4 : 8) == 0;
     alignas(64) CUtensorMap ma, mb;
     if (!encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128)) return DC_ERR_UNSUPPORTED;
