@@ -191,6 +191,9 @@ def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, thr
     for t, name in ((mask, "mask"), (out_mask, "out_mask")):
         if t.device != delta.device or not t.is_contiguous():
             _fail(op, f"{name} must be contiguous and on {delta.device}")
+    if len({t.data_ptr() for t in (delta, prev_in, prev_out)}) < 3 or out.data_ptr() in (prev_in.data_ptr(), prev_out.data_ptr()):
+        if delta.numel() > 0:
+            _fail(op, "delta, prev_in and prev_out must be three tensors, and out none of the caches")
     _launch(op, lib.dc_layer_norm_delta, delta, delta.data_ptr(), mask.data_ptr(), prev_in.data_ptr(), prev_out.data_ptr(), _ptr(weight), _ptr(bias),
             out.data_ptr(), out_mask.data_ptr(), n * h * w, c, code, wcode, float(threshold), eps)
     return out, out_mask

@@ -143,7 +143,7 @@ class DCModule(nn.Module):
         for mod in self.modules():
             if type(mod) in (DCConv2d, DCConvTranspose2d):
                 mod.process_filters()
-            elif type(mod) is DCMX4Linear and mod is not self:
+            elif isinstance(mod, DCMX4Linear) and mod is not self:
                 mod.process_filters()
 
     def reset_layers(self):

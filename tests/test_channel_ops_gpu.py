@@ -60,7 +60,8 @@ def y_bound(w, b, n, a, y, t):
 # ---- layer norm ------------------------------------------------------------------------------------------------
 
 SHAPES = [(1, 1), (5, 1), (1, 8), (3, 7), (40, 24), (5, 33), (259, 64), (2, 96), (130, 100), (33, 1000), (7, 1024), (3, 1032), (6, 1001),
-          (2, 4096), (3, 4100), (2, 4099), (2, 8192), (3, 16384), (2, 20000), (1, 40000), (1500, 8), (700, 257)]
+          (2, 4096), (3, 4100), (2, 4099), (2, 8192), (3, 16384), (2, 20000), (1, 40000), (1500, 8), (700, 257),
+          (2, 9001), (3, 2500), (2, 10000), (80001, 96), (160001, 24), (30000, 512)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -165,6 +166,15 @@ def test_layer_norm_of_a_feature_map_is_per_pixel(dtype):
     assert torch.equal(dx.permute(0, 2, 3, 1).reshape(-1, 40), dxf) and torch.equal(dw, dwf)
 
 
+def test_gradients_of_gradients_are_refused():
+    g = gen(30)
+    x, w = randn((8, 64), g).requires_grad_(), randn((64,), g).requires_grad_()
+    for f in (lambda: dc().layer_norm(x, w), lambda: dc().mx4_linear(x, w.expand(32, 64).contiguous())):
+        first, = torch.autograd.grad(f().square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(first.square().sum(), x)
+
+
 def test_layer_norm_hard_values():
     g = gen(6)
     x = randn((8, 64), g)
@@ -218,7 +228,7 @@ def delta64(delta, mask, prev_in, prev_out, w, b, thr):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("n,h,w,c", [(1, 1, 1, 8), (2, 5, 7, 24), (3, 9, 11, 64), (1, 16, 16, 100), (2, 6, 6, 576), (1, 5, 5, 1280), (1, 3, 5, 33), (1, 3, 3, 1001), (1, 2, 3, 4096)])
+@pytest.mark.parametrize("n,h,w,c", [(1, 1, 1, 8), (2, 5, 7, 24), (3, 9, 11, 64), (1, 16, 16, 100), (2, 6, 6, 576), (1, 5, 5, 1280), (1, 3, 5, 33), (1, 3, 3, 1001), (1, 2, 3, 4096), (1, 2, 3, 8191), (1, 1, 2, 8192), (40, 30, 30, 72)])
 @pytest.mark.parametrize("density", [0.0, 0.3, 1.0])
 def test_layer_norm_delta(dtype, n, h, w, c, density):
     g = gen(c + int(density * 10))
@@ -564,6 +574,23 @@ def test_delta_module_follows_the_dense_norm(dtype):
         assert ln.first_iter and ln.prev_in is None
 
 
+def test_first_calls_inside_a_capture():
+    """Nothing that a first call of a shape sets up may disturb a capture."""
+    d = dc()
+    g = gen(31)
+    x, w, b, q = randn((37, 552), g, BF16), randn((552,), g, BF16), randn((552,), g, BF16), d.mx4_quantize(randn((776, 552), g))
+    tokens = randn((3, 552), g, BF16)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = d.layer_norm(x, w, b)
+        z, few = d.mx4_linear(y, q), d.mx4_linear(tokens, q)
+        both = d.mx4_quantize_both(y)
+    graph.replay()
+    assert torch.equal(y, d.layer_norm(x, w, b)) and torch.equal(z, d.mx4_linear(y, q)) and torch.equal(few, d.mx4_linear(tokens, q))
+    assert torch.equal(both[1].dequantize(), d.mx4_quantize_both(y)[1].dequantize())
+
+
 def test_streams():
     d = dc()
     g = gen(22)
@@ -599,11 +626,15 @@ def test_refusals():
     ]
     delta = torch.randn(1, 8, 4, 4, device="cuda").contiguous(memory_format=torch.channels_last)
     mask = torch.ones(1, 1, 4, 4, dtype=torch.int32, device="cuda")
+    wide = torch.zeros(1, 40000, 1, 1, device="cuda").contiguous(memory_format=torch.channels_last)      # no kernel for so many channels
     bad += [
         lambda: d.layer_norm_delta(delta.bfloat16(), mask, delta.bfloat16(), delta.bfloat16()),
         lambda: d.layer_norm_delta(delta, mask[:, :, :2], delta.clone(), delta.clone()),
         lambda: d.layer_norm_delta(delta, mask, delta.half(), delta.clone()),
         lambda: d.layer_norm_delta(delta, mask, delta.clone(), delta[:, :, :2].clone()),
+        lambda: d.layer_norm_delta(delta, mask, delta, delta.clone()),
+        lambda: d.layer_norm_delta(delta, mask, *[delta.clone()] * 2),
+        lambda: d.layer_norm_delta(wide, mask[:, :, :1, :1].contiguous(), wide.clone(), wide.clone()),
     ]
     for i, call in enumerate(bad):
         with pytest.raises(RuntimeError):
