@@ -533,6 +533,12 @@ static MxEncodeFn mx_encoder() {
     }();
     return fn;
 }
+// The encoder needs a context; a thread that has not called the runtime yet gets the current device's one and a second try.
+template <typename F> static bool mx_encode(F&& encode) {
+    if (encode() == CUDA_SUCCESS) return true;
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess && encode() == CUDA_SUCCESS;
+}
 static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int64_t row_bytes, int box_rows) {
     const MxEncodeFn fn = mx_encoder();
     if (fn == nullptr) return false;
@@ -540,8 +546,10 @@ static bool encode_mx4_map(CUtensorMap* map, const void* data, int64_t rows, int
     const cuuint64_t gstride[1] = {(cuuint64_t)row_bytes};
     const cuuint32_t box[2] = {128u, (cuuint32_t)box_rows};
     const cuuint32_t estride[2] = {1u, 1u};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return mx_encode([&] {
+        return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(data), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 // The scale tiles as rows of 128 words, a box of two consecutive tiles along k.
@@ -552,8 +560,10 @@ static bool encode_mx4_scales(CUtensorMap* map, const void* scales, int64_t tile
     const cuuint64_t gstride[1] = {512u};
     const cuuint32_t box[2] = {128u, 2u};
     const cuuint32_t estride[2] = {1u, 1u};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
-              CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    return mx_encode([&] {
+        return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 2, const_cast<void*>(scales), gdim, gstride, box, estride, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    });
 }
 
 template <typename OT>

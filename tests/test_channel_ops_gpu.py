@@ -591,6 +591,36 @@ def test_first_calls_inside_a_capture():
     assert torch.equal(both[1].dequantize(), d.mx4_quantize_both(y)[1].dequantize())
 
 
+def test_threads():
+    """First calls of threads that have not touched the device yet, several at once."""
+    import threading
+    d = dc()
+    g = gen(32)
+    x, q = randn((200, 256), g, F16), d.mx4_quantize(randn((500, 256), g))
+    want = d.mx4_linear(d.layer_norm(x), q)
+    torch.cuda.synchronize()
+    got, threads = [None] * 4, []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got[i] = d.mx4_linear(d.layer_norm(x), q)
+
+    def first(i):                                        # nothing but the product itself
+        got[i] = d.mx4_matmul(qx, q, None, F16)
+
+    qx = d.mx4_quantize(d.layer_norm(x))
+    torch.cuda.synchronize()
+    for i in range(4):
+        threads.append(threading.Thread(target=first if i == 0 else work, args=(i,)))
+        threads[-1].start()
+        if i == 0:
+            threads[-1].join()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want) for v in got)
+
+
 def test_streams():
     d = dc()
     g = gen(22)
