@@ -658,25 +658,34 @@ template <typename T, int W> __device__ __forceinline__ bool frag_any_above(cons
     }
 }
 
-// One pixel by its team; returns whether any channel's change is above the threshold (the same answer in the whole team).
-// Packs behind the last channel hold zeros all along.
-template <typename T, typename WT, int W, int P, bool BLOCK>
-__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, Frag<WT, W> (&w)[P], Frag<WT, W> (&b)[P],
-                                               float* red0, float* red1) {
-    const int64_t off = px * p.c + t.rank * W;
-    Frag<T, W> d[P], u[P], o[P];
-    bool valid[P];
+// What a team reads of a pixel; packs behind the last channel hold zeros.
+template <typename T, int W, int P> struct DeltaPixel {
+    Frag<T, W> d[P], u[P], o[P];           // the delta, the accumulated input, the accumulated output
+    template <bool BLOCK> __device__ __forceinline__ void load(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on) {
+        const int64_t off = px * p.c + t.rank * W;
 #pragma unroll
-    for (int k = 0; k < P; ++k) {
-        valid[k] = t.rank + k * t.size < p.nvec;
-        d[k].fill(0.f); u[k].fill(0.f); o[k].fill(0.f);
-        if (on && valid[k]) {
-            const int64_t at = off + k * t.size * W;
-            d[k].load((const T*)p.delta + at);
-            u[k].load((const T*)p.prev_in + at);
-            o[k].load((const T*)p.prev_out + at);
+        for (int k = 0; k < P; ++k) {
+            d[k].fill(0.f); u[k].fill(0.f); o[k].fill(0.f);
+            if (on && t.rank + k * t.size < p.nvec) {
+                const int64_t at = off + k * t.size * W;
+                d[k].load((const T*)p.delta + at);
+                u[k].load((const T*)p.prev_in + at);
+                o[k].load((const T*)p.prev_out + at);
+            }
         }
     }
+};
+// One pixel by its team; returns whether any channel's change is above the threshold (the same answer in the whole team).
+template <typename T, typename WT, int W, int P, bool BLOCK>
+__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, DeltaPixel<T, W, P>& v, Frag<WT, W> (&w)[P],
+                                               Frag<WT, W> (&b)[P], float* red0, float* red1) {
+    const int64_t off = px * p.c + t.rank * W;
+    Frag<T, W> (&d)[P] = v.d;
+    Frag<T, W> (&u)[P] = v.u;
+    Frag<T, W> (&o)[P] = v.o;
+    bool valid[P];
+#pragma unroll
+    for (int k = 0; k < P; ++k) valid[k] = t.rank + k * t.size < p.nvec;
     using V = typename Vals<W>::V;
     constexpr int N = Vals<W>::N;
     Vals<W> x[P];
@@ -728,7 +737,7 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
 // Teams of lanes: a warp reads the mask of `chunk` pixels at once, lists the active ones and hands them to its teams, so that
 // sparse maps cost one coalesced mask read and no idle teams. The next chunk's mask is on its way meanwhile.
 template <typename T, typename WT, int W, int P>
-__global__ void __launch_bounds__(256, P == 1 ? 5 : 1) k_ln_delta(LnDeltaParams p) {
+__global__ void __launch_bounds__(256, P == 1 ? 4 : 1) k_ln_delta(LnDeltaParams p) {
     __shared__ uint8_t list[8][32], kept[8][32];
     grid_dep_launch();
     grid_dep_wait();
@@ -749,12 +758,21 @@ __global__ void __launch_bounds__(256, P == 1 ? 5 : 1) k_ln_delta(LnDeltaParams 
         kept[warp][lane] = 0;
         __syncwarp();
         const int n = __popc(m);
+        // the next pixel's reads are on their way while one is normalised, where a lane has the registers for both
+        constexpr bool kAhead = P == 1;
+        DeltaPixel<T, W, P> v, ahead;
+        int at = lane / p.g, px = at < n ? list[warp][at] : 0;
+        if (n > 0) v.load(p, t, base + px, at < n);
         for (int k = 0; k < n; k += teams) {
-            const int at = k + lane / p.g;
             const bool on = at < n;
-            const int px = on ? list[warp][at] : 0;
-            const bool keep = ln_delta_pixel<T, WT, W, P, false>(p, t, base + px, on, w, b, nullptr, nullptr);
+            const int next_at = at + teams, next_px = next_at < n ? list[warp][next_at] : 0;
+            if (kAhead && k + teams < n) ahead.load(p, t, base + next_px, next_at < n);
+            const bool keep = ln_delta_pixel<T, WT, W, P, false>(p, t, base + px, on, v, w, b, nullptr, nullptr);
             if (on && t.rank == 0 && keep) kept[warp][px] = 1;
+            at = next_at;
+            px = next_px;
+            if constexpr (kAhead) v = ahead;
+            else if (k + teams < n) v.load(p, t, base + px, at < n);
         }
         __syncwarp();
         if (mine && base + lane < p.npix) p.mask_out[base + lane] = kept[warp][lane];
@@ -773,7 +791,12 @@ __global__ void __launch_bounds__(kLnCta) k_ln_delta_cta(LnDeltaParams p) {
     load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
     for (int64_t px = t.row; px < p.npix; px += t.stride) {
         const bool act = p.mask[px] != 0;      // the same word in every thread
-        const bool keep = act && ln_delta_pixel<T, WT, W, P, true>(p, t, px, true, w, b, red[0], red[1]);
+        bool keep = false;
+        if (act) {
+            DeltaPixel<T, W, P> v;
+            v.load(p, t, px, true);
+            keep = ln_delta_pixel<T, WT, W, P, true>(p, t, px, true, v, w, b, red[0], red[1]);
+        }
         __syncthreads();                       // mask_out may be mask: everybody has read it
         if (t.rank == 0) p.mask_out[px] = keep ? 1 : 0;
     }
@@ -902,7 +925,7 @@ static int ln_delta_run(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
     const int64_t resident = (int64_t)sm_count() * resident_ctas<KERNEL>(s.threads, 0);
     // teams of lanes: pixels that a warp takes at once, as many as leave every resident warp some
     p.chunk = 32;
-    while (p.chunk > 8 && divup64(p.npix, p.chunk) < resident * 8) p.chunk >>= 1;
+    while (p.chunk > 4 && divup64(p.npix, p.chunk) < resident * 8) p.chunk >>= 1;
     const int64_t want = s.g > 0 ? divup64(p.npix, p.chunk * 8) : p.npix;
     return launch_pdl(KERNEL, dim3((unsigned)(want < resident ? want : resident)), dim3(s.threads), 0, st, p);
 }
