@@ -6,10 +6,12 @@
 // largest magnitude takes two shuffles, the codes of a lane are one 4-byte store, the scales of four blocks one more.
 //
 // Both images (k_mx4_tile): a CTA takes 128 x 128 values at a time, which is exactly one 512-byte scale tile of either image,
-// and has the next tile on its way into shared memory meanwhile. The rows are encoded as above, the columns two neighbouring
-// ones of a 32-row block per thread. Rows 32 apart would meet in the same banks, so every 32 rows are skewed by 16 values:
-// a warp reads 8 column pairs x 4 blocks without a conflict and writes 64 contiguous bytes per column. The column sums (the
-// bias gradient of a linear layer, whose dy this kernel reads anyway) fall out of the columns' pass.
+// and has the next tile on its way into shared memory meanwhile. A lane encodes a whole block of a row (no shuffles, the scale's
+// arithmetic once per 32 values), then two neighbouring columns of a 32-row block; a warp writes 64 contiguous bytes per
+// column. The column sums (the bias gradient of a linear layer, whose dy this kernel reads anyway) fall out of the columns' pass.
+//
+// Measured (bf16): rows only, 8192 x 4096, 18 us (85 MB: 13 us at the copy rate); both images of 8192 x 5120 30 us (128 MB: 20 us;
+// 50 us with four lanes a block and no tile ahead), issue slots 64 % busy; dequantising 8192 x 5120 18 us (106 MB: 16 us).
 #include "dc_mx4.cuh"
 
 namespace dc {

@@ -6,11 +6,17 @@
 // dx = r (g - mean(g) - n mean(g n)), dw = sum_rows dy n, db = sum_rows dy.
 //
 // Split: a row belongs to a team of threads that keeps it in registers between its one read and its one write: an aligned
-// group of lanes while the row has at most 128 packs of 16 bytes (several short rows share a warp, sums are shuffles), a
-// whole CTA above that. Teams walk rows with the grid's stride; weight and bias are read once per team and stay in
-// registers, and the next row is requested before the sums of the current one are taken, so the memory system always has a
-// row per team in flight. Rows whose width or address does not allow 16-byte accesses take the same code with single
-// elements; rows beyond the registers of a CTA are read three times by a plain loop.
+// group of lanes while the row has at most 128 packs of 16 bytes (backward: 64; several short rows share a warp, sums are
+// shuffles), a whole CTA above that. Teams walk rows with the grid's stride and have the next rows on their way (cp.async into
+// their own slots of shared memory); weight, and the column sums of the backward pass, stay in registers, whose per-CTA rests a
+// second kernel adds in a fixed order. Rows whose width or address does not allow 16-byte accesses take the same code with
+// single elements; rows beyond the registers of a CTA are read two or three times by a plain loop.
+//
+// Bound: memory, once the arithmetic is packed (two float32 per instruction): 16384 x 4096 bf16 forward 45 us (268 MB, 41 us at
+// the copy rate), backward 72 us (403 MB, 61 us); with scalar arithmetic and a branch per pack the issue slots were the bound
+// (58 and 99 us). 12544 x 576 fp16 forward 9 us (29 MB, 4.4 us: launch and two round trips). Delta form, fp16: 64 channels
+// 136 x 240 x 32, a tenth active, 25 us (83 MB, 12.7 us: sparse pixels leave teams idle); 96 channels 56 x 56 x 64, all active, 49 us
+// (231 MB, 35 us).
 #include <type_traits>
 #include "dc_common.cuh"
 

@@ -936,6 +936,7 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
         bias = None if self.bias is None else self.bias.detach()
         if self.first_iter:
             K._check_feature(val, "input")
+            K._dtype(val)
             self.first_iter = False
             if self not in DCThreshold.t:
                 DCThreshold.set(self, self.delta_threshold)

@@ -359,7 +359,7 @@ def product_bound(a, b, k):
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 1, 1), (1, 128, 32), (3, 8, 33), (16, 128, 64), (17, 130, 96), (32, 1000, 255), (33, 127, 256), (64, 1000, 1280), (65, 257, 257),
                                    (127, 129, 512), (128, 128, 1024), (129, 384, 300), (200, 100, 4096), (256, 256, 768), (300, 1001, 2000), (1, 4096, 4096), (2, 1000, 5000),
-                                   (700, 5000, 544), (1030, 4100, 288), (2500, 1900, 160), (2050, 4802, 1000), (2177, 4801, 96), (1500, 5120, 2080), (129, 12000, 320)])
+                                   (700, 5000, 544), (1030, 4100, 288), (2500, 1900, 160), (2050, 4802, 1000), (2177, 4801, 96), (1500, 5120, 2080), (129, 12000, 320), (100, 30000, 320), (16, 40000, 64)])
 def test_matmul(m, n, k, dtype):
     g = gen(m + n + k)
     (qa, a), (qb, b) = packed((m, k), g), packed((n, k), g)
@@ -446,7 +446,7 @@ def test_linear_gradients(m, n, k, dtype):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("m,n,k", [(1, 100, 40), (1, 14000, 1024), (2, 1000, 1281), (5, 130, 2052), (16, 1000, 4096), (17, 300, 31), (31, 5000, 500), (33, 1000, 1280), (64, 1000, 700),
-                                   (64, 9000, 2048), (65, 100, 260)])
+                                   (64, 9000, 2048), (65, 100, 260), (1, 30000, 256), (3, 40000, 200), (20, 25000, 96)])
 def test_linear_with_packed_weight_is_quantize_and_matmul(m, n, k, dtype):
     """Few tokens are packed inside the product: the same bits as the two calls, hard values and odd widths included."""
     g = gen(m + n)
