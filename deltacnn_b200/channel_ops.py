@@ -86,16 +86,21 @@ def _ptr(t):
 
 def _ln_params(x, c, code, weight, bias, op):
     """The weight's dtype code; weight and bias are (C,) of x's type or float32, of one type."""
-    wcode = None
-    for t, name in ((weight, "weight"), (bias, "bias")):
-        if t is None:
-            continue
-        if t.dim() != 1 or t.shape[0] != c or not t.is_contiguous() or t.device != x.device or (t.dtype != x.dtype and t.dtype != torch.float32):
-            _fail(op, f"{name} must be a contiguous ({c},) tensor of type {x.dtype} or float32 on {x.device}")
-        if wcode is not None and wcode != _CODES[t.dtype]:
+    wcode, index = code, x.get_device()
+    if weight is not None:
+        wcode = _ln_param(x, c, weight, index, "weight", op)
+    if bias is not None:
+        bcode = _ln_param(x, c, bias, index, "bias", op)
+        if weight is not None and bcode != wcode:
             _fail(op, "weight and bias must have the same type")
-        wcode = _CODES[t.dtype]
-    return code if wcode is None else wcode
+        wcode = bcode
+    return wcode
+
+
+def _ln_param(x, c, t, index, name, op):
+    if t.shape != (c,) or t.get_device() != index or not t.is_contiguous() or (t.dtype is not x.dtype and t.dtype is not torch.float32):
+        _fail(op, f"{name} must be a contiguous ({c},) tensor of type {x.dtype} or float32 on {x.device}")
+    return _CODES[t.dtype]
 
 
 def _ln_forward(x, rows, c, weight, bias, eps, keep):
@@ -298,7 +303,7 @@ def mx4_dequantize(q, dtype=torch.float32):
 
 
 def _check_bias(op, bias, n, device):
-    if bias is not None and (bias.dim() != 1 or bias.shape[0] != n or not bias.is_contiguous() or bias.device != device or bias.dtype not in _CODES):
+    if bias is not None and (bias.shape != (n,) or not bias.is_contiguous() or bias.device != device or bias.dtype not in _CODES):
         _fail(op, f"bias must be a contiguous ({n},) tensor on {device}")
 
 
