@@ -89,6 +89,10 @@ _SIGNATURES = {
     "dc_mx4_dequantize": (c_int, [_P, _P, _P, c_i64, c_i64, c_int, _P]),
     "dc_mx4_linear_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64]),
     "dc_mx4_linear": (c_int, [_P, _P, _P, _P, _P, c_i64, c_i64, c_i64, c_int, c_int, _P, c_size_t, _P]),
+    "dc_mx4_linear_train_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64]),
+    "dc_mx4_linear_train": (c_int, [_P, _P, _P, _P, _P, _P, c_i64, c_i64, c_i64, c_int, c_int, c_int, _P, c_size_t, _P]),
+    "dc_mx4_linear_backward_workspace_bytes": (c_size_t, [c_i64, c_i64, c_i64]),
+    "dc_mx4_linear_backward": (c_int, [_P, _P, _P, _P, _P, _P, c_i64, c_i64, c_i64, c_int, c_int, c_int, _P, c_size_t, _P]),
     "dc_mx4_matmul": (c_int, [_P, _P, _P, _P, _P, _P, c_i64, c_i64, c_i64, c_int, c_int, _P]),
 }
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)

@@ -211,6 +211,11 @@ def _mx4_shapes(rows, cols):
     return (rows, 16 * nb), ((rows + 127) // 128, (nb + 3) // 4, 32, 4, 4)
 
 
+def _packed_bytes(rows, cols):
+    nb = (cols + 31) // 32
+    return rows * nb * 16 + (rows + 127) // 128 * ((nb + 3) // 4) * 512
+
+
 class MX4Tensor:
     """A packed rows x cols matrix. ``data``: uint8 (rows, 16 * nb), nb = ceil(cols / 32), two e2m1 codes a byte, the even
     column in the low half, zeros behind the last column. ``scales``: uint8 (ceil(rows / 128), ceil(nb / 4), 32, 4, 4), block b of
@@ -231,9 +236,8 @@ class MX4Tensor:
     def _empty(cls, rows, cols, like):
         """A new matrix in one allocation: the scales stand behind the codes, ``_at`` bytes into it."""
         q = cls.__new__(cls)
-        nb = (cols + 31) // 32
-        q._at = rows * nb * 16
-        q._data, q._scales, q.shape = like.new_empty(q._at + (rows + 127) // 128 * ((nb + 3) // 4) * 512, dtype=torch.uint8), None, (rows, cols)
+        q._at = rows * ((cols + 31) // 32) * 16
+        q._data, q._scales, q.shape = like.new_empty(_packed_bytes(rows, cols), dtype=torch.uint8), None, (rows, cols)
         return q
 
     @property
@@ -252,19 +256,13 @@ class MX4Tensor:
         return mx4_dequantize(self, dtype)
 
 
-def _quantize(x, rows, cols, along_rows, along_cols, colsum=None):
-    """(packed x or None, packed x^T or None); ``colsum``: a (cols,) tensor that receives the column sums. An empty x has no
-    packed transpose (a matrix without columns)."""
+def _quantize(x, rows, cols, both):
+    """(packed x, packed x^T or None)."""
     code = _code(x, "mx4_quantize", "x")
-    q = MX4Tensor._empty(rows, cols, x) if along_rows else None
-    qt = MX4Tensor._empty(cols, rows, x) if along_cols and rows > 0 else None
-    ws, nbytes, sum_code = None, 0, 0
-    if colsum is not None:
-        nbytes, sum_code = lib.dc_mx4_colsum_workspace_bytes(rows, cols), _CODES[colsum.dtype]
-        ws = x.new_empty(nbytes, dtype=torch.uint8)
-    if rows > 0 or colsum is not None:
-        _launch("mx4_quantize", lib.dc_mx4_quantize, x, x.data_ptr(), *(q._ptrs() if q is not None else _NONE), *(qt._ptrs() if qt is not None else _NONE),
-                _ptr(colsum), rows, cols, code, sum_code, _ptr(ws), nbytes)
+    q = MX4Tensor._empty(rows, cols, x)
+    qt = MX4Tensor._empty(cols, rows, x) if both else None
+    if rows > 0:
+        _launch("mx4_quantize", lib.dc_mx4_quantize, x, x.data_ptr(), *q._ptrs(), *(qt._ptrs() if both else _NONE), None, rows, cols, code, 0, None, 0)
     return q, qt
 
 
@@ -276,7 +274,7 @@ def mx4_quantize(x):
     2^(floor(log2 max|v|) - 2); values are rounded to the nearest of +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} times the scale (ties to
     even, saturating); a block with an infinity or a NaN becomes NaN. No gradient, no reference counterpart."""
     rows, cols = _rows(x, "mx4_quantize")
-    return _quantize(x, rows, cols, True, False)[0]
+    return _quantize(x, rows, cols, False)[0]
 
 
 def mx4_quantize_both(x):
@@ -285,7 +283,7 @@ def mx4_quantize_both(x):
     rows, cols = _rows(x, "mx4_quantize_both")
     if rows == 0:
         _fail("mx4_quantize_both", "x has no rows")
-    return _quantize(x, rows, cols, True, True)
+    return _quantize(x, rows, cols, True)
 
 
 def mx4_dequantize(q, dtype=torch.float32):
@@ -345,13 +343,23 @@ class _MX4Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         rows, cols = _rows(x, "mx4_linear")
+        outs = weight.shape[0]
         need_x, need_w, _ = ctx.needs_input_grad
-        xq, xt = _quantize(x, rows, cols, True, need_w)
-        wq, wt = _quantize(weight, weight.shape[0], cols, True, need_x)
-        ctx.xt, ctx.wt = xt, wt
+        ctx.sizes = rows, cols, outs
         ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        ctx.sizes = (rows, cols, weight.shape[0])
-        return _unrows(mx4_matmul(xq, wq, bias, x.dtype), x)
+        out = x.new_empty((rows, outs))
+        ctx.kept, ctx.at = None, (None, None)
+        if rows > 0:
+            # the packed x^T and w^T that the backward pass reads, in one piece
+            x_bytes, w_bytes = _packed_bytes(cols, rows) if need_w else 0, _packed_bytes(cols, outs) if need_x else 0
+            ctx.kept = x.new_empty(x_bytes + w_bytes, dtype=torch.uint8)
+            at = ctx.kept.data_ptr()
+            ctx.at = at if need_w else None, at + x_bytes if need_x else None
+            nbytes = _packed_bytes(rows, cols) + _packed_bytes(outs, cols)
+            ws = x.new_empty(nbytes, dtype=torch.uint8)
+            _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), *ctx.at, rows, outs, cols,
+                    _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype], ws.data_ptr(), nbytes)
+        return _unrows(out, x)
 
     @staticmethod
     def backward(ctx, dy):
@@ -371,16 +379,19 @@ class _MX4Linear(torch.autograd.Function):
         if rows == 0:
             dx = dy.new_zeros(ctx.x_shape, dtype=ctx.dtypes[0]) if need_x else None
             return dx, dy.new_zeros((outs, cols), dtype=ctx.dtypes[1]) if need_w else None, None if db is None else db.zero_()
-        dq, dt = _quantize(dy, rows, outs, need_x, need_w, db)
-        dx = None
+        dx = dy.new_empty((rows, cols), dtype=ctx.dtypes[0]) if need_x else None
+        dw = dy.new_empty((outs, cols), dtype=ctx.dtypes[1]) if need_w else None
+        nbytes = _bytes_wanted("dc_mx4_linear_backward_workspace_bytes", dy.get_device(), rows, outs, cols)
+        ws = dy.new_empty(nbytes, dtype=torch.uint8)
+        _launch("mx4_linear_backward", lib.dc_mx4_linear_backward, dy, dy.data_ptr(), *ctx.at, _ptr(dx), _ptr(dw), _ptr(db), rows, outs, cols, _CODES[dy.dtype],
+                _CODES[ctx.dtypes[1]], 0 if db is None else _CODES[db.dtype], ws.data_ptr(), nbytes)
         if need_x:
-            dx = mx4_matmul(dq, ctx.wt, None, ctx.dtypes[0])
             if len(ctx.x_shape) == 4:
                 n, _, h, w = ctx.x_shape
                 dx = dx.view(n, h, w, cols).permute(0, 3, 1, 2)
-            else:
+            elif len(ctx.x_shape) != 2:
                 dx = dx.view(ctx.x_shape)
-        return dx, mx4_matmul(dt, ctx.xt, None, ctx.dtypes[1]) if need_w else None, db
+        return dx, dw, db
 
 
 def mx4_linear(x, weight, bias=None):
@@ -406,7 +417,7 @@ def mx4_linear(x, weight, bias=None):
             _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
         if grad:
             return _MX4Linear.apply(x, weight, bias)
-        weight = _quantize(weight, outs, cols, True, False)[0]
+        weight = _quantize(weight, outs, cols, False)[0]
     out = x.new_empty((rows, outs))
     if rows > 0 and outs > 0:
         nbytes = _bytes_wanted("dc_mx4_linear_workspace_bytes", x.get_device(), rows, outs, cols)

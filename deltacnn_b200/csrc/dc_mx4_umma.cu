@@ -734,4 +734,50 @@ int dc_mx4_linear(const void* x, const void* w_data, const void* w_scales, const
     return mx4_product(nullptr, ws, ws + data, w_data, w_scales, bias, out, m, n, k, bias_dtype, dtype, (cudaStream_t)stream);
 }
 
+// A packed matrix in one piece of memory, the scales behind the codes (both multiples of 16 bytes).
+static size_t mx4_bytes(int64_t rows, int64_t cols) { return dc_mx4_data_bytes(rows, cols) + dc_mx4_scale_bytes(rows, cols); }
+static uint8_t* mx4_scales_of(void* piece, int64_t rows, int64_t cols) { return piece == nullptr ? nullptr : (uint8_t*)piece + dc_mx4_data_bytes(rows, cols); }
+static bool mx4_dtype_ok(int d) { return d >= DC_F32 && d <= DC_BF16; }
+
+size_t dc_mx4_linear_train_workspace_bytes(int64_t m, int64_t n, int64_t k) { return mx4_bytes(m, k) + mx4_bytes(n, k); }
+
+int dc_mx4_linear_train(const void* x, const void* w, const void* bias, void* out, void* xt, void* wt, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                        int32_t w_dtype, int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!mx4_sizes_ok(m, n, k) || m == 0 || n == 0) return DC_ERR_SHAPE;
+    if (!mx4_dtype_ok(dtype) || !mx4_dtype_ok(w_dtype) || (bias != nullptr && !mx4_dtype_ok(bias_dtype))) return DC_ERR_DTYPE;
+    if (x == nullptr || w == nullptr || out == nullptr || workspace == nullptr) return DC_ERR_NULL_POINTER;
+    if (!aligned16(workspace) || !aligned16(xt) || !aligned16(wt)) return DC_ERR_ALIGNMENT;
+    if (workspace_bytes < dc_mx4_linear_train_workspace_bytes(m, n, k)) return DC_ERR_WORKSPACE;
+    uint8_t *xq = (uint8_t*)workspace, *wq = xq + mx4_bytes(m, k);
+    int rc = dc_mx4_quantize(x, xq, mx4_scales_of(xq, m, k), xt, mx4_scales_of(xt, k, m), nullptr, m, k, dtype, 0, nullptr, 0, stream);
+    if (rc != DC_OK) return rc;
+    rc = dc_mx4_quantize(w, wq, mx4_scales_of(wq, n, k), wt, mx4_scales_of(wt, k, n), nullptr, n, k, w_dtype, 0, nullptr, 0, stream);
+    if (rc != DC_OK) return rc;
+    return mx4_product(nullptr, xq, mx4_scales_of(xq, m, k), wq, mx4_scales_of(wq, n, k), bias, out, m, n, k, bias_dtype, dtype, (cudaStream_t)stream);
+}
+
+size_t dc_mx4_linear_backward_workspace_bytes(int64_t m, int64_t n, int64_t k) {
+    if (!mx4_sizes_ok(m, n, k)) return 0;
+    return mx4_bytes(m, n) + mx4_bytes(n, m) + dc_mx4_colsum_workspace_bytes(m, n);
+}
+
+int dc_mx4_linear_backward(const void* dy, const void* xt, const void* wt, void* dx, void* dw, void* db, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                           int32_t w_dtype, int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!mx4_sizes_ok(m, n, k) || m == 0 || n == 0) return DC_ERR_SHAPE;
+    if (!mx4_dtype_ok(dtype) || (dw != nullptr && !mx4_dtype_ok(w_dtype)) || (db != nullptr && !mx4_dtype_ok(bias_dtype))) return DC_ERR_DTYPE;
+    if (dx == nullptr && dw == nullptr && db == nullptr) return DC_OK;
+    if (dy == nullptr || workspace == nullptr || (dx != nullptr && wt == nullptr) || (dw != nullptr && xt == nullptr)) return DC_ERR_NULL_POINTER;
+    if (!aligned16(workspace) || !aligned16(xt) || !aligned16(wt)) return DC_ERR_ALIGNMENT;
+    if (workspace_bytes < dc_mx4_linear_backward_workspace_bytes(m, n, k)) return DC_ERR_WORKSPACE;
+    uint8_t *dq = (uint8_t*)workspace, *dt = dq + mx4_bytes(m, n), *sums = dt + mx4_bytes(n, m);
+    int rc = dc_mx4_quantize(dy, dx != nullptr ? dq : nullptr, dx != nullptr ? mx4_scales_of(dq, m, n) : nullptr, dw != nullptr ? dt : nullptr,
+                             dw != nullptr ? mx4_scales_of(dt, n, m) : nullptr, db, m, n, dtype, bias_dtype, db != nullptr ? sums : nullptr,
+                             db != nullptr ? dc_mx4_colsum_workspace_bytes(m, n) : 0, stream);
+    if (rc == DC_OK && dx != nullptr)
+        rc = mx4_product(nullptr, dq, mx4_scales_of(dq, m, n), wt, mx4_scales_of(const_cast<void*>(wt), k, n), nullptr, dx, m, k, n, 0, dtype, (cudaStream_t)stream);
+    if (rc == DC_OK && dw != nullptr)
+        rc = mx4_product(nullptr, dt, mx4_scales_of(dt, n, m), xt, mx4_scales_of(const_cast<void*>(xt), k, m), nullptr, dw, n, k, m, 0, w_dtype, (cudaStream_t)stream);
+    return rc;
+}
+
 }  // extern "C"

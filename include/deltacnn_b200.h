@@ -383,6 +383,18 @@ int dc_mx4_matmul(const void* a_data, const void* a_scales, const void* b_data, 
  * dtype; few rows of x are packed inside the product (one launch). workspace: dc_mx4_linear_workspace_bytes of device
  * memory, 16-byte aligned, only meaningful during the call (0 bytes, NULL: none wanted). Same bits as the two calls. */
 size_t dc_mx4_linear_workspace_bytes(int64_t m, int64_t n, int64_t k);
+/* The layer in training. Forward: out = Q(x) Q(w)^T + bias with both operands packed in the call (x m x k and out in dtype, w n x k
+ * in w_dtype, each read once); xt, wt (may be NULL): what the backward pass reads, the packed x^T (k x m) for dw and w^T
+ * (k x n) for dx, each dc_mx4_data_bytes + dc_mx4_scale_bytes, the scales behind the codes. Backward: dx = Q(dy) Q(w^T)^T in
+ * dtype, dw = Q(dy^T) Q(x^T)^T in w_dtype, db = sum of dy's rows in bias_dtype; NULL where not wanted, dy is read once. Every
+ * operand is rounded along the axis its product sums over; the rounding's own gradient is taken as 1. workspace: the bytes that
+ * the queries name, 16-byte aligned, only meaningful during the call. m, n, k > 0. */
+size_t dc_mx4_linear_train_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int dc_mx4_linear_train(const void* x, const void* w, const void* bias, void* out, void* xt, void* wt, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                        int32_t w_dtype, int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t dc_mx4_linear_backward_workspace_bytes(int64_t m, int64_t n, int64_t k);
+int dc_mx4_linear_backward(const void* dy, const void* xt, const void* wt, void* dx, void* dw, void* db, int64_t m, int64_t n, int64_t k, int32_t dtype,
+                           int32_t w_dtype, int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
 int dc_mx4_linear(const void* x, const void* w_data, const void* w_scales, const void* bias, void* out, int64_t m, int64_t n, int64_t k, int32_t dtype,
                   int32_t bias_dtype, void* workspace, size_t workspace_bytes, void* stream);
 

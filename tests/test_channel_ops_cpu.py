@@ -76,6 +76,20 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.dc_mx4_linear(p, p, p, None, p, 500, 500, 32, f32, f32, p, 64, None) == space
     assert lib.dc_mx4_linear(p, p, p, None, p, 500, 500, 32, f32, f32, None, 0, None) == null
     assert lib.dc_mx4_linear_workspace_bytes(1, 500, 64) == 0 and lib.dc_mx4_linear_workspace_bytes(500, 500, 64) == 500 * 32 + 4 * 512
+    train = lib.dc_mx4_linear_train
+    assert train(p, p, None, p, p, p, 4, 8, 0, f32, f32, f32, p, 1 << 20, None) == shape
+    assert train(p, p, None, p, p, p, 0, 8, 32, f32, f32, f32, p, 1 << 20, None) == shape
+    assert train(p, p, None, p, p, p, 4, 8, 32, f32, 3, f32, p, 1 << 20, None) == dtype
+    assert train(p, None, None, p, p, p, 4, 8, 32, f32, f32, f32, p, 1 << 20, None) == null
+    assert train(p, p, None, p, p + 8, p, 4, 8, 32, f32, f32, f32, p, 1 << 20, None) == align
+    assert train(p, p, None, p, p, p, 4, 8, 32, f32, f32, f32, p, 64, None) == space
+    back = lib.dc_mx4_linear_backward
+    assert back(p, None, None, None, None, None, 4, 8, 32, f32, f32, f32, p, 1 << 20, None) == 0
+    assert back(p, None, p, p, p, None, 4, 8, 32, f32, f32, f32, p, 1 << 20, None) == null
+    assert back(p, p, None, p, p, None, 4, 8, 32, f32, f32, f32, p, 1 << 20, None) == null
+    assert back(p, p, p, p, p, p, 4, 8, 32, f32, f32, 3, p, 1 << 20, None) == dtype
+    assert back(p, p, p, p, p, p, 4, 8, 32, f32, f32, f32, p, 64, None) == space
+    assert lib.dc_mx4_linear_train_workspace_bytes(4, 8, 32) == 4 * 16 + 512 + 8 * 16 + 512
     assert lib.dc_mx4_data_bytes(3, 33) == 3 * 32 and lib.dc_mx4_scale_bytes(129, 129) == 2 * 2 * 512
 
 
