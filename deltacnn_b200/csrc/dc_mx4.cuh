@@ -94,13 +94,11 @@ template <typename T> struct Eight {
 template <typename T> __device__ __forceinline__ uint32_t amax_word(uint32_t a, uint32_t b);
 template <> __device__ __forceinline__ uint32_t amax_word<float>(uint32_t a, uint32_t b) { return max(a, b & 0x7fffffffu); }
 template <> __device__ __forceinline__ uint32_t amax_word<__half>(uint32_t a, uint32_t b) {
-    b &= 0x7fff7fffu;
-    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    const __half2 r = __hmax2_nan(*reinterpret_cast<__half2*>(&a), __habs2(*reinterpret_cast<__half2*>(&b)));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 template <> __device__ __forceinline__ uint32_t amax_word<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    b &= 0x7fff7fffu;
-    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    const __nv_bfloat162 r = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), __habs2(*reinterpret_cast<__nv_bfloat162*>(&b)));
     return *reinterpret_cast<const uint32_t*>(&r);
 }
 // A word's two values (or its one) in float32.
