@@ -43,7 +43,7 @@ struct MxPlace {
     }
 };
 
-template <typename T, bool VEC>
+template <typename T, int BYTES>
 __global__ void __launch_bounds__(256) k_mx4_rows(const T* __restrict__ x, uint8_t* __restrict__ data, uint8_t* __restrict__ scales, int cols, MxWalk w) {
     grid_dep_launch();
     grid_dep_wait();
@@ -56,7 +56,7 @@ __global__ void __launch_bounds__(256) k_mx4_rows(const T* __restrict__ x, uint8
         uint8_t* srow = scales + mx4_scale_word(at.row, 0, tiles);
         Eight<T> v[kMxAhead];
 #pragma unroll
-        for (int a = 0; a < kMxAhead; ++a) v[a].template load<VEC>(row, c0 + a * kMxChunk, cols);
+        for (int a = 0; a < kMxAhead; ++a) v[a].template load<BYTES>(row, c0 + a * kMxChunk, cols);
 #pragma unroll
         for (int a = 0; a < kMxAhead; ++a) {
             const int col = c0 + a * kMxChunk, b = col >> 5;
@@ -331,25 +331,27 @@ static int launch_tile(const MxTileParams& p, cudaStream_t st) {
 }
 template <typename T, bool SUMS>
 static int launch_tile_copy(const MxTileParams& p, cudaStream_t st) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(p.x);
-    const int64_t pitch = p.cols * (int64_t)sizeof(T);
-    if ((x & 15u) == 0 && pitch % 16 == 0) return launch_tile<T, 16, SUMS>(p, st);
-    if ((x & 3u) == 0 && pitch % 4 == 0) return launch_tile<T, 4, SUMS>(p, st);
-    if constexpr (sizeof(T) == 2) return launch_tile<T, 0, SUMS>(p, st);
-    return DC_ERR_ALIGNMENT;          // float32 off 4 bytes
+    const int access = row_access<T>(p.x, p.cols);
+    if (access == 16) return launch_tile<T, 16, SUMS>(p, st);
+    if constexpr (sizeof(T) == 2)
+        if (access == 2) return launch_tile<T, 0, SUMS>(p, st);
+    return launch_tile<T, 4, SUMS>(p, st);
 }
 
 template <typename T>
 static int quantize_t(const void* x, void* data, void* scales, void* data_t, void* scales_t, float* colsum, int64_t rows, int64_t cols, cudaStream_t st) {
     if (data_t == nullptr && colsum == nullptr) {
-        const bool vec = aligned16(x) && cols % VecTraits<T>::kVec == 0;
         const int segments = (int)divup64(mx4_scale_tiles(cols) * 128, kMxChunk * kMxAhead);
         int64_t ctas = divup64(rows * segments, 8);
         const int64_t cap = (int64_t)sm_count() * 5;
         if (ctas > cap) ctas = cap;
         const MxWalk w = mx_walk(rows, segments, ctas * 8);
-        if (vec) return launch_pdl(k_mx4_rows<T, true>, dim3((unsigned)ctas), dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, (int)cols, w);
-        return launch_pdl(k_mx4_rows<T, false>, dim3((unsigned)ctas), dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, (int)cols, w);
+        const dim3 grid((unsigned)ctas);
+        const int access = row_access<T>(x, cols);
+        if (access == 16) return launch_pdl(k_mx4_rows<T, 16>, grid, dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, (int)cols, w);
+        if constexpr (sizeof(T) == 2)
+            if (access == 2) return launch_pdl(k_mx4_rows<T, 2>, grid, dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, (int)cols, w);
+        return launch_pdl(k_mx4_rows<T, 4>, grid, dim3(256), 0, st, (const T*)x, (uint8_t*)data, (uint8_t*)scales, (int)cols, w);
     }
     const int64_t tx = divup64(cols, kTile), ty = divup64(rows, kTile);
     if (tx * ty > 0x3fffffffLL || rows > 0x7ffff000LL) return DC_ERR_SHAPE;

@@ -70,8 +70,12 @@ template <typename T> struct Eight {
     static constexpr int kWords = 8 * (int)sizeof(T) / 4;
     alignas(16) uint32_t w[kWords];
 
-    template <bool VEC> __device__ __forceinline__ void load(const T* row, int64_t col, int64_t cols) {
-        if constexpr (VEC) {
+    // BYTES: what an access may take, 16, 4 or an element's own (rows start and end on multiples of it).
+    template <int BYTES> __device__ __forceinline__ void load(const T* row, int64_t col, int64_t cols) {
+        if constexpr (BYTES == 4 && sizeof(T) == 2) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[k] = col + 2 * k < cols ? *reinterpret_cast<const uint32_t*>(row + col + 2 * k) : 0u;
+        } else if constexpr (BYTES == 16) {
             constexpr int N = VecTraits<T>::kVec;
 #pragma unroll
             for (int k = 0; k < 8 / N; ++k)
@@ -152,6 +156,12 @@ __device__ __forceinline__ uint32_t mx4_scale_quad(uint32_t scale, int lane) {
     uint32_t word = scale << (8 * ((lane >> 2) & 3));
     word |= __shfl_xor_sync(DC_FULL, word, 4);
     return word | __shfl_xor_sync(DC_FULL, word, 8);
+}
+
+// The widest access that rows of `cols` elements at x allow.
+template <typename T> inline int row_access(const void* x, int64_t cols) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(x) | (uintptr_t)(cols * (int64_t)sizeof(T));
+    return (a & 15u) == 0 ? 16 : (a & 3u) == 0 ? 4 : (int)sizeof(T);
 }
 
 }  // namespace dc

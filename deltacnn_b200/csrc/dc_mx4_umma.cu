@@ -52,7 +52,7 @@ template <int NT> struct MxCfg {
 struct MxGemmParams {
     const uint8_t *a_sc, *b_sc;            // scales of the tokens, of the features
     const void* x;                         // tokens in the result's type, where they are quantised on the way
-    int k, x_vec, groups;                  // their width; rows allow 16-byte reads; groups of eight rows
+    int k, access, groups;                 // their width; bytes a read of theirs may take; groups of eight rows
     const void* bias;
     void* out;
     int64_t m;
@@ -236,8 +236,9 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
                             const int r = g * 8 + j;
                             const OT* row = (const OT*)p.x + (row0 + r) * p.k;
                             const int64_t end = r < rows ? p.k : 0;
-                            if (p.x_vec) v[j].template load<true>(row, col, end);
-                            else v[j].template load<false>(row, col, end);
+                            if (p.access == 16) v[j].template load<16>(row, col, end);
+                            else if (p.access == 4) v[j].template load<4>(row, col, end);
+                            else v[j].template load<(int)sizeof(OT)>(row, col, end);
                         }
                         if (!mbar_wait_warp(empty(s), ((uint32_t)(seq / S) & 1u) ^ 1u, ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 9); ok = false; break; }
 #pragma unroll
@@ -291,18 +292,26 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
         const int64_t t0 = (int64_t)tt * NT;
         const int cols = (int)(p.m - t0 < NT ? p.m - t0 : NT);
         const bool good = *ok_flag != 0;
-        for (int i = threadIdx.x; i < 128 * ((cols - rank + ranks - 1) / ranks); i += blockDim.x) {
-            const int col = rank + (i >> 7) * ranks, f = tf * 128 + (i & 127);
-            if (f >= p.n || !good) continue;
-            float v = 0.f;
-            for (int q = 0; q < ranks; ++q) {
-                uint32_t remote;
-                float x;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(ring + (uint32_t)(col * 128 + (i & 127)) * 4u), "r"(q));
-                asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(remote) : "memory");
-                v += x;
-            }
-            ((OT*)p.out)[(t0 + col) * p.n + f] = from_f<OT>(v + mx_bias(p, f));
+        // four features at a time, every rank's share of them in flight together
+        const int mine = 32 * ((cols - rank + ranks - 1) / ranks);
+        for (int i = threadIdx.x; i < mine && good; i += blockDim.x) {
+            const int col = rank + (i >> 5) * ranks, f = tf * 128 + (i & 31) * 4;
+            float4 x[8];
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < ranks) {
+                    uint32_t remote;
+                    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(ring + (uint32_t)(col * 128 + (i & 31) * 4) * 4u), "r"(q));
+                    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[q].x), "=f"(x[q].y), "=f"(x[q].z), "=f"(x[q].w) : "r"(remote) : "memory");
+                }
+            float v[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (q < ranks) { v[0] += x[q].x; v[1] += x[q].y; v[2] += x[q].z; v[3] += x[q].w; }
+            OT* o = (OT*)p.out + (t0 + col) * p.n + f;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (f + j < p.n) o[j] = from_f<OT>(v[j] + mx_bias(p, f + j));
         }
         asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
@@ -617,31 +626,37 @@ static int launch_mx4_nt(int nt, const MxGemmParams& p, int split, const CUtenso
         case 16: return launch_mx4<OT, 16, SPLIT, false>(p, split, ma, mb, st);
         case 32: return launch_mx4<OT, 32, SPLIT, false>(p, split, ma, mb, st);
         case 64: return launch_mx4<OT, 64, SPLIT, false>(p, split, ma, mb, st);
-        default: return launch_mx4<OT, 128, SPLIT, false>(p, split, ma, mb, st);
+        default: break;
     }
+    if constexpr (SPLIT) return launch_mx4<OT, 128, SPLIT, false>(p, split, ma, mb, st);
+    else return DC_ERR_UNSUPPORTED;          // 128 tokens a tile: clusters only
 }
 template <typename OT>
 static int launch_mx4_split(const MxPlan& pl, const MxGemmParams& p, const CUtensorMap& ma, const CUtensorMap& mb, cudaStream_t st) {
     return pl.split > 1 ? launch_mx4_nt<OT, true>(pl.nt, p, pl.split, ma, mb, st) : launch_mx4_nt<OT, false>(pl.nt, p, 1, ma, mb, st);
 }
 
-// How a product is cut: pairs of SMs, or tiles of nt tokens shared along k by `split` CTAs; quant: dc_mx4_linear quantises the
-// tokens inside the product.
+// How a product is cut: pairs of SMs, or tiles of nt tokens, each by one CTA or shared along k by `split`; quant: dc_mx4_linear
+// quantises the tokens inside the product.
 static MxPlan mx4_plan(int64_t m, int64_t n, int64_t k) {
     const int sms = sm_count();
     const int steps = (int)divup64(k, kMxStep);
-    const int64_t tiles_k = mx4_scale_tiles(k);
     MxPlan pl{};
     pl.split = 1;
-    // many tokens: pairs of SMs, where their tiles fill at least half of the GPU
-    const int64_t pair_tiles = divup64(n, 256) * divup64(m, kM2Tok);
-    pl.pair = m > 128 && pair_tiles * 4 >= sms && pair_tiles <= 0x7fffffffLL && (divup64(m > n ? m : n, 128) + 2) * tiles_k <= 0x7fffffffLL;
-    if (pl.pair) { pl.tiles = pair_tiles; return pl; }
     // columns of a tile: no more than the tokens need
     pl.nt = m <= 16 ? 16 : m <= 32 ? 32 : m <= 64 ? 64 : 128;
     pl.tiles = divup64(n, 128) * divup64(m, pl.nt);
-    // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each
-    while (pl.split < 8 && pl.tiles * pl.split * 2 <= sms && steps >= pl.split * 2) pl.split *= 2;
+    // tiles that leave most SMs idle are shared along k by a cluster of up to 8 CTAs, at least one step each (clusters of 8 take
+    // the SMs of a GPC by halves: more than a dozen do not run at once, 200 x 2048 -> 1000 took 11.4 us with 16)
+    while (pl.split < 8 && pl.tiles * pl.split * 2 <= sms && steps >= pl.split * 2 && (pl.split < 4 || pl.tiles <= 12)) pl.split *= 2;
+    // More than 64 tokens: pairs of SMs (5.3 us and 0.39 us a step for one tile each), unless a cluster saves seven steps and more.
+    // Pairs / clusters: 128 x 256 -> 256 5.6 / 8.4 us, 1024 x 1024 -> 1024 7.0 / 8.4, 128 x 4096 -> 14336 (no room for clusters) 12.2 /
+    // 14.2, 200 x 4096 -> 4096 11.6 / 10.8, 128 x 4096 -> 4096 11.6 / 8.4, 4096 x 8192 -> 256 17.5 / 13.7.
+    pl.pair = m > 64 && steps - steps / pl.split < 7;
+    if (pl.pair) {
+        pl.tiles = divup64(n, 256) * divup64(m, kM2Tok);
+        return pl;
+    }
     // Quantising inside makes every feature tile's CTA read the tokens unpacked: eight rows of a step and warp at a time, which
     // waits for their 1 us of latency in every round of the eight warps. Device time inside / with a launch of its own (2.2 us of
     // it), bf16: one round, 1 x 4096 -> 14336, 10.0 / 11.8 us; two, 8 x 4096 -> 14336, 11.4 / 11.7, and 64 x 1280 -> 1000, 12.3 /
@@ -655,7 +670,7 @@ static MxPlan mx4_plan(int64_t m, int64_t n, int64_t k) {
 static int mx4_product(const void* x, const void* a_data, const void* a_scales, const void* b_data, const void* b_scales, const void* bias, void* out, int64_t m,
                        int64_t n, int64_t k, int bias_dtype, int out_dtype, cudaStream_t st) {
     const MxPlan pl = mx4_plan(m, n, k);
-    if (pl.tiles > 0x7fffffffLL) return DC_ERR_SHAPE;
+    if (pl.tiles > 0x7fffff00LL || (divup64(m > n ? m : n, 128) + 2) * mx4_scale_tiles(k) > 0x7fffff00LL) return DC_ERR_SHAPE;
     MxGemmParams p{};
     p.a_sc = (const uint8_t*)a_scales; p.b_sc = (const uint8_t*)b_scales; p.bias = bias; p.out = out;
     p.m = m; p.n = (int)n; p.nb = (int)mx4_blocks(k); p.tiles_k = (int)mx4_scale_tiles(k); p.steps = (int)divup64(k, kMxStep);
@@ -664,7 +679,7 @@ static int mx4_product(const void* x, const void* a_data, const void* a_scales, 
     p.tiles_f = (int)divup64(n, pl.pair ? 256 : 128);
     p.tiles = (int)pl.tiles;
     p.x = x; p.k = (int)k; p.groups = (int)divup64(m < 64 ? m : 64, 8);
-    p.x_vec = aligned16(x) && k % (out_dtype == DC_F32 ? 4 : 8) == 0;
+    p.access = out_dtype == DC_F32 ? row_access<float>(x, k) : row_access<__half>(x, k);
     alignas(64) CUtensorMap ma, mb;
     if (!encode_mx4_map(&mb, b_data, n, (int64_t)p.nb * 16, 128)) return DC_ERR_UNSUPPORTED;
     if (x != nullptr) ma = mb;          // not read

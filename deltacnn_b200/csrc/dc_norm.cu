@@ -576,13 +576,13 @@ __global__ void __launch_bounds__(1024) k_ln_bwd_long(LnBwdParams p) {
             for (int j = 0; j < W; ++j) { out[(int64_t)i * W + j] = cols[(int64_t)i * W + j]; out[p.c + (int64_t)i * W + j] = cols[p.c + (int64_t)i * W + j]; }
 }
 
-// Column sums of the CTAs' partial rows, in a fixed order: 32 columns per CTA, 32 threads share a column's rows and have four
-// of them in flight each (16 threads and one row at a time: 17 us for 296 x 4096, all of it latency).
-constexpr int kRedRows = 32;
-template <typename OT>
-__global__ void __launch_bounds__(32 * kRedRows) k_col_reduce(const float* __restrict__ partial, int n, int c, int64_t pitch, OT* __restrict__ o0,
-                                                              OT* __restrict__ o1) {
-    __shared__ float s[kRedRows][33];
+// Column sums of the CTAs' partial rows, in a fixed order: 32 columns per CTA, R threads share a column's rows and have four of
+// them in flight each. R = 32; 4 for few rows, where the threads of a wide CTA would find nothing (4 rows of 14801 columns: 14
+// against 4 us; with 16 threads and one row at a time 296 rows of 4096 took 17 us, all of it latency).
+template <typename OT, int R>
+__global__ void __launch_bounds__(32 * R) k_col_reduce(const float* __restrict__ partial, int n, int c, int64_t pitch, OT* __restrict__ o0,
+                                                       OT* __restrict__ o1) {
+    __shared__ float s[R][33];
     grid_dep_launch();
     grid_dep_wait();
     const int col = blockIdx.x * 32 + threadIdx.x;
@@ -591,26 +591,33 @@ __global__ void __launch_bounds__(32 * kRedRows) k_col_reduce(const float* __res
     float a[4] = {0.f, 0.f, 0.f, 0.f};
     if (col < c) {
         const float* src = partial + (int64_t)blockIdx.y * c + col;
-        for (int i = threadIdx.y; i < n; i += 4 * kRedRows) {
+        for (int i = threadIdx.y; i < n; i += 4 * R) {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                if (i + j * kRedRows < n) a[j] += src[(i + j * kRedRows) * pitch];
+                if (i + j * R < n) a[j] += src[(i + j * R) * pitch];
         }
     }
     s[threadIdx.y][threadIdx.x] = (a[0] + a[1]) + (a[2] + a[3]);
     __syncthreads();
-    // a warp takes a column: its 32 sums by shuffles
-    const float v = group_sum(s[threadIdx.x][threadIdx.y], 32);
-    const int mine = blockIdx.x * 32 + threadIdx.y;
-    if (threadIdx.x == 0 && mine < c) o[mine] = from_f<OT>(v);
+    if (threadIdx.y == 0 && col < c) {
+        float v[4] = {s[0][threadIdx.x], s[1][threadIdx.x], s[2][threadIdx.x], s[3][threadIdx.x]};
+#pragma unroll
+        for (int i = 4; i < R; ++i) v[i & 3] += s[i][threadIdx.x];
+        o[col] = from_f<OT>((v[0] + v[1]) + (v[2] + v[3]));
+    }
 }
 
+template <typename OT>
+static int col_reduce_t(const float* partial, int n, int c, int64_t pitch, void* o0, void* o1, cudaStream_t st) {
+    const dim3 grid((unsigned)divup(c, 32), o1 != nullptr ? 2u : 1u);
+    if (n <= 64) return launch_pdl(k_col_reduce<OT, 4>, grid, dim3(32, 4), 0, st, partial, n, c, pitch, (OT*)o0, (OT*)o1);
+    return launch_pdl(k_col_reduce<OT, 32>, grid, dim3(32, 32), 0, st, partial, n, c, pitch, (OT*)o0, (OT*)o1);
+}
 int col_reduce(const float* partial, int n, int c, int64_t pitch, void* o0, void* o1, int dtype, cudaStream_t st) {
-    const dim3 grid((unsigned)divup(c, 32), o1 != nullptr ? 2u : 1u), block(32, kRedRows);
     switch (dtype) {
-        case DC_F32: return launch_pdl(k_col_reduce<float>, grid, block, 0, st, partial, n, c, pitch, (float*)o0, (float*)o1);
-        case DC_F16: return launch_pdl(k_col_reduce<__half>, grid, block, 0, st, partial, n, c, pitch, (__half*)o0, (__half*)o1);
-        case DC_BF16: return launch_pdl(k_col_reduce<__nv_bfloat16>, grid, block, 0, st, partial, n, c, pitch, (__nv_bfloat16*)o0, (__nv_bfloat16*)o1);
+        case DC_F32: return col_reduce_t<float>(partial, n, c, pitch, o0, o1, st);
+        case DC_F16: return col_reduce_t<__half>(partial, n, c, pitch, o0, o1, st);
+        case DC_BF16: return col_reduce_t<__nv_bfloat16>(partial, n, c, pitch, o0, o1, st);
         default: return DC_ERR_DTYPE;
     }
 }
