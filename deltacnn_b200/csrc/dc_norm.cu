@@ -10,39 +10,39 @@
 // shuffles), a whole CTA above that. Teams walk rows with the grid's stride and have the next rows on their way (cp.async into
 // their own slots of shared memory); weight, and the column sums of the backward pass, stay in registers, whose per-CTA rests a
 // second kernel adds in a fixed order. Rows whose width or address does not allow 16-byte accesses take the same code with
-// single elements; rows beyond the registers of a CTA are read two or three times by a plain loop.
+// two halves or single elements (delta form, 82 channels 73 x 18 x 42: 44 us with single halves, 18 with two); rows beyond the
+// registers of a CTA are read two or three times by a plain loop.
 //
 // Bound: memory, once the arithmetic is packed (two float32 per instruction): 16384 x 4096 bf16 forward 45 us (268 MB, 41 us at
 // the copy rate), backward 72 us (403 MB, 61 us); with scalar arithmetic and a branch per pack the issue slots were the bound
 // (58 and 99 us). 12544 x 576 fp16 forward 9 us (29 MB, 4.4 us: launch and two round trips). Delta form, fp16: 64 channels
 // 136 x 240 x 32, a tenth active, 25 us (83 MB, 12.7 us: sparse pixels leave teams idle); 96 channels 56 x 56 x 64, all active, 49 us
 // (231 MB, 35 us).
+#include <initializer_list>
 #include <type_traits>
 #include "dc_common.cuh"
 
 namespace dc {
 
-// W consecutive elements in storage precision; 16-byte accesses where the size allows.
+// W consecutive elements in storage precision: 16-byte accesses, one of 8 or 4 bytes, or an element.
 template <typename T, int W> struct Frag {
     static constexpr int kBytes = W * (int)sizeof(T);
-    alignas(kBytes % 16 == 0 ? 16 : alignof(T)) T s[W];
+    alignas(kBytes % 16 == 0 ? 16 : kBytes) T s[W];
     __device__ __forceinline__ void load(const T* p) {
         if constexpr (kBytes % 16 == 0) {
 #pragma unroll
             for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(s)[i] = reinterpret_cast<const uint4*>(p)[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) s[i] = p[i];
-        }
+        } else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(s) = *reinterpret_cast<const uint2*>(p);
+        else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(s) = *reinterpret_cast<const uint32_t*>(p);
+        else s[0] = p[0];
     }
     __device__ __forceinline__ void store(T* p) const {
         if constexpr (kBytes % 16 == 0) {
 #pragma unroll
             for (int i = 0; i < kBytes / 16; ++i) reinterpret_cast<uint4*>(p)[i] = reinterpret_cast<const uint4*>(s)[i];
-        } else {
-#pragma unroll
-            for (int i = 0; i < W; ++i) p[i] = s[i];
-        }
+        } else if constexpr (kBytes == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(s);
+        else if constexpr (kBytes == 4) *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(s);
+        else p[0] = s[0];
     }
     __device__ __forceinline__ float get(int i) const { return to_f<T>(s[i]); }
     __device__ __forceinline__ void set(int i, float x) { s[i] = from_f<T>(x); }
@@ -116,7 +116,7 @@ template <> struct Vals<1> {
 
 constexpr int kLnCta = 512;         // most threads of a CTA that holds a row: 128 registers a thread
 // Threads of a CTA at most for a row split into so many packs per thread.
-__host__ __device__ constexpr int row_threads(int w, int p) { return (w == 1 ? p > 8 : p > 1) ? kLnCta : 256; }
+__host__ __device__ constexpr int row_threads(int w, int p) { return (w <= 2 ? p > 4 : p > 1) ? kLnCta : 256; }
 constexpr int kMaxWarps = 32;
 
 // Sum over an aligned group of g lanes, g the same in the whole grid: five predicated steps instead of a loop.
@@ -164,7 +164,7 @@ __device__ __forceinline__ void cp16(void* dst, const void* src) {
 }
 // Packs behind the end of a row (rank + k size >= nvec) read as zeros, so that the arithmetic needs no branch for them.
 template <typename T, int W, int P, int N> struct RowPipe {
-    static constexpr bool kRing = W > 1;
+    static constexpr bool kRing = W * sizeof(T) == 16;
     static constexpr int kAhead = rows_ahead(N * P);
     Frag<T, W> next[kRing ? 1 : N][kRing ? 1 : P];
     uint8_t* mine;
@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
     T* y = (T*)p.y + t.row * p.c + t.rank * W;
     // weight and bias stay in registers; lanes with three packs and more read them from L1 for every row instead and have the
     // registers for twice the warps (12544 x 576: 12.3 -> 8.9 us)
-    constexpr bool kHeld = BLOCK || P < 3 || W == 1;
+    constexpr bool kHeld = BLOCK || P < 3 || W <= 2;
     Frag<WT, W> w[kHeld ? P : 1], b[kHeld ? P : 1];
     if constexpr (kHeld) {
         load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
@@ -381,7 +381,7 @@ struct LnBwdParams {
 };
 
 // CTAs of so many threads whose registers an SM holds: the accumulators alone are 2 P W registers.
-__host__ __device__ constexpr int bwd_ctas(int w, int p) { return row_threads(w, p) == kLnCta ? 1 : w == 1 && p > 2 ? 2 : 3; }
+__host__ __device__ constexpr int bwd_ctas(int w, int p) { return row_threads(w, p) == kLnCta ? 1 : w == 2 && p > 2 ? 2 : 3; }
 
 template <typename T, typename WT, int W, int P, bool BLOCK>
 __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(LnBwdParams p) {
@@ -578,7 +578,7 @@ __global__ void __launch_bounds__(1024) k_ln_bwd_long(LnBwdParams p) {
 
 // Column sums of the CTAs' partial rows, in a fixed order: 32 columns per CTA, R threads share a column's rows and have four of
 // them in flight each. R = 32; 4 for few rows, where the threads of a wide CTA would find nothing (4 rows of 14801 columns: 14
-// against 4 us; with 16 threads and one row at a time 296 rows of 4096 took 17 us, all of it latency).
+// -> 10 us, started under the kernel before; with 16 threads and one row at a time 296 rows of 4096 took 17 us, all latency).
 template <typename OT, int R>
 __global__ void __launch_bounds__(32 * R) k_col_reduce(const float* __restrict__ partial, int n, int c, int64_t pitch, OT* __restrict__ o0,
                                                        OT* __restrict__ o1) {
@@ -750,7 +750,7 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
 // Teams of lanes: a warp reads the mask of `chunk` pixels at once, lists the active ones and hands them to its teams, so that
 // sparse maps cost one coalesced mask read and no idle teams. The next chunk's mask is on its way meanwhile.
 template <typename T, typename WT, int W, int P>
-__global__ void __launch_bounds__(256, P == 1 ? 4 : 1) k_ln_delta(LnDeltaParams p) {
+__global__ void __launch_bounds__(256, P == 1 ? 4 : W > 2 ? 1 : 3) k_ln_delta(LnDeltaParams p) {
     __shared__ uint8_t list[8][32], kept[8][32];
     grid_dep_launch();
     grid_dep_wait();
@@ -825,26 +825,30 @@ struct LnShape {
 
 // warp_packs: most packs per lane of a row that a group of lanes takes (more registers per lane than a CTA's threads need, but
 // no barriers).
-static LnShape ln_shape(int c, int64_t rows, int elem_bytes, bool aligned, int warp_packs) {
+// access: bytes that the arrays' addresses allow, 16, 4 or less.
+static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int warp_packs) {
     LnShape s{};
     const int vec = 16 / elem_bytes;
-    s.w = aligned && c % vec == 0 ? vec : 1;
+    // 16-byte packs; two halves where a row's width or place allows no more (half the instructions of single ones); elements
+    s.w = access >= 16 && c % vec == 0 ? vec : elem_bytes == 2 && access >= 4 && c % 2 == 0 ? 2 : 1;
     const int n = c / s.w;
-    // single elements: eight per thread, so that a thread has as many bytes in flight as a packed one
-    if (n <= 32 * (s.w > 1 ? warp_packs : 8)) {
+    // narrow accesses: at least four per thread, so that a thread has several reads in flight
+    const bool wide = s.w == vec;
+    if (n <= 32 * (wide ? warp_packs : 4)) {
         s.g = lanes_per_pixel(n);
         // Rows enough for every SM's threads all the same: fewer lanes with more packs each shuffle less per element (96 channels
-        // in fp16, 200000 rows: 16 lanes of one pack 25 us, 4 lanes of three 20 us).
-        while (s.w > 1 && s.g > 1 && divup(n, s.g / 2) <= warp_packs && rows * (s.g / 2) >= (int64_t)sm_count() * 1024) s.g /= 2;
+        // in fp16, 200000 rows: 16 lanes of one pack 25 us, 4 lanes of three 17.8 us).
+        while (wide && s.g > 1 && divup(n, s.g / 2) <= warp_packs && rows * (s.g / 2) >= (int64_t)sm_count() * 1024) s.g /= 2;
         const int need = divup(n, s.g);
-        s.p = s.w == 1 ? (need <= 2 ? 2 : 8) : need;
+        s.p = wide ? need : need <= 2 ? 2 : 4;
         s.threads = 256;
         return s;
     }
-    s.p = s.w == 1 ? (n <= 2048 ? 8 : 16) : n <= 256 ? 1 : n <= 2 * kLnCta ? 2 : 4;
+    s.p = wide ? (n <= 256 ? 1 : n <= 2 * kLnCta ? 2 : 4) : n <= 512 ? 4 : s.w == 2 || n <= 4096 ? 8 : 16;
     const int threads = divup(divup(n, s.p), 32) * 32;
     if (threads <= kLnCta) { s.threads = threads; return s; }
     s.p = 0; s.threads = 1024;
+    if (!wide) s.w = 1;
     return s;
 }
 
@@ -880,9 +884,17 @@ static int64_t ln_ctas(const LnShape& s, int64_t rows, int per_sm) {
         DC_LN_CASE(1, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(2, KERNEL, T, WT, W, BLOCK)                          \
         DC_LN_CASE(3, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(4, KERNEL, T, WT, W, BLOCK) default: break;          \
     }
-// Single elements, and the delta kernels have no BLOCK parameter.
-#define DC_LN_SINGLE_WARP(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(2, KERNEL, T, WT, 1, false) DC_LN_CASE(8, KERNEL, T, WT, 1, false) default: break; }
-#define DC_LN_SINGLE_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
+// Narrow accesses: single elements (W 1) or two halves (W 2).
+#define DC_LN_NARROW_WARP(KERNEL, T, WT, W) \
+    switch (s.p) { DC_LN_CASE(2, KERNEL, T, WT, W, false) DC_LN_CASE(4, KERNEL, T, WT, W, false) default: break; }
+#define DC_LN_SINGLE_CTA(KERNEL, T, WT) \
+    switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 1, true) DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
+#define DC_LN_PAIR_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 2, true) DC_LN_CASE(8, KERNEL, T, WT, 2, true) default: break; }
+// The kernel of teams of lanes and the one of a CTA per row, for every access.
+#define DC_LN_ALL(WARP_KERNEL, WARP_PACKS, CTA_KERNEL, T, WT)                                                                       \
+    if (s.w == V) { if (s.g > 0) { WARP_PACKS(WARP_KERNEL, T, WT, V, false) } else { DC_LN_PACKS4(CTA_KERNEL, T, WT, V, true) } }    \
+    else if (s.w == 1) { if (s.g > 0) { DC_LN_NARROW_WARP(WARP_KERNEL, T, WT, 1) } else { DC_LN_SINGLE_CTA(CTA_KERNEL, T, WT) } }    \
+    else if constexpr (sizeof(T) == 2) { if (s.g > 0) { DC_LN_NARROW_WARP(WARP_KERNEL, T, WT, 2) } else { DC_LN_PAIR_CTA(CTA_KERNEL, T, WT) } }
 
 #define DC_LN_TAIL(BLOCK) , BLOCK
 template <auto KERNEL>
@@ -893,12 +905,11 @@ static int ln_forward_run(const LnShape& s, LnParams& p, size_t smem, cudaStream
 template <typename T, typename WT>
 static int ln_forward_t(const LnShape& s, LnParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
-    const size_t smem = s.w > 1 ? (size_t)s.threads * s.p * (rows_ahead(s.p) + 1) * 16 : 0;
+    const size_t smem = s.w == V ? (size_t)s.threads * s.p * (rows_ahead(s.p) + 1) * 16 : 0;
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_forward_run<K>(s, p, smem, st)
-    if (s.p == 0) return s.w > 1 ? ln_forward_run<k_ln_fwd_long<T, WT, V>>(s, p, 0, st) : ln_forward_run<k_ln_fwd_long<T, WT, 1>>(s, p, 0, st);
-    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS1234(k_ln_fwd, T, WT, V, false) } else { DC_LN_PACKS4(k_ln_fwd, T, WT, V, true) } }
-    else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_fwd, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_fwd, T, WT) } }
+    if (s.p == 0) return s.w == V ? ln_forward_run<k_ln_fwd_long<T, WT, V>>(s, p, 0, st) : ln_forward_run<k_ln_fwd_long<T, WT, 1>>(s, p, 0, st);
+    DC_LN_ALL(k_ln_fwd, DC_LN_PACKS1234, k_ln_fwd, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
@@ -917,16 +928,15 @@ static int ln_backward_run(const LnShape& s, LnBwdParams& p, int64_t ctas, size_
 template <typename T, typename WT>
 static int ln_backward_t(const LnShape& s, LnBwdParams& p, int64_t ctas, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
-    size_t smem = s.w > 1 ? (size_t)s.threads * s.p * 2 * (rows_ahead(2 * s.p) + 1) * 16 : 0;
+    size_t smem = s.w == V ? (size_t)s.threads * s.p * 2 * (rows_ahead(2 * s.p) + 1) * 16 : 0;
     if (s.g > 0 && smem < (size_t)8 * p.c) smem = (size_t)8 * p.c;
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_backward_run<K>(s, p, ctas, smem, st)
     if (s.p == 0) {
         smem = (size_t)p.c * 8 <= (size_t)kLongSmem ? (size_t)kLongSmem : 0;
-        return s.w > 1 ? ln_backward_run<k_ln_bwd_long<T, WT, V>>(s, p, ctas, smem, st) : ln_backward_run<k_ln_bwd_long<T, WT, 1>>(s, p, ctas, smem, st);
+        return s.w == V ? ln_backward_run<k_ln_bwd_long<T, WT, V>>(s, p, ctas, smem, st) : ln_backward_run<k_ln_bwd_long<T, WT, 1>>(s, p, ctas, smem, st);
     }
-    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS2(k_ln_bwd, T, WT, V, false) } else { DC_LN_PACKS4(k_ln_bwd, T, WT, V, true) } }
-    else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_bwd, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_bwd, T, WT) } }
+    DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, k_ln_bwd, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
@@ -947,8 +957,7 @@ static int ln_delta_t(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_delta_run<K>(s, p, st)
-    if (s.w > 1) { if (s.g > 0) { DC_LN_PACKS1234(k_ln_delta, T, WT, V, ) } else { DC_LN_PACKS4(k_ln_delta_cta, T, WT, V, ) } }
-    else { if (s.g > 0) { DC_LN_SINGLE_WARP(k_ln_delta, T, WT) } else { DC_LN_SINGLE_CTA(k_ln_delta_cta, T, WT) } }
+    DC_LN_ALL(k_ln_delta, DC_LN_PACKS1234, k_ln_delta_cta, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
@@ -969,6 +978,12 @@ static bool ln_dtypes_ok(int dtype, int weight_dtype) {
 }
 static int ln_elem(int dtype) { return dtype == DC_F32 ? 4 : 2; }
 
+// Bytes that an access of the arrays may take: 16, 4, or an element's.
+static int ln_access(std::initializer_list<const void*> arrays, const void* weight, const void* bias) {
+    uintptr_t a = 0;
+    for (const void* p : arrays) a |= reinterpret_cast<uintptr_t>(p);
+    return !aligned16(weight) || !aligned16(bias) ? 1 : (a & 15u) == 0 ? 16 : (a & 3u) == 0 ? 4 : 1;
+}
 constexpr int kFwdWarpPacks = 4, kBwdWarpPacks = 2, kDeltaWarpPacks = 4;
 
 }  // namespace dc
@@ -983,16 +998,20 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
     if (rows < 0 || c <= 0) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     if (rows == 0) return DC_OK;
-    const LnShape s = ln_shape(c, rows, ln_elem(dtype), aligned16(x) && aligned16(y) && aligned16(weight) && aligned16(bias), kFwdWarpPacks);
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({x, y}, weight, bias), kFwdWarpPacks);
     LnParams p{x, weight, bias, y, mean, rstd, rows, c, c / s.w, s.g, eps, 1.f / (float)c};
     DC_LN_TYPES(ln_forward_t, s, p, (cudaStream_t)stream)
 }
 
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype) {
     if (rows <= 0 || c <= 0 || dtype < DC_F32 || dtype > DC_BF16) return 0;
-    // the split may differ with the pointers' alignment: room for either
-    const int64_t a = ln_backward_ctas(ln_shape(c, rows, ln_elem(dtype), true, kBwdWarpPacks), rows), b = ln_backward_ctas(ln_shape(c, rows, ln_elem(dtype), false, kBwdWarpPacks), rows);
-    return (size_t)((a > b ? a : b) * 2 * c) * sizeof(float);
+    // the split may differ with the pointers' alignment: room for any
+    int64_t most = 0;
+    for (int access : {16, 4, 1}) {
+        const int64_t n = ln_backward_ctas(ln_shape(c, rows, ln_elem(dtype), access, kBwdWarpPacks), rows);
+        if (n > most) most = n;
+    }
+    return (size_t)(most * 2 * c) * sizeof(float);
 }
 
 int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
@@ -1006,7 +1025,7 @@ int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (sums && workspace == nullptr)) return DC_ERR_NULL_POINTER;
     if (dx == nullptr && !sums) return DC_OK;
     if (sums && (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0) return DC_ERR_ALIGNMENT;
-    const LnShape s = ln_shape(c, rows, ln_elem(dtype), aligned16(dy) && aligned16(x) && aligned16(dx) && aligned16(weight), kBwdWarpPacks);
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({dy, x, dx}, weight, nullptr), kBwdWarpPacks);
     const int64_t ctas = ln_backward_ctas(s, rows);
     if (sums && workspace_bytes < (size_t)(ctas * 2 * c) * sizeof(float)) return DC_ERR_WORKSPACE;
     LnBwdParams p{dy, x, weight, mean, rstd, dx, sums ? (float*)workspace : nullptr, rows, c, c / s.w, s.g, 1.f / (float)c};
@@ -1023,8 +1042,7 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
     if (npix < 0 || c <= 0) return DC_ERR_SHAPE;
     if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;      // the caches are those of the delta path
     if (npix == 0) return DC_OK;
-    const LnShape s = ln_shape(c, 0, ln_elem(dtype), aligned16(delta) && aligned16(prev_in) && aligned16(prev_out) && aligned16(out) &&
-                                                      aligned16(weight) && aligned16(bias), kDeltaWarpPacks);
+    const LnShape s = ln_shape(c, 0, ln_elem(dtype), ln_access({delta, prev_in, prev_out, out}, weight, bias), kDeltaWarpPacks);
     if (s.p == 0) return DC_ERR_UNSUPPORTED;      // more channels than the registers of a CTA hold
     const float thr = dtype == DC_F16 ? host_round_threshold<__half>(threshold) : threshold;
     LnDeltaParams p{delta, weight, bias, mask, prev_in, prev_out, out, mask_out, npix, c, c / s.w, s.g, thr, eps, 1.f / (float)c, 32};

@@ -61,7 +61,7 @@ def y_bound(w, b, n, a, y, t):
 
 SHAPES = [(1, 1), (5, 1), (1, 8), (3, 7), (40, 24), (5, 33), (259, 64), (2, 96), (130, 100), (33, 1000), (7, 1024), (3, 1032), (6, 1001),
           (2, 4096), (3, 4100), (2, 4099), (2, 8192), (3, 16384), (2, 20000), (1, 40000), (1500, 8), (700, 257),
-          (2, 9001), (3, 2500), (2, 10000), (80001, 96), (160001, 24), (30000, 512)]
+          (2, 9001), (3, 2500), (2, 10000), (300, 50), (90, 82), (41, 170), (77, 430), (5, 514), (3, 8190), (2, 8194), (9, 2), (80001, 96), (160001, 24), (30000, 512)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -200,6 +200,14 @@ def test_layer_norm_unaligned_rows_and_empty_input():
     w, b = randn((64,), g), randn((64,), g)
     y64, n, r, a = norm64(x, w.double(), b.double())
     within(dc().layer_norm(x, w, b), y64, y_bound(w.double(), b.double(), n, a, y64, F32))
+    for off in (1, 2):                      # halves two and four bytes off, with a gradient of another alignment
+        h = randn((off + 6 * 72,), g, F16)[off:].view(6, 72).requires_grad_()
+        wh = randn((72,), g, F16).requires_grad_()
+        dy = randn((3 - off + 6 * 72,), g, F16)[3 - off:].view(6, 72)
+        got = torch.autograd.grad(dc().layer_norm(h, wh), (h, wh), dy)
+        want = torch.autograd.grad(dc().layer_norm(h2 := h.detach().clone().requires_grad_(), w2 := wh.detach().clone().requires_grad_()), (h2, w2), dy.clone())
+        for p, q in zip(got, want):         # the same sums in another order, rounded once
+            assert (p.float() - q.float()).abs().max() <= 2 * half(F16) * q.float().abs().max() + 1e-4
     e = torch.empty((0, 64), device="cuda", requires_grad=True)
     w.requires_grad_(), b.requires_grad_()
     dx, dw, db = torch.autograd.grad(dc().layer_norm(e, w, b).sum(), (e, w, b))
@@ -228,7 +236,7 @@ def delta64(delta, mask, prev_in, prev_out, w, b, thr):
 
 
 @pytest.mark.parametrize("dtype", [F32, F16])
-@pytest.mark.parametrize("n,h,w,c", [(1, 1, 1, 8), (2, 5, 7, 24), (3, 9, 11, 64), (1, 16, 16, 100), (2, 6, 6, 576), (1, 5, 5, 1280), (1, 3, 5, 33), (1, 3, 3, 1001), (1, 2, 3, 4096), (1, 2, 3, 8191), (1, 1, 2, 8192), (40, 30, 30, 72)])
+@pytest.mark.parametrize("n,h,w,c", [(1, 1, 1, 8), (2, 5, 7, 24), (3, 9, 11, 64), (1, 16, 16, 100), (2, 6, 6, 576), (1, 5, 5, 1280), (1, 3, 5, 33), (1, 3, 3, 1001), (1, 2, 3, 4096), (1, 2, 3, 8191), (1, 1, 2, 8192), (40, 30, 30, 72), (3, 9, 9, 82), (2, 7, 7, 212), (1, 6, 5, 430), (1, 3, 3, 1002), (1, 2, 2, 8190)])
 @pytest.mark.parametrize("density", [0.0, 0.3, 1.0])
 def test_layer_norm_delta(dtype, n, h, w, c, density):
     g = gen(c + int(density * 10))
