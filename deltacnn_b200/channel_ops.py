@@ -141,13 +141,11 @@ class _LayerNorm(torch.autograd.Function):
         dx = torch.empty_like(x) if need_x else None
         dw = x.new_empty(c, dtype=wtype) if need_w else None
         db = x.new_empty(c, dtype=wtype) if need_b else None
-        ws, nbytes = None, 0
-        if need_w or need_b:
-            nbytes = _bytes_wanted("dc_layer_norm_backward_workspace_bytes", x.get_device(), rows, c, code)
-            ws = x.new_empty(nbytes, dtype=torch.uint8)
+        nbytes = _bytes_wanted("dc_layer_norm_backward_workspace_bytes", x.get_device(), rows, c, code)
+        ws = x.new_empty(nbytes, dtype=torch.uint8)
         mean = stats.data_ptr()
         _launch("layer_norm_backward", lib.dc_layer_norm_backward, x, dy.data_ptr(), x.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw),
-                _ptr(db), rows, c, code, _CODES[wtype], _ptr(ws), nbytes)
+                _ptr(db), rows, c, code, _CODES[wtype], ws.data_ptr(), nbytes)
         return dx, dw, db, None
 
     @staticmethod

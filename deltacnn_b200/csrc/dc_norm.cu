@@ -11,7 +11,7 @@
 // their own slots of shared memory); weight, and the column sums of the backward pass, stay in registers, whose per-CTA rests a
 // second kernel adds in a fixed order. Rows whose width or address does not allow 16-byte accesses take the same code with
 // two halves or single elements (delta form, 82 channels 73 x 18 x 42: 44 us with single halves, 18 with two); rows beyond the
-// registers of a CTA are read two or three times by a plain loop.
+// registers of a CTA pass through shared memory (forward) or are read twice (backward).
 //
 // Bound: memory, once the arithmetic is packed (two float32 per instruction): 16384 x 4096 bf16 forward 45 us (268 MB, 41 us at
 // the copy rate), backward 72 us (403 MB, 61 us); with scalar arithmetic and a branch per pack the issue slots were the bound
@@ -326,43 +326,104 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
     }
 }
 
-// Rows beyond the registers of a CTA: three reads, the second and third mostly from L2.
-template <typename T, typename WT, int W>
-__global__ void __launch_bounds__(1024) k_ln_fwd_long(LnParams p) {
+// Rows beyond the registers of a CTA. Three CTAs of 512 threads per SM, so that one's barriers pass under another's reads; every
+// thread asks for several packs before it uses the first.
+constexpr int kLongThreads = 512, kLongCtas = 3;
+template <int W> constexpr int kLongBatch = W == 1 ? 8 : W == 8 ? 1 : W == 2 ? 4 : 2;
+constexpr int kLongSmem = 200 * 1024;
+
+// A thread's packs of a row of n, a batch at a time: body(first pack, all of them inside the row). The CTA's size is a constant,
+// so that a batch's accesses are one address with constant offsets, and only the last batch looks where the row ends: with a
+// bound on every element and 64-bit products for its address a forward pass of 15001 elements in bf16 took 79 instructions per
+// element, and 104 us instead of 58 us for 2236 rows.
+template <int W, typename F>
+__device__ __forceinline__ void long_row(int n, F&& body) {
+    constexpr int B = kLongBatch<W>;
+    int i = threadIdx.x;
+    for (; i + (B - 1) * kLongThreads < n; i += B * kLongThreads) body(i, std::true_type{});
+    if (i < n) body(i, std::false_type{});
+}
+// Packs i, i + kLongThreads, ... of p; those behind the end, and all of an absent one, are `other`.
+template <bool ALL, typename T, int W>
+__device__ __forceinline__ void long_load(Frag<T, W> (&v)[kLongBatch<W>], const T* p, int i, int n, float other) {
+    p += (int64_t)i * W;
+#pragma unroll
+    for (int k = 0; k < kLongBatch<W>; ++k)
+        if (ALL || i + k * kLongThreads < n) v[k].load(p + k * kLongThreads * W);
+        else v[k].fill(other);
+}
+template <bool ALL, typename T, int W>
+__device__ __forceinline__ void long_param(Frag<T, W> (&v)[kLongBatch<W>], const T* p, int i, int n, float other) {
+    if (p != nullptr) long_load<ALL, T, W>(v, p, i, n, other);
+    else
+#pragma unroll
+        for (int k = 0; k < kLongBatch<W>; ++k) v[k].fill(other);
+}
+
+// One read of a row that shared memory holds meanwhile (HELD: every thread reads back its own packs); longer ones are read three
+// times, the second and third time mostly from L2.
+template <typename T, typename WT, int W, bool HELD>
+__global__ void __launch_bounds__(kLongThreads, kLongCtas) k_ln_fwd_long(LnParams p) {
     __shared__ float red[2][kMaxWarps];
+    extern __shared__ __align__(16) uint8_t held[];
+    constexpr int B = kLongBatch<W>;
+    using V = typename Vals<W>::V;
+    constexpr int N = Vals<W>::N;
     grid_dep_launch();
     grid_dep_wait();
     const Team<true> t(0);
     for (int64_t row = t.row; row < p.rows; row += t.stride) {
         const T* x = (const T*)p.x + row * p.c;
+        const T* again = HELD ? reinterpret_cast<const T*>(held) : x;
         T* y = (T*)p.y + row * p.c;
-        float s = 0.f, q = 0.f;
-        Frag<T, W> v;
-#pragma unroll 4
-        for (int i = t.rank; i < p.nvec; i += t.size) {
-            v.load(x + (int64_t)i * W);
+        V s = V::all(0.f), q = V::all(0.f);
+        long_row<W>(p.nvec, [&](int i, auto all) {
+            Frag<T, W> v[B];
+            long_load<all.value, T, W>(v, x, i, p.nvec, 0.f);
 #pragma unroll
-            for (int j = 0; j < W; ++j) s += v.get(j);
-        }
-        const float m = t.sum(s, red[0]) * p.inv_c;
-#pragma unroll 4
-        for (int i = t.rank; i < p.nvec; i += t.size) {
-            v.load(x + (int64_t)i * W);
+            for (int k = 0; k < B; ++k) {
+                if (HELD && (all.value || i + k * kLongThreads < p.nvec)) v[k].store(reinterpret_cast<T*>(held) + (i + k * kLongThreads) * W);
+                Vals<W> f;
+                f.from(v[k]);
 #pragma unroll
-            for (int j = 0; j < W; ++j) { const float d = v.get(j) - m; q += d * d; }
-        }
-        const float r = rsqrtf(t.sum(q, red[1]) * p.inv_c + p.eps);
-        for (int i = t.rank; i < p.nvec; i += t.size) {
-            Frag<WT, W> w, b;
-            w.fill(1.f);
-            b.fill(0.f);
-            v.load(x + (int64_t)i * W);
-            if (p.w != nullptr) w.load((const WT*)p.w + (int64_t)i * W);
-            if (p.b != nullptr) b.load((const WT*)p.b + (int64_t)i * W);
+                for (int j = 0; j < N; ++j) s = add(s, f.v[j]);
+            }
+        });
+        const float m = t.sum(s.sum(), red[0]) * p.inv_c;
+        const V neg = V::all(-m);
+        long_row<W>(p.nvec, [&](int i, auto all) {
+            Frag<T, W> v[B];
+            long_load<all.value, T, W>(v, again, i, p.nvec, 0.f);
 #pragma unroll
-            for (int j = 0; j < W; ++j) v.set(j, (v.get(j) - m) * r * w.get(j) + b.get(j));
-            v.store(y + (int64_t)i * W);
-        }
+            for (int k = 0; k < B; ++k)
+                if (all.value || i + k * kLongThreads < p.nvec) {
+                    Vals<W> f;
+                    f.from(v[k]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) { const V d = add(f.v[j], neg); q = fma(d, d, q); }
+                }
+        });
+        const float r = rsqrtf(t.sum(q.sum(), red[1]) * p.inv_c + p.eps);
+        const V rr = V::all(r);
+        long_row<W>(p.nvec, [&](int i, auto all) {
+            Frag<T, W> v[B];
+            Frag<WT, W> w[B], b[B];
+            long_load<all.value, T, W>(v, again, i, p.nvec, 0.f);
+            long_param<all.value, WT, W>(w, (const WT*)p.w, i, p.nvec, 1.f);
+            long_param<all.value, WT, W>(b, (const WT*)p.b, i, p.nvec, 0.f);
+            T* const o = y + (int64_t)i * W;
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                Vals<W> f, ww, bb;
+                f.from(v[k]);
+                ww.from(w[k]);
+                bb.from(b[k]);
+#pragma unroll
+                for (int j = 0; j < N; ++j) f.v[j] = fma(mul(add(f.v[j], neg), rr), ww.v[j], bb.v[j]);
+                f.to(v[k]);
+                if (all.value || i + k * kLongThreads < p.nvec) v[k].store(o + k * kLongThreads * W);
+            }
+        });
         if (t.rank == 0 && p.mean != nullptr) { p.mean[row] = m; p.rstd[row] = r; }
     }
 }
@@ -374,8 +435,9 @@ struct LnBwdParams {
     const void *dy, *x, *w;
     const float *mean, *rstd;
     void* dx;
-    float* partial;            // [gridDim.x][2][c]: this CTA's sums of dy n and dy; NULL: not wanted
-    int64_t rows;
+    float* partial;            // [slices][2][c]: a CTA's sums of dy n and dy; NULL: not wanted
+    float* means;              // long rows: [rows][2], the rows' means of g and g n
+    int64_t rows, per;         // per: long rows, rows of a block
     int c, nvec, g;
     float inv_c;
 };
@@ -517,63 +579,138 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
     }
 }
 
-// Long rows: the row's two sums in a first loop, dx in a second. A column belongs to one thread, which adds its sums in shared
-// memory, or in the CTA's own slice of the workspace where they do not fit there.
-constexpr int kLongSmem = 200 * 1024;
+// Long rows, in two kernels (2236 x 15001 in bf16 227 -> 132 us, 1677 x 20000 205 -> 67 us against one that kept the column sums in
+// shared memory), since no thread can keep the column sums of a whole row's share: the rows' two means (every row once),
+// then dx and the column sums by CTAs that own a block of columns and walk down some rows (every row once more, and weight and
+// the sums in registers). The second read comes from L2 where the batch fits there.
 template <typename T, typename WT, int W>
-__global__ void __launch_bounds__(1024) k_ln_bwd_long(LnBwdParams p) {
+__global__ void __launch_bounds__(kLongThreads, kLongCtas) k_ln_bwd_means(LnBwdParams p) {
     __shared__ float red[2][kMaxWarps];
-    extern __shared__ __align__(16) uint8_t ring[];
+    constexpr int B = kLongBatch<W>;
+    using V = typename Vals<W>::V;
+    constexpr int N = Vals<W>::N;
     grid_dep_launch();
     grid_dep_wait();
     const Team<true> t(0);
-    const bool inside = (size_t)p.c * 8 <= (size_t)kLongSmem;
-    float* out = p.partial == nullptr ? nullptr : p.partial + (int64_t)blockIdx.x * 2 * p.c;
-    float* cols = inside ? reinterpret_cast<float*>(ring) : out;
-    if (out != nullptr)
-        for (int i = t.rank; i < p.nvec; i += t.size)
-#pragma unroll
-            for (int j = 0; j < W; ++j) cols[(int64_t)i * W + j] = cols[p.c + (int64_t)i * W + j] = 0.f;
     for (int64_t row = t.row; row < p.rows; row += t.stride) {
         const T *x = (const T*)p.x + row * p.c, *dy = (const T*)p.dy + row * p.c;
-        const float m = p.mean[row], r = p.rstd[row];
-        float sg = 0.f, sgn = 0.f;
-#pragma unroll 2
-        for (int i = t.rank; i < p.nvec; i += t.size) {
-            Frag<T, W> v, d;
-            Frag<WT, W> w;
-            w.fill(1.f);
-            v.load(x + (int64_t)i * W);
-            d.load(dy + (int64_t)i * W);
-            if (p.w != nullptr) w.load((const WT*)p.w + (int64_t)i * W);
+        const V neg = V::all(-p.mean[row]), r = V::all(p.rstd[row]);
+        V sg = V::all(0.f), sgn = V::all(0.f);
+        long_row<W>(p.nvec, [&](int i, auto all) {
+            Frag<T, W> v[B], d[B];
+            Frag<WT, W> w[B];
+            long_load<all.value, T, W>(v, x, i, p.nvec, 0.f);
+            long_load<all.value, T, W>(d, dy, i, p.nvec, 0.f);
+            long_param<all.value, WT, W>(w, (const WT*)p.w, i, p.nvec, 1.f);
 #pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const float n = (v.get(j) - m) * r, e = d.get(j), g = e * w.get(j);
-                if (out != nullptr) { cols[(int64_t)i * W + j] += e * n; cols[p.c + (int64_t)i * W + j] += e; }
-                sg += g;
-                sgn += g * n;
+            for (int k = 0; k < B; ++k)
+                if (all.value || i + k * kLongThreads < p.nvec) {
+                    Vals<W> n, e, ww;
+                    n.from(v[k]);
+                    e.from(d[k]);
+                    ww.from(w[k]);
+#pragma unroll
+                    for (int j = 0; j < N; ++j) {
+                        const V g = mul(e.v[j], ww.v[j]);
+                        sg = add(sg, g);
+                        sgn = fma(g, mul(add(n.v[j], neg), r), sgn);
+                    }
+                }
+        });
+        const float a = t.sum(sg.sum(), red[0]) * p.inv_c, c = t.sum(sgn.sum(), red[1]) * p.inv_c;
+        if (t.rank == 0) { p.means[2 * row] = a; p.means[2 * row + 1] = c; }
+    }
+}
+
+constexpr int kColThreads = 256, kColCtas = 3, kColMinRows = 8;
+template <int W> constexpr int kColRows = W == 8 ? 2 : 4;      // in flight
+template <int W> constexpr int kColPacks = W >= 4 ? 1 : 4 / W;
+// grid: blocks of columns x blocks of p.per rows.
+template <typename T, typename WT, int W>
+__global__ void __launch_bounds__(kColThreads, kColCtas) k_ln_bwd_cols(LnBwdParams p) {
+    constexpr int K = kColPacks<W>, R = kColRows<W>;
+    using V = typename Vals<W>::V;
+    constexpr int N = Vals<W>::N;
+    grid_dep_launch();
+    grid_dep_wait();
+    const int first = blockIdx.x * kColThreads * K + threadIdx.x;
+    Frag<WT, W> w[K];
+    load_param<WT, W, K>(w, (const WT*)p.w, first, kColThreads, p.nvec, 1.f);
+    Vals<W> dw[K], db[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int i = 0; i < N; ++i) dw[k].v[i] = db[k].v[i] = V::all(0.f);
+    const int64_t begin = (int64_t)blockIdx.y * p.per, end = begin + p.per < p.rows ? begin + p.per : p.rows;
+    unsigned valid = 0;
+#pragma unroll
+    for (int k = 0; k < K; ++k) valid |= first + k * kColThreads < p.nvec ? 1u << k : 0u;
+    int64_t at = begin * p.c + (int64_t)first * W;
+    // rows row ... row + R - 1; ALL: none is behind the end, and all of the thread's columns are inside
+    auto take = [&](int64_t row, auto all) {
+        constexpr bool ALL = all.value;
+        Frag<T, W> x[R][K], dy[R][K];
+        float m[R], r[R], a[R], c[R];
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const bool on = ALL || row + j < end;
+            m[j] = r[j] = a[j] = c[j] = 0.f;
+            if (on) {
+                m[j] = p.mean[row + j];
+                r[j] = p.rstd[row + j];
+                if (p.dx != nullptr) { a[j] = p.means[2 * (row + j)]; c[j] = p.means[2 * (row + j) + 1]; }
+            }
+            const T *px = (const T*)p.x + at + (int64_t)j * p.c, *pd = (const T*)p.dy + at + (int64_t)j * p.c;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                if (ALL || (on && (valid >> k & 1u))) {
+                    x[j][k].load(px + k * kColThreads * W);
+                    dy[j][k].load(pd + k * kColThreads * W);
+                } else {
+                    x[j][k].fill(0.f);
+                    dy[j][k].fill(0.f);
+                }
+        }
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+            const V neg = V::all(-m[j]), rr = V::all(r[j]), na = V::all(-a[j]), nc = V::all(-c[j]);
+            T* o = (T*)p.dx + at + (int64_t)j * p.c;
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                Vals<W> n, e, ww;
+                n.from(x[j][k]);
+                e.from(dy[j][k]);
+                ww.from(w[k]);
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    n.v[i] = mul(add(n.v[i], neg), rr);
+                    dw[k].v[i] = fma(e.v[i], n.v[i], dw[k].v[i]);
+                    db[k].v[i] = add(db[k].v[i], e.v[i]);
+                    e.v[i] = mul(rr, fma(n.v[i], nc, add(mul(e.v[i], ww.v[i]), na)));
+                }
+                if (p.dx != nullptr && (ALL || (row + j < end && (valid >> k & 1u)))) {
+                    e.to(x[j][k]);
+                    x[j][k].store(o + k * kColThreads * W);
+                }
             }
         }
-        if (p.dx == nullptr) continue;
-        const float a = t.sum(sg, red[0]) * p.inv_c, c = t.sum(sgn, red[1]) * p.inv_c;
-        T* dx = (T*)p.dx + row * p.c;
-#pragma unroll 2
-        for (int i = t.rank; i < p.nvec; i += t.size) {
-            Frag<T, W> v, d;
-            Frag<WT, W> w;
-            w.fill(1.f);
-            v.load(x + (int64_t)i * W);
-            d.load(dy + (int64_t)i * W);
-            if (p.w != nullptr) w.load((const WT*)p.w + (int64_t)i * W);
+    };
+    int64_t row = begin;
+    if (valid == (1u << K) - 1)
+        for (; row + R <= end; row += R, at += (int64_t)R * p.c) take(row, std::true_type{});
+    for (; row < end; row += R, at += (int64_t)R * p.c) take(row, std::false_type{});
+    if (p.partial == nullptr) return;
+    float* out = p.partial + (int64_t)blockIdx.y * 2 * p.c;
 #pragma unroll
-            for (int j = 0; j < W; ++j) d.set(j, r * (d.get(j) * w.get(j) - a - (v.get(j) - m) * r * c));
-            d.store(dx + (int64_t)i * W);
+    for (int k = 0; k < K; ++k)
+        if (first + k * kColThreads < p.nvec) {
+            const int col = (first + k * kColThreads) * W;
+            Frag<float, W> f;
+            dw[k].put(f.s);
+            f.store(out + col);
+            db[k].put(f.s);
+            f.store(out + p.c + col);
         }
-    }
-    if (out != nullptr && inside)
-        for (int i = t.rank; i < p.nvec; i += t.size)
-#pragma unroll
-            for (int j = 0; j < W; ++j) { out[(int64_t)i * W + j] = cols[(int64_t)i * W + j]; out[p.c + (int64_t)i * W + j] = cols[p.c + (int64_t)i * W + j]; }
 }
 
 // Column sums of the CTAs' partial rows, in a fixed order: 32 columns per CTA, R threads share a column's rows and have four of
@@ -824,9 +961,9 @@ struct LnShape {
 };
 
 // warp_packs: most packs per lane of a row that a group of lanes takes (more registers per lane than a CTA's threads need, but
-// no barriers).
+// no barriers). cta_packs: most 16-byte packs per thread of a CTA.
 // access: bytes that the arrays' addresses allow, 16, 4 or less.
-static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int warp_packs) {
+static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int warp_packs, int cta_packs) {
     LnShape s{};
     const int vec = 16 / elem_bytes;
     // 16-byte packs; two halves where a row's width or place allows no more (half the instructions of single ones); elements
@@ -846,9 +983,8 @@ static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int war
     }
     s.p = wide ? (n <= 256 ? 1 : n <= 2 * kLnCta ? 2 : 4) : n <= 512 ? 4 : s.w == 2 || n <= 4096 ? 8 : 16;
     const int threads = divup(divup(n, s.p), 32) * 32;
-    if (threads <= kLnCta) { s.threads = threads; return s; }
-    s.p = 0; s.threads = 1024;
-    if (!wide) s.w = 1;
+    if (threads <= kLnCta && (!wide || s.p <= cta_packs)) { s.threads = threads; return s; }
+    s.p = 0; s.threads = kLongThreads;
     return s;
 }
 
@@ -891,8 +1027,8 @@ static int64_t ln_ctas(const LnShape& s, int64_t rows, int per_sm) {
     switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 1, true) DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
 #define DC_LN_PAIR_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 2, true) DC_LN_CASE(8, KERNEL, T, WT, 2, true) default: break; }
 // The kernel of teams of lanes and the one of a CTA per row, for every access.
-#define DC_LN_ALL(WARP_KERNEL, WARP_PACKS, CTA_KERNEL, T, WT)                                                                       \
-    if (s.w == V) { if (s.g > 0) { WARP_PACKS(WARP_KERNEL, T, WT, V, false) } else { DC_LN_PACKS4(CTA_KERNEL, T, WT, V, true) } }    \
+#define DC_LN_ALL(WARP_KERNEL, WARP_PACKS, CTA_KERNEL, CTA_PACKS, T, WT)                                                                       \
+    if (s.w == V) { if (s.g > 0) { WARP_PACKS(WARP_KERNEL, T, WT, V, false) } else { CTA_PACKS(CTA_KERNEL, T, WT, V, true) } }    \
     else if (s.w == 1) { if (s.g > 0) { DC_LN_NARROW_WARP(WARP_KERNEL, T, WT, 1) } else { DC_LN_SINGLE_CTA(CTA_KERNEL, T, WT) } }    \
     else if constexpr (sizeof(T) == 2) { if (s.g > 0) { DC_LN_NARROW_WARP(WARP_KERNEL, T, WT, 2) } else { DC_LN_PAIR_CTA(CTA_KERNEL, T, WT) } }
 
@@ -902,23 +1038,64 @@ static int ln_forward_run(const LnShape& s, LnParams& p, size_t smem, cudaStream
     const int64_t ctas = ln_ctas(s, p.rows, resident_ctas<KERNEL>(s.threads, smem));
     return launch_pdl(KERNEL, dim3((unsigned)ctas), dim3(s.threads), smem, st, p);
 }
+template <typename T, typename WT, int W>
+static int ln_forward_long(LnParams& p, cudaStream_t st) {
+    const size_t smem = (size_t)p.c * sizeof(T);
+    const bool held = smem <= kLongSmem;
+    // an SM's 227 KB, of which every CTA takes 1 KB and the sums of its warps besides
+    const int fit = held ? (int)(227 * 1024 / (smem + 1536)) : kLongCtas;
+    const int64_t cap = (int64_t)sm_count() * (fit < kLongCtas ? fit : kLongCtas);
+    const dim3 grid((unsigned)(p.rows < cap ? p.rows : cap));
+    if (!held) return launch_pdl(k_ln_fwd_long<T, WT, W, false>, grid, dim3(kLongThreads), 0, st, p);
+    (void)resident_ctas<k_ln_fwd_long<T, WT, W, true>>(kLongThreads, kLongSmem);      // sets the shared memory limit once per device
+    return launch_pdl(k_ln_fwd_long<T, WT, W, true>, grid, dim3(kLongThreads), smem, st, p);
+}
 template <typename T, typename WT>
 static int ln_forward_t(const LnShape& s, LnParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
     const size_t smem = s.w == V ? (size_t)s.threads * s.p * (rows_ahead(s.p) + 1) * 16 : 0;
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_forward_run<K>(s, p, smem, st)
-    if (s.p == 0) return s.w == V ? ln_forward_run<k_ln_fwd_long<T, WT, V>>(s, p, 0, st) : ln_forward_run<k_ln_fwd_long<T, WT, 1>>(s, p, 0, st);
-    DC_LN_ALL(k_ln_fwd, DC_LN_PACKS1234, k_ln_fwd, T, WT)
+    if (s.p == 0) {
+        if (s.w == V) return ln_forward_long<T, WT, V>(p, st);
+        if constexpr (sizeof(T) == 2) if (s.w == 2) return ln_forward_long<T, WT, 2>(p, st);
+        return ln_forward_long<T, WT, 1>(p, st);
+    }
+    DC_LN_ALL(k_ln_fwd, DC_LN_PACKS1234, k_ln_fwd, DC_LN_PACKS4, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
 
-// CTAs of the backward kernel; each owns a slice of the workspace, so the count depends on nothing but the sizes and the GPU: what
-// an SM holds at the kernels' register bounds.
-static int64_t ln_backward_ctas(const LnShape& s, int64_t rows) {
-    const int per_sm = s.p == 0 ? 1 : bwd_ctas(s.w, s.p) * row_threads(s.w, s.p) / s.threads;
-    return ln_ctas(s, rows, per_sm < 1 ? 1 : per_sm);
+// How the backward pass is split: slices of the workspace with a CTA's column sums each (long rows: a block of rows), which depend
+// on nothing but the sizes and the GPU; long rows: blocks of columns, rows of a block.
+struct LnSplit {
+    int64_t slices, per;
+    int blocks;
+};
+static LnSplit ln_split(const LnShape& s, int c, int64_t rows) {
+    LnSplit t{0, 0, 1};
+    if (s.p > 0) {      // what an SM holds at the kernels' register bounds
+        const int per_sm = bwd_ctas(s.w, s.p) * row_threads(s.w, s.p) / s.threads;
+        t.slices = ln_ctas(s, rows, per_sm < 1 ? 1 : per_sm);
+        return t;
+    }
+    t.blocks = divup(c / s.w, kColThreads * (s.w >= 4 ? 1 : 4 / s.w));
+    const int64_t room = (int64_t)sm_count() * kColCtas / t.blocks;      // one wave of CTAs
+    t.per = divup64(rows, room < 1 ? 1 : room);
+    if (t.per < kColMinRows) t.per = kColMinRows;
+    t.slices = divup64(rows, t.per);
+    return t;
+}
+static size_t ln_means_floats(const LnShape& s, int64_t rows) { return s.p == 0 ? (size_t)rows * 2 : 0; }
+
+template <typename T, typename WT, int W>
+static int ln_backward_long(LnBwdParams& p, const LnSplit& t, cudaStream_t st) {
+    if (p.dx != nullptr) {
+        const int64_t cap = (int64_t)sm_count() * kLongCtas;
+        const int rc = launch_pdl(k_ln_bwd_means<T, WT, W>, dim3((unsigned)(p.rows < cap ? p.rows : cap)), dim3(kLongThreads), 0, st, p);
+        if (rc != DC_OK) return rc;
+    }
+    return launch_pdl(k_ln_bwd_cols<T, WT, W>, dim3((unsigned)t.blocks, (unsigned)t.slices), dim3(kColThreads), 0, st, p);
 }
 template <auto KERNEL>
 static int ln_backward_run(const LnShape& s, LnBwdParams& p, int64_t ctas, size_t smem, cudaStream_t st) {
@@ -926,17 +1103,19 @@ static int ln_backward_run(const LnShape& s, LnBwdParams& p, int64_t ctas, size_
     return launch_pdl(KERNEL, dim3((unsigned)ctas), dim3(s.threads), smem, st, p);
 }
 template <typename T, typename WT>
-static int ln_backward_t(const LnShape& s, LnBwdParams& p, int64_t ctas, cudaStream_t st) {
+static int ln_backward_t(const LnShape& s, LnBwdParams& p, const LnSplit& t, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
     size_t smem = s.w == V ? (size_t)s.threads * s.p * 2 * (rows_ahead(2 * s.p) + 1) * 16 : 0;
     if (s.g > 0 && smem < (size_t)8 * p.c) smem = (size_t)8 * p.c;
     int rc = DC_ERR_UNSUPPORTED;
-#define DC_LN_RUN(K) rc = ln_backward_run<K>(s, p, ctas, smem, st)
+#define DC_LN_RUN(K) rc = ln_backward_run<K>(s, p, t.slices, smem, st)
     if (s.p == 0) {
-        smem = (size_t)p.c * 8 <= (size_t)kLongSmem ? (size_t)kLongSmem : 0;
-        return s.w == V ? ln_backward_run<k_ln_bwd_long<T, WT, V>>(s, p, ctas, smem, st) : ln_backward_run<k_ln_bwd_long<T, WT, 1>>(s, p, ctas, smem, st);
+        if (s.w == V) return ln_backward_long<T, WT, V>(p, t, st);
+        if constexpr (sizeof(T) == 2) if (s.w == 2) return ln_backward_long<T, WT, 2>(p, t, st);
+        return ln_backward_long<T, WT, 1>(p, t, st);
     }
-    DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, k_ln_bwd, T, WT)
+    if constexpr (sizeof(T) == 4) { DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, k_ln_bwd, DC_LN_PACKS4, T, WT) }
+    else { DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, k_ln_bwd, DC_LN_PACKS2, T, WT) }
 #undef DC_LN_RUN
     return rc;
 }
@@ -957,7 +1136,7 @@ static int ln_delta_t(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_delta_run<K>(s, p, st)
-    DC_LN_ALL(k_ln_delta, DC_LN_PACKS1234, k_ln_delta_cta, T, WT)
+    DC_LN_ALL(k_ln_delta, DC_LN_PACKS1234, k_ln_delta_cta, DC_LN_PACKS4, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
@@ -984,6 +1163,9 @@ static int ln_access(std::initializer_list<const void*> arrays, const void* weig
     for (const void* p : arrays) a |= reinterpret_cast<uintptr_t>(p);
     return !aligned16(weight) || !aligned16(bias) ? 1 : (a & 15u) == 0 ? 16 : (a & 3u) == 0 ? 4 : 1;
 }
+// Four packs of eight halves are 64 column sums per thread, which its 128 registers do not hold beside the row: the long kernels'
+// two reads are faster (3276 x 10240 in bf16: 87 -> 68 us).
+static int bwd_cta_packs(int elem_bytes) { return elem_bytes == 2 ? 2 : 4; }
 constexpr int kFwdWarpPacks = 4, kBwdWarpPacks = 2, kDeltaWarpPacks = 4;
 
 }  // namespace dc
@@ -998,7 +1180,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
     if (rows < 0 || c <= 0) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     if (rows == 0) return DC_OK;
-    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({x, y}, weight, bias), kFwdWarpPacks);
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({x, y}, weight, bias), kFwdWarpPacks, 4);
     LnParams p{x, weight, bias, y, mean, rstd, rows, c, c / s.w, s.g, eps, 1.f / (float)c};
     DC_LN_TYPES(ln_forward_t, s, p, (cudaStream_t)stream)
 }
@@ -1006,12 +1188,13 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype) {
     if (rows <= 0 || c <= 0 || dtype < DC_F32 || dtype > DC_BF16) return 0;
     // the split may differ with the pointers' alignment: room for any
-    int64_t most = 0;
+    size_t most = 0;
     for (int access : {16, 4, 1}) {
-        const int64_t n = ln_backward_ctas(ln_shape(c, rows, ln_elem(dtype), access, kBwdWarpPacks), rows);
+        const LnShape s = ln_shape(c, rows, ln_elem(dtype), access, kBwdWarpPacks, bwd_cta_packs(ln_elem(dtype)));
+        const size_t n = ln_means_floats(s, rows) + (size_t)ln_split(s, c, rows).slices * 2 * c;
         if (n > most) most = n;
     }
-    return (size_t)(most * 2 * c) * sizeof(float);
+    return most * sizeof(float);
 }
 
 int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
@@ -1022,16 +1205,22 @@ int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     const bool sums = dweight != nullptr || dbias != nullptr;
     cudaStream_t st = (cudaStream_t)stream;
     if (rows == 0) return sums ? col_reduce(nullptr, 0, c, 0, dweight, dbias, weight_dtype, st) : (int)DC_OK;
-    if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr || (sums && workspace == nullptr)) return DC_ERR_NULL_POINTER;
+    if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr) return DC_ERR_NULL_POINTER;
     if (dx == nullptr && !sums) return DC_OK;
-    if (sums && (reinterpret_cast<uintptr_t>(workspace) & 3u) != 0) return DC_ERR_ALIGNMENT;
-    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({dy, x, dx}, weight, nullptr), kBwdWarpPacks);
-    const int64_t ctas = ln_backward_ctas(s, rows);
-    if (sums && workspace_bytes < (size_t)(ctas * 2 * c) * sizeof(float)) return DC_ERR_WORKSPACE;
-    LnBwdParams p{dy, x, weight, mean, rstd, dx, sums ? (float*)workspace : nullptr, rows, c, c / s.w, s.g, 1.f / (float)c};
-    const int rc = [&]() -> int { DC_LN_TYPES(ln_backward_t, s, p, ctas, st) }();
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({dy, x, dx}, weight, nullptr), kBwdWarpPacks, bwd_cta_packs(ln_elem(dtype)));
+    const LnSplit t = ln_split(s, c, rows);
+    const size_t means = ln_means_floats(s, rows);
+    if (sums || means > 0) {
+        if (workspace == nullptr) return DC_ERR_NULL_POINTER;
+        if ((reinterpret_cast<uintptr_t>(workspace) & 15u) != 0) return DC_ERR_ALIGNMENT;
+        if (workspace_bytes < (means + (sums ? (size_t)t.slices * 2 * c : 0)) * sizeof(float)) return DC_ERR_WORKSPACE;
+    }
+    // the column sums first: their packs want the workspace's alignment
+    float* partial = sums ? (float*)workspace : nullptr;
+    LnBwdParams p{dy, x, weight, mean, rstd, dx, partial, (float*)workspace + (sums ? t.slices * 2 * c : 0), rows, t.per, c, c / s.w, s.g, 1.f / (float)c};
+    const int rc = [&]() -> int { DC_LN_TYPES(ln_backward_t, s, p, t, st) }();
     if (rc != DC_OK || !sums) return rc;
-    return col_reduce((const float*)workspace, (int)ctas, c, 2 * (int64_t)c, dweight, dbias, weight_dtype, st);
+    return col_reduce(partial, (int)t.slices, c, 2 * (int64_t)c, dweight, dbias, weight_dtype, st);
 }
 
 int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, void* prev_out, const void* weight, const void* bias,
@@ -1042,7 +1231,7 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
     if (npix < 0 || c <= 0) return DC_ERR_SHAPE;
     if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;      // the caches are those of the delta path
     if (npix == 0) return DC_OK;
-    const LnShape s = ln_shape(c, 0, ln_elem(dtype), ln_access({delta, prev_in, prev_out, out}, weight, bias), kDeltaWarpPacks);
+    const LnShape s = ln_shape(c, 0, ln_elem(dtype), ln_access({delta, prev_in, prev_out, out}, weight, bias), kDeltaWarpPacks, 4);
     if (s.p == 0) return DC_ERR_UNSUPPORTED;      // more channels than the registers of a CTA hold
     const float thr = dtype == DC_F16 ? host_round_threshold<__half>(threshold) : threshold;
     LnDeltaParams p{delta, weight, bias, mask, prev_in, prev_out, out, mask_out, npix, c, c / s.w, s.g, thr, eps, 1.f / (float)c, 32};

@@ -336,8 +336,9 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
 /* Gradients of dc_layer_norm: with g = dy * weight and n = (x - mean) * rstd,
  *   dx = rstd * (g - mean(g) - n * mean(g * n)),  dweight = sum_rows(dy * n),  dbias = sum_rows(dy).
  * dx, dweight, dbias may be NULL where not wanted. dx may be dy. workspace: dc_layer_norm_backward_workspace_bytes of device
- * memory, only meaningful during the call (per-CTA partial sums of the column reductions, added in a fixed order: the same
- * inputs give the same bits). rows == 0 writes zeros to dweight and dbias. */
+ * memory, 16-byte aligned, only meaningful during the call (per-CTA partial sums of the column reductions, added in a fixed
+ * order: the same inputs give the same bits; the means of long rows). May be NULL where only dx is wanted of rows of at most
+ * 8192 elements. rows == 0 writes zeros to dweight and dbias. */
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype);
 int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
                            void* dweight, void* dbias, int64_t rows, int32_t c, int32_t dtype, int32_t weight_dtype, void* workspace,

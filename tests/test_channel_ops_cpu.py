@@ -52,6 +52,9 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.dc_layer_norm_backward(p, p, p, p, p, p, p, p, 1, 8, f32, f32, None, 0, None) == null
     assert lib.dc_layer_norm_backward(p, p, p, p, p, p, p, p, 1, 8, f32, f32, p, 8, None) == space
     assert lib.dc_layer_norm_backward(p, p, p, None, p, p, p, p, 1, 8, f32, f32, p, 1 << 20, None) == null
+    assert lib.dc_layer_norm_backward(p, p, p, p, p, p, p, p, 1, 8, f32, f32, 20, 1 << 20, None) == align
+    assert lib.dc_layer_norm_backward(p, p, p, p, p, p, None, None, 1, 9001, f32, f32, None, 0, None) == null
+    assert lib.dc_layer_norm_backward(p, p, p, p, p, p, None, None, 1, 9001, f32, f32, p, 7, None) == space
     assert lib.dc_layer_norm_backward_workspace_bytes(0, 8, f32) == 0
     assert lib.dc_layer_norm_delta(p, None, p, p, p, p, p, p, 1, 8, f32, f32, 0.0, 1e-5, None) == null
     assert lib.dc_layer_norm_delta(p, p, p, p, p, p, p, p, 1, 8, bf16, bf16, 0.0, 1e-5, None) == dtype

@@ -61,7 +61,7 @@ def y_bound(w, b, n, a, y, t):
 
 SHAPES = [(1, 1), (5, 1), (1, 8), (3, 7), (40, 24), (5, 33), (259, 64), (2, 96), (130, 100), (33, 1000), (7, 1024), (3, 1032), (6, 1001),
           (2, 4096), (3, 4100), (2, 4099), (2, 8192), (3, 16384), (2, 20000), (1, 40000), (1500, 8), (700, 257),
-          (2, 9001), (3, 2500), (2, 10000), (300, 50), (90, 82), (41, 170), (77, 430), (5, 514), (3, 8190), (2, 8194), (9, 2), (80001, 96), (160001, 24), (30000, 512)]
+          (2, 9001), (3, 2500), (2, 10000), (300, 50), (90, 82), (41, 170), (77, 430), (5, 514), (3, 8190), (2, 8194), (9, 2), (1, 8193), (17, 12001), (1000, 9006), (450, 8200), (100, 10240), (5, 16392), (3, 60001), (2, 120000), (80001, 96), (160001, 24), (30000, 512)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -125,6 +125,23 @@ def test_layer_norm_with_float32_weights(dtype):
     d = dy.double()
     within(dw, (d * n).sum(0), 140 * U * (d.abs() * (n.abs() + (1 + n.abs()) * a)).sum(0))
     within(db, d.sum(0), 140 * U * d.abs().sum(0))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("rows,c", [(5, 1000), (70, 9001), (70, 9002), (33, 20000)])
+def test_layer_norm_gradients_alone_are_those_together(rows, c, dtype):
+    g = gen(c)
+    x, dy = randn((rows, c), g, dtype), randn((rows, c), g, dtype)
+    w, b = randn((c,), g, F32, 0.3, 1.0), randn((c,), g)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    together = torch.autograd.grad(dc().layer_norm(*leaves, EPS), leaves, dy)
+    for i in range(3):
+        parts = [t.detach().requires_grad_(j == i) for j, t in enumerate(leaves)]
+        assert torch.equal(torch.autograd.grad(dc().layer_norm(*parts, EPS), parts[i], dy)[0], together[i])
+    bare = x.detach().requires_grad_()
+    unit = x.detach().requires_grad_()
+    plain = torch.autograd.grad(dc().layer_norm(bare, eps=EPS), bare, dy)[0]
+    assert torch.equal(plain, torch.autograd.grad(dc().layer_norm(unit, torch.ones(c, device="cuda"), eps=EPS), unit, dy)[0])
 
 
 @pytest.mark.parametrize("with_w,with_b", [(False, False), (True, False), (False, True)])
