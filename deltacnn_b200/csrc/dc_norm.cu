@@ -909,7 +909,7 @@ __global__ void __launch_bounds__(256, P == 1 ? 4 : W > 2 ? 1 : 3) k_ln_delta(Ln
         __syncwarp();
         const int n = __popc(m);
         // the next pixel's reads are on their way while one is normalised, where a lane has the registers for both
-        constexpr bool kAhead = P == 1;
+        constexpr bool kAhead = P * W * sizeof(T) <= 16;
         DeltaPixel<T, W, P> v, ahead;
         int at = lane / p.g, px = at < n ? list[warp][at] : 0;
         if (n > 0) v.load(p, t, base + px, at < n);
@@ -939,8 +939,10 @@ __global__ void __launch_bounds__(kLnCta) k_ln_delta_cta(LnDeltaParams p) {
     Frag<WT, W> w[P], b[P];
     load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
     load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
+    int32_t next = t.row < p.npix ? p.mask[t.row] : 0;
     for (int64_t px = t.row; px < p.npix; px += t.stride) {
-        const bool act = p.mask[px] != 0;      // the same word in every thread
+        const bool act = next != 0;            // the same word in every thread
+        next = px + t.stride < p.npix ? p.mask[px + t.stride] : 0;
         bool keep = false;
         if (act) {
             DeltaPixel<T, W, P> v;
@@ -976,8 +978,11 @@ static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int war
         // Rows enough for every SM's threads all the same: fewer lanes with more packs each shuffle less per element (96 channels
         // in fp16, 200000 rows: 16 lanes of one pack 25 us, 4 lanes of three 17.8 us).
         while (wide && s.g > 1 && divup(n, s.g / 2) <= warp_packs && rows * (s.g / 2) >= (int64_t)sm_count() * 1024) s.g /= 2;
+        // Narrow accesses: as few lanes as four of them each allow, for the reads in flight (delta form, 19 channels in fp32, 64 maps of
+        // 130 x 200: 32 lanes of one 125 us, 8 lanes of four 79 us).
+        while (!wide && s.g > 1 && divup(n, s.g / 2) <= 4) s.g /= 2;
         const int need = divup(n, s.g);
-        s.p = wide ? need : need <= 2 ? 2 : 4;
+        s.p = wide ? need : 4;
         s.threads = 256;
         return s;
     }
@@ -1022,7 +1027,7 @@ static int64_t ln_ctas(const LnShape& s, int64_t rows, int per_sm) {
     }
 // Narrow accesses: single elements (W 1) or two halves (W 2).
 #define DC_LN_NARROW_WARP(KERNEL, T, WT, W) \
-    switch (s.p) { DC_LN_CASE(2, KERNEL, T, WT, W, false) DC_LN_CASE(4, KERNEL, T, WT, W, false) default: break; }
+    switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, W, false) default: break; }
 #define DC_LN_SINGLE_CTA(KERNEL, T, WT) \
     switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 1, true) DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
 #define DC_LN_PAIR_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 2, true) DC_LN_CASE(8, KERNEL, T, WT, 2, true) default: break; }
