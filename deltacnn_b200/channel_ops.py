@@ -87,6 +87,8 @@ def _ptr(t):
 def _ln_params(x, c, code, weight, bias, op):
     """The weight's dtype code; weight and bias are (C,) of x's type or float32, of one type."""
     wcode, index = code, x.get_device()
+    if c > 1 << 30:
+        _fail(op, f"{c} channels are more than 2^30")
     if weight is not None:
         wcode = _ln_param(x, c, weight, index, "weight", op)
     if bias is not None:
@@ -170,7 +172,8 @@ def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, thr
     ``prev_in += delta`` and ``e = layer_norm(prev_in) - prev_out``; where any ``|e| > threshold`` the pixel stays in the mask,
     ``out = e`` and ``prev_out += e``; elsewhere the out-mask is 0 and ``out`` and ``prev_out`` keep what they hold.
     ``prev_in``: the accumulated input, ``prev_out``: the sum of what was handed on, both updated in place. ``out`` may be
-    ``delta`` and ``out_mask`` may be ``mask``; new tensors where None. Returns (out, out_mask). No reference counterpart."""
+    ``delta`` and ``out_mask`` may be ``mask``; new tensors where None. At most 8192 channels. Returns (out, out_mask). No
+    reference counterpart."""
     op = "layer_norm_delta"
     _check_feature(delta, "delta")
     if delta.dtype not in (torch.float32, torch.float16):

@@ -1173,6 +1173,7 @@ static int ln_access(std::initializer_list<const void*> arrays, const void* weig
 // Four packs of eight halves are 64 column sums per thread, which its 128 registers do not hold beside the row: the long kernels'
 // two reads are faster (3276 x 10240 in bf16: 87 -> 68 us).
 static int bwd_cta_packs(int elem_bytes) { return elem_bytes == 2 ? 2 : 4; }
+constexpr int kLnMaxC = 1 << 30;          // a row's places are 32-bit
 constexpr int kFwdWarpPacks = 4, kBwdWarpPacks = 2, kDeltaWarpPacks = 4;
 
 }  // namespace dc
@@ -1184,7 +1185,7 @@ extern "C" {
 int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd, int64_t rows, int32_t c,
                   int32_t dtype, int32_t weight_dtype, float eps, void* stream) {
     if (x == nullptr || y == nullptr || (mean == nullptr) != (rstd == nullptr)) return DC_ERR_NULL_POINTER;
-    if (rows < 0 || c <= 0) return DC_ERR_SHAPE;
+    if (rows < 0 || c <= 0 || c > kLnMaxC) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     if (rows == 0) return DC_OK;
     const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({x, y}, weight, bias), kFwdWarpPacks, 4);
@@ -1193,7 +1194,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
 }
 
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype) {
-    if (rows <= 0 || c <= 0 || dtype < DC_F32 || dtype > DC_BF16) return 0;
+    if (rows <= 0 || c <= 0 || c > kLnMaxC || dtype < DC_F32 || dtype > DC_BF16) return 0;
     // the split may differ with the pointers' alignment: room for any
     size_t most = 0;
     for (int access : {16, 4, 1}) {
@@ -1207,7 +1208,7 @@ size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t d
 int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
                            void* dweight, void* dbias, int64_t rows, int32_t c, int32_t dtype, int32_t weight_dtype, void* workspace,
                            size_t workspace_bytes, void* stream) {
-    if (rows < 0 || c <= 0) return DC_ERR_SHAPE;
+    if (rows < 0 || c <= 0 || c > kLnMaxC) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     const bool sums = dweight != nullptr || dbias != nullptr;
     cudaStream_t st = (cudaStream_t)stream;
@@ -1235,7 +1236,7 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
                         float eps, void* stream) {
     if (delta == nullptr || mask == nullptr || prev_in == nullptr || prev_out == nullptr || out == nullptr || mask_out == nullptr)
         return DC_ERR_NULL_POINTER;
-    if (npix < 0 || c <= 0) return DC_ERR_SHAPE;
+    if (npix < 0 || c <= 0 || c > kLnMaxC) return DC_ERR_SHAPE;
     if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;      // the caches are those of the delta path
     if (npix == 0) return DC_OK;
     const LnShape s = ln_shape(c, 0, ln_elem(dtype), ln_access({delta, prev_in, prev_out, out}, weight, bias), kDeltaWarpPacks, 4);

@@ -326,7 +326,7 @@ int dc_centernet_decode(const void* heat, const void* wh, const void* offset, co
  * No counterpart in the reference, whose only norm is DCBatchNorm2d (src/deltacnn/sparse_layers.py:1516-1585).
  * A row is the channel vector of one pixel or token: rows x c contiguous elements. Statistics, sums and products are
  * float32, each stored value is rounded once. dtype: DC_F32, DC_F16 or DC_BF16; weight_dtype: dtype or DC_F32.
- * weight and bias (c elements) may be NULL (1 and 0). */
+ * weight and bias (c elements) may be NULL (1 and 0). c is at most 2^30. */
 
 /* y = (x - mean) * rstd * weight + bias, mean and rstd = 1 / sqrt(variance + eps) over the row (variance with divisor
  * c). mean, rstd: float32 per row for the backward pass, or both NULL. y may be x. */
@@ -347,7 +347,8 @@ int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, co
 /* Layer norm over the channels in delta form (DC_F32, DC_F16). prev_in holds the accumulated input, prev_out the sum of what
  * was handed on so far. On pixels with mask != 0: prev_in += delta; e = layer_norm(prev_in) - prev_out; where any
  * |e| > threshold: out = e, prev_out += e, mask_out = 1. Everywhere else mask_out = 0, and out and prev_out stay as they are
- * (a change below the threshold is not lost: it stays in prev_in). out may be delta, mask_out may be mask. */
+ * (a change below the threshold is not lost: it stays in prev_in). out may be delta, mask_out may be mask. A pixel's channels
+ * stay in registers: more than 8192 are DC_ERR_UNSUPPORTED (DC_F16 in multiples of 8 at 16-byte addresses: than 16384). */
 int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, void* prev_out, const void* weight, const void* bias,
                         void* out, int32_t* mask_out, int64_t npix, int32_t c, int32_t dtype, int32_t weight_dtype, float threshold,
                         float eps, void* stream);

@@ -44,6 +44,7 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.dc_layer_norm(None, p, p, p, None, None, 1, 8, f32, f32, 1e-5, None) == null
     assert lib.dc_layer_norm(p, p, p, p, p, None, 1, 8, f32, f32, 1e-5, None) == null
     assert lib.dc_layer_norm(p, p, p, p, None, None, 1, 0, f32, f32, 1e-5, None) == shape
+    assert lib.dc_layer_norm(p, p, p, p, None, None, 1, (1 << 30) + 1, f32, f32, 1e-5, None) == shape
     assert lib.dc_layer_norm(p, p, p, p, None, None, -1, 8, f32, f32, 1e-5, None) == shape
     assert lib.dc_layer_norm(p, p, p, p, None, None, 1, 8, 3, f32, 1e-5, None) == dtype
     assert lib.dc_layer_norm(p, p, p, p, None, None, 1, 8, f32, f16, 1e-5, None) == dtype
