@@ -130,19 +130,24 @@ __device__ __forceinline__ float lanes_sum(float x, int g) {
 }
 
 // A row's team: g lanes of a warp (BLOCK false) or the whole CTA (BLOCK true).
-template <bool BLOCK> struct Team {
+// Pack k of a thread is first + k hop(): the lanes of a group go round; in a CTA every warp has a stretch of 32 P packs of its own,
+// so that a thread's packs are one address with constant offsets and only the last warps look where the row ends.
+template <bool BLOCK, int P = 1> struct Team {
     int rank, size;            // this thread's place in the team, the team's threads
+    int first;
     int64_t row, stride;       // first row, distance to the next one
     __device__ __forceinline__ Team(int g) {
         if constexpr (BLOCK) {
             rank = threadIdx.x; size = blockDim.x; row = blockIdx.x; stride = gridDim.x;
+            first = (threadIdx.x >> 5) * 32 * P + (threadIdx.x & 31);
         } else {
             const int per_cta = blockDim.x / g;
-            rank = threadIdx.x & (g - 1); size = g;
+            rank = first = threadIdx.x & (g - 1); size = g;
             row = (int64_t)blockIdx.x * per_cta + threadIdx.x / g;
             stride = (int64_t)gridDim.x * per_cta;
         }
     }
+    __device__ __forceinline__ int hop() const { return BLOCK ? 32 : size; }
     // Sum over the team, the same bits in every thread. red: kMaxWarps floats per call site (BLOCK); a site is used again
     // only after another site's barrier.
     __device__ __forceinline__ float sum(float x, float* red) const {
@@ -155,6 +160,17 @@ template <bool BLOCK> struct Team {
     }
 };
 
+// f(k, pack k is inside the row) for a thread's packs. SPLIT: warps that are inside as a whole (`all`) run it without the question.
+template <int P, bool SPLIT, typename F> __device__ __forceinline__ void each_pack(bool all, unsigned valid, F&& f) {
+    if (SPLIT && all) {
+#pragma unroll
+        for (int k = 0; k < P; ++k) f(k, true);
+    } else {
+#pragma unroll
+        for (int k = 0; k < P; ++k) f(k, (valid >> k & 1u) != 0);
+    }
+}
+
 // The rows ahead of the one at hand. 16-byte packs: every thread copies its own packs of the next rows of N arrays into its own
 // slots of a ring in shared memory (cp.async: no registers, no barrier, a wait for the thread's own copies). Three rows, or one
 // where a row alone is 64 KB or more of a CTA's shared memory. Single elements: the next row in registers.
@@ -163,28 +179,30 @@ __device__ __forceinline__ void cp16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src) : "memory");
 }
 // Packs behind the end of a row (rank + k size >= nvec) read as zeros, so that the arithmetic needs no branch for them.
-template <typename T, int W, int P, int N> struct RowPipe {
+template <typename T, int W, int P, int N, bool BLOCK> struct RowPipe {
     static constexpr bool kRing = W * sizeof(T) == 16;
     static constexpr int kAhead = rows_ahead(N * P);
     Frag<T, W> next[kRing ? 1 : N][kRing ? 1 : P];
     uint8_t* mine;
     const T* at[N];                        // this thread's first pack of the next row to ask for
     int64_t step, left;                    // elements between the team's rows; rows it still has to ask for
-    int size, in, out;                     // slots to fill, to read
+    int group, in, out;                    // slots to fill, to read
     unsigned valid;                        // bit k: pack k is inside the row
+    bool all;                              // all packs of the warp are
+    __device__ __forceinline__ int hop() const { return BLOCK ? 32 : group; }
+    template <typename F> __device__ __forceinline__ void each(F&& f) const { each_pack<P, BLOCK && !kRing>(all, valid, f); }
 
     __device__ __forceinline__ void ask() {
         if (left > 0) {
+            each([&](int k, bool inside) {
+                if (!inside) return;
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
+                for (int n = 0; n < N; ++n)
+                    if constexpr (kRing) cp16(mine + (size_t)((in * N + n) * P + k) * blockDim.x * 16, at[n] + k * hop() * W);
+                    else next[n][k].load(at[n] + k * hop() * W);
+            });
 #pragma unroll
-                for (int k = 0; k < P; ++k)
-                    if (valid >> k & 1u) {
-                        if constexpr (kRing) cp16(mine + (size_t)((in * N + n) * P + k) * blockDim.x * 16, at[n] + k * size * W);
-                        else next[n][k].load(at[n] + k * size * W);
-                    }
-                at[n] += step;
-            }
+            for (int n = 0; n < N; ++n) at[n] += step;
         }
         if constexpr (kRing) {
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -192,19 +210,19 @@ template <typename T, int W, int P, int N> struct RowPipe {
         }
         --left;
     }
-    template <bool BLOCK>
-    __device__ __forceinline__ void start(const Team<BLOCK>& t, const void* const (&src)[N], int64_t rows, int c, int nvec, uint8_t* smem) {
+    __device__ __forceinline__ void start(const Team<BLOCK, P>& t, const void* const (&src)[N], int64_t rows, int c, int nvec, uint8_t* smem) {
         mine = smem + threadIdx.x * 16;
-        size = t.size;
+        group = t.size;
         step = t.stride * c;
         left = t.row < rows ? (rows - t.row + t.stride - 1) / t.stride : 0;
         in = out = 0;
         valid = 0;
 #pragma unroll
-        for (int k = 0; k < P; ++k) valid |= t.rank + k * t.size < nvec ? 1u << k : 0u;
+        for (int k = 0; k < P; ++k) valid |= t.first + k * t.hop() < nvec ? 1u << k : 0u;
+        all = __all_sync(DC_FULL, valid == (1u << P) - 1u);
 #pragma unroll
         for (int n = 0; n < N; ++n) {
-            at[n] = (const T*)src[n] + t.row * c + t.rank * W;
+            at[n] = (const T*)src[n] + t.row * c + t.first * W;
 #pragma unroll
             for (int k = 0; k < P; ++k) {
                 if constexpr (kRing) {
@@ -265,17 +283,17 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
     extern __shared__ __align__(16) uint8_t ring[];
     grid_dep_launch();
     grid_dep_wait();
-    const Team<BLOCK> t(p.g);
-    RowPipe<T, W, P, 1> pipe;
+    const Team<BLOCK, P> t(p.g);
+    RowPipe<T, W, P, 1, BLOCK> pipe;
     pipe.start(t, {p.x}, p.rows, p.c, p.nvec, ring);
-    T* y = (T*)p.y + t.row * p.c + t.rank * W;
+    T* y = (T*)p.y + t.row * p.c + t.first * W;
     // weight and bias stay in registers; lanes with three packs and more read them from L1 for every row instead and have the
     // registers for twice the warps (12544 x 576: 12.3 -> 8.9 us)
     constexpr bool kHeld = BLOCK || P < 3 || W <= 2;
     Frag<WT, W> w[kHeld ? P : 1], b[kHeld ? P : 1];
     if constexpr (kHeld) {
-        load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
-        load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
+        load_param<WT, W, P>(w, (const WT*)p.w, t.first, t.hop(), p.nvec, 1.f);
+        load_param<WT, W, P>(b, (const WT*)p.b, t.first, t.hop(), p.nvec, 0.f);
     }
     using V = typename Vals<W>::V;
     constexpr int N = Vals<W>::N;
@@ -293,16 +311,14 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
             for (int i = 0; i < N; ++i) s = add(s, x[k].v[i]);
         }
         const float m = t.sum(s.sum(), red[0]) * p.inv_c;
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
-            const V neg = V::all(pipe.valid >> k & 1u ? -m : 0.f);
+        pipe.each([&](int k, bool inside) {
+            const V neg = V::all(inside ? -m : 0.f);
 #pragma unroll
             for (int i = 0; i < N; ++i) { x[k].v[i] = add(x[k].v[i], neg); q = fma(x[k].v[i], x[k].v[i], q); }
-        }
+        });
         const float r = rsqrtf(t.sum(q.sum(), red[1]) * p.inv_c + p.eps);
         const V rr = V::all(r);
-#pragma unroll
-        for (int k = 0; k < P; ++k) {
+        pipe.each([&](int k, bool inside) {
             Vals<W> ww, bb;
             if constexpr (kHeld) {
                 ww.from(w[k]);
@@ -311,17 +327,17 @@ __global__ void __launch_bounds__(BLOCK ? row_threads(W, P) : 256) k_ln_fwd(LnPa
                 Frag<WT, W> f[2];
                 f[0].fill(1.f);
                 f[1].fill(0.f);
-                const int col = (t.rank + k * t.size) * W;
-                if (p.w != nullptr && (pipe.valid >> k & 1u)) f[0].load((const WT*)p.w + col);
-                if (p.b != nullptr && (pipe.valid >> k & 1u)) f[1].load((const WT*)p.b + col);
+                const int col = (t.first + k * t.hop()) * W;
+                if (p.w != nullptr && inside) f[0].load((const WT*)p.w + col);
+                if (p.b != nullptr && inside) f[1].load((const WT*)p.b + col);
                 ww.from(f[0]);
                 bb.from(f[1]);
             }
 #pragma unroll
             for (int i = 0; i < N; ++i) x[k].v[i] = fma(mul(x[k].v[i], rr), ww.v[i], bb.v[i]);
             x[k].to(in[0][k]);
-            if (on && (pipe.valid >> k & 1u)) in[0][k].store(y + k * t.size * W);
-        }
+            if (on && inside) in[0][k].store(y + k * t.hop() * W);
+        });
         if (on && t.rank == 0 && p.mean != nullptr) { p.mean[row] = m; p.rstd[row] = r; }
     }
 }
@@ -451,12 +467,12 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
     extern __shared__ __align__(16) uint8_t ring[];      // the rows ahead; at the end [2][c] column sums of the CTA's teams
     grid_dep_launch();
     grid_dep_wait();
-    const Team<BLOCK> t(p.g);
-    RowPipe<T, W, P, 2> pipe;
+    const Team<BLOCK, P> t(p.g);
+    RowPipe<T, W, P, 2, BLOCK> pipe;
     pipe.start(t, {p.x, p.dy}, p.rows, p.c, p.nvec, ring);
-    T* dx = (T*)p.dx + t.row * p.c + t.rank * W;
+    T* dx = (T*)p.dx + t.row * p.c + t.first * W;
     Frag<WT, W> w[P];
-    load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
+    load_param<WT, W, P>(w, (const WT*)p.w, t.first, t.hop(), p.nvec, 1.f);
     using V = typename Vals<W>::V;
     constexpr int N = Vals<W>::N;
     Vals<W> dw[P], db[P];
@@ -478,20 +494,19 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
         Vals<W> n[kKeep ? P : 1], g[kKeep ? P : 1];
         V sg = V::all(0.f), sgn = V::all(0.f);
         const V rr = V::all(r);
-        auto form = [&](int k, Vals<W>& nn, Vals<W>& ee, Vals<W>& gg) {
+        auto form = [&](int k, bool inside, Vals<W>& nn, Vals<W>& ee, Vals<W>& gg) {
             Vals<W> ww;
             nn.from(in[0][k]);
             ee.from(in[1][k]);
             ww.from(w[k]);
-            const V shift = V::all(pipe.valid >> k & 1u ? -m : 0.f);
+            const V shift = V::all(inside ? -m : 0.f);
 #pragma unroll
             for (int i = 0; i < N; ++i) { nn.v[i] = mul(add(nn.v[i], shift), rr); gg.v[i] = mul(ee.v[i], ww.v[i]); }
         };
-        if (on) {
-#pragma unroll
-            for (int k = 0; k < P; ++k) {
+        if (on)
+            pipe.each([&](int k, bool inside) {
                 Vals<W> nn, ee, gg;
-                form(k, nn, ee, gg);
+                form(k, inside, nn, ee, gg);
 #pragma unroll
                 for (int i = 0; i < N; ++i) {
                     dw[k].v[i] = fma(ee.v[i], nn.v[i], dw[k].v[i]);
@@ -500,8 +515,7 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
                     sgn = fma(gg.v[i], nn.v[i], sgn);
                 }
                 if constexpr (kKeep) { n[k] = nn; g[k] = gg; }
-            }
-        }
+            });
         if (p.dx != nullptr) {
             float a, c;
             if constexpr (BLOCK) {             // both sums behind one barrier
@@ -519,16 +533,15 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
                 c = lanes_sum(sgn.sum(), t.size) * p.inv_c;
             }
             const V na = V::all(-a), nc = V::all(-c);
-#pragma unroll
-            for (int k = 0; k < P; ++k) {
+            pipe.each([&](int k, bool inside) {
                 Vals<W> nn, ee, gg;
                 if constexpr (kKeep) { nn = n[k]; gg = g[k]; }
-                else form(k, nn, ee, gg);
+                else form(k, inside, nn, ee, gg);
 #pragma unroll
                 for (int i = 0; i < N; ++i) gg.v[i] = mul(rr, fma(nn.v[i], nc, add(gg.v[i], na)));
                 gg.to(in[0][k]);
-                if (on && (pipe.valid >> k & 1u)) in[0][k].store(dx + k * t.size * W);
-            }
+                if (on && inside) in[0][k].store(dx + k * t.hop() * W);
+            });
         }
     }
     if (p.partial == nullptr) return;
@@ -536,8 +549,8 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
     if constexpr (BLOCK) {
 #pragma unroll
         for (int k = 0; k < P; ++k)
-            if (t.rank + k * t.size < p.nvec) {
-                const int col = (t.rank + k * t.size) * W;
+            if (t.first + k * t.hop() < p.nvec) {
+                const int col = (t.first + k * t.hop()) * W;
                 Frag<float, W> f;
                 dw[k].put(f.s);
                 f.store(out + col);
@@ -565,10 +578,10 @@ __global__ void __launch_bounds__(row_threads(W, P), bwd_ctas(W, P)) k_ln_bwd(Ln
             if (warp == q && (threadIdx.x & 31) < p.g) {
 #pragma unroll
                 for (int k = 0; k < P; ++k)
-                    if (t.rank + k * t.size < p.nvec)
+                    if (t.first + k * t.hop() < p.nvec)
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
-                            const int col = (t.rank + k * t.size) * W + i;
+                            const int col = (t.first + k * t.hop()) * W + i;
                             cols[col] = (q == 0 ? 0.f : cols[col]) + sums[0][k][i];
                             cols[p.c + col] = (q == 0 ? 0.f : cols[p.c + col]) + sums[1][k][i];
                         }
@@ -811,13 +824,13 @@ template <typename T, int W> __device__ __forceinline__ bool frag_any_above(cons
 // What a team reads of a pixel; packs behind the last channel hold zeros.
 template <typename T, int W, int P> struct DeltaPixel {
     Frag<T, W> d[P], u[P], o[P];           // the delta, the accumulated input, the accumulated output
-    template <bool BLOCK> __device__ __forceinline__ void load(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on) {
-        const int64_t off = px * p.c + t.rank * W;
+    template <bool BLOCK> __device__ __forceinline__ void load(const LnDeltaParams& p, const Team<BLOCK, P>& t, int64_t px, bool on) {
+        const int64_t off = px * p.c + t.first * W;
 #pragma unroll
         for (int k = 0; k < P; ++k) {
             d[k].fill(0.f); u[k].fill(0.f); o[k].fill(0.f);
-            if (on && t.rank + k * t.size < p.nvec) {
-                const int64_t at = off + k * t.size * W;
+            if (on && t.first + k * t.hop() < p.nvec) {
+                const int64_t at = off + k * t.hop() * W;
                 d[k].load((const T*)p.delta + at);
                 u[k].load((const T*)p.prev_in + at);
                 o[k].load((const T*)p.prev_out + at);
@@ -827,15 +840,15 @@ template <typename T, int W, int P> struct DeltaPixel {
 };
 // One pixel by its team; returns whether any channel's change is above the threshold (the same answer in the whole team).
 template <typename T, typename WT, int W, int P, bool BLOCK>
-__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK>& t, int64_t px, bool on, DeltaPixel<T, W, P>& v, Frag<WT, W> (&w)[P],
+__device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Team<BLOCK, P>& t, int64_t px, bool on, DeltaPixel<T, W, P>& v, Frag<WT, W> (&w)[P],
                                                Frag<WT, W> (&b)[P], float* red0, float* red1) {
-    const int64_t off = px * p.c + t.rank * W;
+    const int64_t off = px * p.c + t.first * W;
     Frag<T, W> (&d)[P] = v.d;
     Frag<T, W> (&u)[P] = v.u;
     Frag<T, W> (&o)[P] = v.o;
     bool valid[P];
 #pragma unroll
-    for (int k = 0; k < P; ++k) valid[k] = t.rank + k * t.size < p.nvec;
+    for (int k = 0; k < P; ++k) valid[k] = t.first + k * t.hop() < p.nvec;
     using V = typename Vals<W>::V;
     constexpr int N = Vals<W>::N;
     Vals<W> x[P];
@@ -843,7 +856,7 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
 #pragma unroll
     for (int k = 0; k < P; ++k) {
         frag_add(u[k], d[k]);
-        if (on && valid[k]) u[k].store((T*)p.prev_in + off + k * t.size * W);
+        if (on && valid[k]) u[k].store((T*)p.prev_in + off + k * t.hop() * W);
         x[k].from(u[k]);
 #pragma unroll
         for (int i = 0; i < N; ++i) s = add(s, x[k].v[i]);
@@ -877,8 +890,8 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
         for (int k = 0; k < P; ++k)
             if (valid[k]) {
                 frag_add(o[k], d[k]);
-                d[k].store((T*)p.out + off + k * t.size * W);
-                o[k].store((T*)p.prev_out + off + k * t.size * W);
+                d[k].store((T*)p.out + off + k * t.hop() * W);
+                o[k].store((T*)p.prev_out + off + k * t.hop() * W);
             }
     }
     return keep;
@@ -891,15 +904,15 @@ __global__ void __launch_bounds__(256, P == 1 ? 4 : W > 2 ? 1 : 3) k_ln_delta(Ln
     __shared__ uint8_t list[8][32], kept[8][32];
     grid_dep_launch();
     grid_dep_wait();
-    Team<false> t(p.g);
+    const Team<false, P> t(p.g);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, teams = 32 / p.g;
     const int64_t step = (int64_t)gridDim.x * 8 * p.chunk;
     int64_t base = ((int64_t)blockIdx.x * 8 + warp) * p.chunk;
     const bool mine = lane < p.chunk;
     int32_t next = mine && base + lane < p.npix ? p.mask[base + lane] : 0;
     Frag<WT, W> w[P], b[P];
-    load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
-    load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
+    load_param<WT, W, P>(w, (const WT*)p.w, t.first, t.hop(), p.nvec, 1.f);
+    load_param<WT, W, P>(b, (const WT*)p.b, t.first, t.hop(), p.nvec, 0.f);
     for (; base < p.npix; base += step) {
         const bool act = next != 0;
         next = mine && base + step + lane < p.npix ? p.mask[base + step + lane] : 0;
@@ -935,10 +948,10 @@ __global__ void __launch_bounds__(kLnCta) k_ln_delta_cta(LnDeltaParams p) {
     __shared__ float red[2][kMaxWarps];
     grid_dep_launch();
     grid_dep_wait();
-    const Team<true> t(0);
+    const Team<true, P> t(0);
     Frag<WT, W> w[P], b[P];
-    load_param<WT, W, P>(w, (const WT*)p.w, t.rank, t.size, p.nvec, 1.f);
-    load_param<WT, W, P>(b, (const WT*)p.b, t.rank, t.size, p.nvec, 0.f);
+    load_param<WT, W, P>(w, (const WT*)p.w, t.first, t.hop(), p.nvec, 1.f);
+    load_param<WT, W, P>(b, (const WT*)p.b, t.first, t.hop(), p.nvec, 0.f);
     int32_t next = t.row < p.npix ? p.mask[t.row] : 0;
     for (int64_t px = t.row; px < p.npix; px += t.stride) {
         const bool act = next != 0;            // the same word in every thread
