@@ -16,8 +16,9 @@
 // Bound: memory, once the arithmetic is packed (two float32 per instruction): 16384 x 4096 bf16 forward 45 us (268 MB, 41 us at
 // the copy rate), backward 72 us (403 MB, 61 us); with scalar arithmetic and a branch per pack the issue slots were the bound
 // (58 and 99 us). 12544 x 576 fp16 forward 9 us (29 MB, 4.4 us: launch and two round trips). Delta form, fp16: 64 channels
-// 136 x 240 x 32, a tenth active, 25 us (83 MB, 12.7 us: sparse pixels leave teams idle); 96 channels 56 x 56 x 64, all active, 49 us
-// (231 MB, 35 us).
+// 136 x 240 x 32, a tenth active, 25 us (83 MB, 12.7 us: sparse pixels leave teams idle); 96 channels 56 x 56 x 64, all active, 43 us
+// (231 MB, 35 us). Without 16-byte accesses the issue slots and the reads in flight bound it: 11181 x 3001 bf16 forward 46 us, backward
+// 71 us (20 and 31 at the copy rate), 6211 x 5402 28 and 79 us, fp32 11181 x 3001 49 and 87 us (41 and 61).
 #include <initializer_list>
 #include <type_traits>
 #include "dc_common.cuh"
@@ -977,8 +978,9 @@ struct LnShape {
 
 // warp_packs: most packs per lane of a row that a group of lanes takes (more registers per lane than a CTA's threads need, but
 // no barriers). cta_packs: most 16-byte packs per thread of a CTA.
+// narrow_packs: as warp_packs, for narrow accesses, where the rows fill every SM's threads.
 // access: bytes that the arrays' addresses allow, 16, 4 or less.
-static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int warp_packs, int cta_packs) {
+static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int warp_packs, int cta_packs, int narrow_packs = 4) {
     LnShape s{};
     const int vec = 16 / elem_bytes;
     // 16-byte packs; two halves where a row's width or place allows no more (half the instructions of single ones); elements
@@ -986,16 +988,17 @@ static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int war
     const int n = c / s.w;
     // narrow accesses: at least four per thread, so that a thread has several reads in flight
     const bool wide = s.w == vec;
-    if (n <= 32 * (wide ? warp_packs : 4)) {
+    if (n <= 32 * (wide ? warp_packs : rows * 32 >= (int64_t)sm_count() * 1024 ? narrow_packs : 4)) {
         s.g = lanes_per_pixel(n);
         // Rows enough for every SM's threads all the same: fewer lanes with more packs each shuffle less per element (96 channels
         // in fp16, 200000 rows: 16 lanes of one pack 25 us, 4 lanes of three 17.8 us).
         while (wide && s.g > 1 && divup(n, s.g / 2) <= warp_packs && rows * (s.g / 2) >= (int64_t)sm_count() * 1024) s.g /= 2;
         // Narrow accesses: as few lanes as four of them each allow, for the reads in flight (delta form, 19 channels in fp32, 64 maps of
-        // 130 x 200: 32 lanes of one 125 us, 8 lanes of four 79 us).
-        while (!wide && s.g > 1 && divup(n, s.g / 2) <= 4) s.g /= 2;
+        // 130 x 200: 32 lanes of one 125 us, 8 lanes of four 79 us); the forward pass of many rows takes up to eight (332222 x 101 in
+        // bf16 74 -> 56 us, 166111 x 202 42 -> 35; sixteen are no faster, and eight are too many beside the backward's sums).
+        while (!wide && s.g > 1 && (divup(n, s.g / 2) <= 4 || (divup(n, s.g / 2) <= narrow_packs && rows * (s.g / 2) >= (int64_t)sm_count() * 1024))) s.g /= 2;
         const int need = divup(n, s.g);
-        s.p = wide ? need : 4;
+        s.p = wide ? need : need <= 4 ? 4 : 8;
         s.threads = 256;
         return s;
     }
@@ -1039,16 +1042,17 @@ static int64_t ln_ctas(const LnShape& s, int64_t rows, int per_sm) {
         DC_LN_CASE(3, KERNEL, T, WT, W, BLOCK) DC_LN_CASE(4, KERNEL, T, WT, W, BLOCK) default: break;          \
     }
 // Narrow accesses: single elements (W 1) or two halves (W 2).
-#define DC_LN_NARROW_WARP(KERNEL, T, WT, W) \
-    switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, W, false) default: break; }
+#define DC_LN_NARROW4(KERNEL, T, WT, W) switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, W, false) default: break; }
+#define DC_LN_NARROW48(KERNEL, T, WT, W) \
+    switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, W, false) DC_LN_CASE(8, KERNEL, T, WT, W, false) default: break; }
 #define DC_LN_SINGLE_CTA(KERNEL, T, WT) \
     switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 1, true) DC_LN_CASE(8, KERNEL, T, WT, 1, true) DC_LN_CASE(16, KERNEL, T, WT, 1, true) default: break; }
 #define DC_LN_PAIR_CTA(KERNEL, T, WT) switch (s.p) { DC_LN_CASE(4, KERNEL, T, WT, 2, true) DC_LN_CASE(8, KERNEL, T, WT, 2, true) default: break; }
 // The kernel of teams of lanes and the one of a CTA per row, for every access.
-#define DC_LN_ALL(WARP_KERNEL, WARP_PACKS, CTA_KERNEL, CTA_PACKS, T, WT)                                                                       \
-    if (s.w == V) { if (s.g > 0) { WARP_PACKS(WARP_KERNEL, T, WT, V, false) } else { CTA_PACKS(CTA_KERNEL, T, WT, V, true) } }    \
-    else if (s.w == 1) { if (s.g > 0) { DC_LN_NARROW_WARP(WARP_KERNEL, T, WT, 1) } else { DC_LN_SINGLE_CTA(CTA_KERNEL, T, WT) } }    \
-    else if constexpr (sizeof(T) == 2) { if (s.g > 0) { DC_LN_NARROW_WARP(WARP_KERNEL, T, WT, 2) } else { DC_LN_PAIR_CTA(CTA_KERNEL, T, WT) } }
+#define DC_LN_ALL(WARP_KERNEL, WARP_PACKS, NARROW, CTA_KERNEL, CTA_PACKS, T, WT)                                                  \
+    if (s.w == V) { if (s.g > 0) { WARP_PACKS(WARP_KERNEL, T, WT, V, false) } else { CTA_PACKS(CTA_KERNEL, T, WT, V, true) } }                   \
+    else if (s.w == 1) { if (s.g > 0) { NARROW(WARP_KERNEL, T, WT, 1) } else { DC_LN_SINGLE_CTA(CTA_KERNEL, T, WT) } }              \
+    else if constexpr (sizeof(T) == 2) { if (s.g > 0) { NARROW(WARP_KERNEL, T, WT, 2) } else { DC_LN_PAIR_CTA(CTA_KERNEL, T, WT) } }
 
 #define DC_LN_TAIL(BLOCK) , BLOCK
 template <auto KERNEL>
@@ -1079,7 +1083,7 @@ static int ln_forward_t(const LnShape& s, LnParams& p, cudaStream_t st) {
         if constexpr (sizeof(T) == 2) if (s.w == 2) return ln_forward_long<T, WT, 2>(p, st);
         return ln_forward_long<T, WT, 1>(p, st);
     }
-    DC_LN_ALL(k_ln_fwd, DC_LN_PACKS1234, k_ln_fwd, DC_LN_PACKS4, T, WT)
+    DC_LN_ALL(k_ln_fwd, DC_LN_PACKS1234, DC_LN_NARROW48, k_ln_fwd, DC_LN_PACKS4, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
@@ -1132,8 +1136,8 @@ static int ln_backward_t(const LnShape& s, LnBwdParams& p, const LnSplit& t, cud
         if constexpr (sizeof(T) == 2) if (s.w == 2) return ln_backward_long<T, WT, 2>(p, t, st);
         return ln_backward_long<T, WT, 1>(p, t, st);
     }
-    if constexpr (sizeof(T) == 4) { DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, k_ln_bwd, DC_LN_PACKS4, T, WT) }
-    else { DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, k_ln_bwd, DC_LN_PACKS2, T, WT) }
+    if constexpr (sizeof(T) == 4) { DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, DC_LN_NARROW4, k_ln_bwd, DC_LN_PACKS4, T, WT) }
+    else { DC_LN_ALL(k_ln_bwd, DC_LN_PACKS2, DC_LN_NARROW4, k_ln_bwd, DC_LN_PACKS2, T, WT) }
 #undef DC_LN_RUN
     return rc;
 }
@@ -1156,7 +1160,7 @@ static int ln_delta_t(const LnShape& s, LnDeltaParams& p, cudaStream_t st) {
     constexpr int V = 16 / (int)sizeof(T);
     int rc = DC_ERR_UNSUPPORTED;
 #define DC_LN_RUN(K) rc = ln_delta_run<K>(s, p, st)
-    DC_LN_ALL(k_ln_delta, DC_LN_PACKS1234, k_ln_delta_cta, DC_LN_PACKS4, T, WT)
+    DC_LN_ALL(k_ln_delta, DC_LN_PACKS1234, DC_LN_NARROW4, k_ln_delta_cta, DC_LN_PACKS4, T, WT)
 #undef DC_LN_RUN
     return rc;
 }
@@ -1201,7 +1205,7 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
     if (rows < 0 || c <= 0 || c > kLnMaxC) return DC_ERR_SHAPE;
     if (!ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
     if (rows == 0) return DC_OK;
-    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({x, y}, weight, bias), kFwdWarpPacks, 4);
+    const LnShape s = ln_shape(c, rows, ln_elem(dtype), ln_access({x, y}, weight, bias), kFwdWarpPacks, 4, 8);
     LnParams p{x, weight, bias, y, mean, rstd, rows, c, c / s.w, s.g, eps, 1.f / (float)c};
     DC_LN_TYPES(ln_forward_t, s, p, (cudaStream_t)stream)
 }

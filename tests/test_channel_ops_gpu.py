@@ -61,7 +61,7 @@ def y_bound(w, b, n, a, y, t):
 
 SHAPES = [(1, 1), (5, 1), (1, 8), (3, 7), (40, 24), (5, 33), (259, 64), (2, 96), (130, 100), (33, 1000), (7, 1024), (3, 1032), (6, 1001),
           (2, 4096), (3, 4100), (2, 4099), (2, 8192), (3, 16384), (2, 20000), (1, 40000), (1500, 8), (700, 257),
-          (2, 9001), (3, 2500), (2, 10000), (300, 50), (90, 82), (41, 170), (77, 430), (5, 514), (3, 8190), (2, 8194), (9, 2), (1, 8193), (17, 12001), (1000, 9006), (450, 8200), (100, 10240), (5, 16392), (3, 60001), (2, 120000), (80001, 96), (160001, 24), (30000, 512)]
+          (2, 9001), (3, 2500), (2, 10000), (300, 50), (90, 82), (41, 170), (77, 430), (5, 514), (3, 8190), (2, 8194), (9, 2), (1, 8193), (17, 12001), (1000, 9006), (450, 8200), (100, 10240), (5, 16392), (3, 60001), (2, 120000), (80001, 96), (160001, 24), (30000, 512), (20000, 101), (19001, 33), (5000, 202), (5001, 255), (20000, 25), (4800, 129)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
