@@ -164,4 +164,7 @@ template <typename T> inline int row_access(const void* x, int64_t cols) {
     return (a & 15u) == 0 ? 16 : (a & 3u) == 0 ? 4 : (int)sizeof(T);
 }
 
+int mx4_quantize_two(const void* x, void* data, void* scales, void* data_t, void* scales_t, int64_t rows, const void* x2, void* data2, void* scales2,
+                     void* data_t2, void* scales_t2, int64_t rows2, int64_t cols, int dtype, cudaStream_t st);
+
 }  // namespace dc

@@ -764,9 +764,14 @@ int dc_mx4_linear_train(const void* x, const void* w, const void* bias, void* ou
     if (!aligned16(workspace) || !aligned16(xt) || !aligned16(wt)) return DC_ERR_ALIGNMENT;
     if (workspace_bytes < dc_mx4_linear_train_workspace_bytes(m, n, k)) return DC_ERR_WORKSPACE;
     uint8_t *xq = (uint8_t*)workspace, *wq = xq + mx4_bytes(m, k);
-    int rc = dc_mx4_quantize(x, xq, mx4_scales_of(xq, m, k), xt, mx4_scales_of(xt, k, m), nullptr, m, k, dtype, 0, nullptr, 0, stream);
-    if (rc != DC_OK) return rc;
-    rc = dc_mx4_quantize(w, wq, mx4_scales_of(wq, n, k), wt, mx4_scales_of(wt, k, n), nullptr, n, k, w_dtype, 0, nullptr, 0, stream);
+    int rc;
+    if (xt != nullptr && wt != nullptr && dtype == w_dtype) {
+        rc = mx4_quantize_two(x, xq, mx4_scales_of(xq, m, k), xt, mx4_scales_of(xt, k, m), m, w, wq, mx4_scales_of(wq, n, k), wt, mx4_scales_of(wt, k, n), n, k,
+                              dtype, (cudaStream_t)stream);
+    } else {
+        rc = dc_mx4_quantize(x, xq, mx4_scales_of(xq, m, k), xt, mx4_scales_of(xt, k, m), nullptr, m, k, dtype, 0, nullptr, 0, stream);
+        if (rc == DC_OK) rc = dc_mx4_quantize(w, wq, mx4_scales_of(wq, n, k), wt, mx4_scales_of(wt, k, n), nullptr, n, k, w_dtype, 0, nullptr, 0, stream);
+    }
     if (rc != DC_OK) return rc;
     return mx4_product(nullptr, xq, mx4_scales_of(xq, m, k), wq, mx4_scales_of(wq, n, k), bias, out, m, n, k, bias_dtype, dtype, (cudaStream_t)stream);
 }

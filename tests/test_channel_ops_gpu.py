@@ -507,6 +507,28 @@ def test_linear_gradient_against_differences():
 
 # ---- as they are used ------------------------------------------------------------------------------------------
 
+@pytest.mark.parametrize("dtype,wtype", [(BF16, BF16), (F32, F32), (F16, F32), (BF16, F16)])
+@pytest.mark.parametrize("x_off,w_off", [(1, 0), (0, 1), (2, 0), (0, 2), (1, 2)])
+def test_linear_training_at_other_addresses(x_off, w_off, dtype, wtype):
+    m, n, k = 150, 136, 264
+    g = gen(x_off * 7 + w_off)
+    x, w, dy = randn((m, k), g, dtype), randn((n, k), g, wtype), randn((m, n), g, dtype)
+
+    def moved(t, off):
+        room = torch.zeros(t.numel() + 8, device="cuda", dtype=t.dtype)
+        at = room[off:off + t.numel()].view(t.shape)
+        at.copy_(t)
+        return at.requires_grad_()
+
+    y = []
+    for a, b in ((moved(x, 0), moved(w, 0)), (moved(x, x_off), moved(w, w_off))):
+        out = dc().mx4_linear(a, b)
+        y.append((out.detach(), *torch.autograd.grad(out, (a, b), dy)))
+    assert all(torch.equal(p, q) for p, q in zip(*y))
+    packed = dc().mx4_matmul(dc().mx4_quantize(x), dc().mx4_quantize(w), None, dtype)
+    assert torch.equal(y[0][0], packed)
+
+
 def test_block_of_norm_and_linears_trains_and_serves():
     """norm -> 4-bit linear -> GELU -> 4-bit linear -> residual, forward and backward, then served with packed weights, also from a
     captured graph."""
