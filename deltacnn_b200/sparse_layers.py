@@ -963,25 +963,48 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
 
 class DCMX4Linear(nn.Linear, DCModule):
     """Fully connected (or pointwise) layer on dense features in MXFP4: activations and weight are rounded to 4 bits with a
-    scale per 32 values and multiplied on the block-scaled tensor core path. ``process_filters()`` packs the weight once for
-    inference; before it the weight is packed in every call and the layer has gradients (three 4-bit products, the
-    rounding's own gradient taken as 1). Takes (..., in_features), or (N, C, H, W) channels-last maps. A (delta, mask) pair is refused: rounding
+    scale per 32 values and multiplied on the block-scaled tensor core path. ``process_filters()`` packs the weight once, for
+    calls that want no gradient. Every other call packs the weight it has: where the input, the weight or the bias wants a gradient
+    (three 4-bit products, the rounding's own gradient taken as 1), and where the weight is no longer the packed one (written in place,
+    replaced, converted or moved; call ``process_filters()`` again. Writes through ``.data`` and to inference tensors leave no
+    trace and are not noticed). Takes (..., in_features), or (N, C, H, W) channels-last maps. A (delta, mask) pair is refused: rounding
     errors of deltas would add up over the frames (put it behind ``DCDensify``). No reference counterpart."""
 
     def __init__(self, in_features, out_features, bias=True):
         nn.Linear.__init__(self, in_features, out_features, bias)
         self.weight_mx4 = None
+        self._packed_from = None
+
+    def _weight_state(self):
+        """The weight's memory (held, so that no other tensor can take its place) and its version."""
+        w = self.weight
+        return w.detach(), None if w.is_inference() else w._version
+
+    def _is_packed(self):
+        if self._packed_from is None:
+            return False
+        (held, version), w = self._packed_from, self.weight
+        return held.dtype == w.dtype and held.device == w.device and held.is_set_to(w) and (w.is_inference() or w._version == version)
 
     def process_filters(self):
         """Pack the weight; call again after changing it."""
         self.weight_mx4 = C.mx4_quantize(self.weight.detach().contiguous())
+        self._packed_from = self._weight_state()
+
+    def __getstate__(self):
+        state = self.__dict__.copy()
+        state["_packed_from"] = self._is_packed()          # a copy has memory of its own
+        return state
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._packed_from = self._weight_state() if state.get("_packed_from") else None
 
     def forward(self, input):
         if type(input) == tuple:
             raise RuntimeError("DCMX4Linear takes dense features: put it behind DCDensify")
-        if self.weight_mx4 is None:
-            return C.mx4_linear(input, self.weight, self.bias)
-        return C.mx4_linear(input, self.weight_mx4, None if self.bias is None else self.bias.detach())
+        grad = torch.is_grad_enabled() and (input.requires_grad or self.weight.requires_grad or (self.bias is not None and self.bias.requires_grad))
+        return C.mx4_linear(input, self.weight if grad or not self._is_packed() else self.weight_mx4, self.bias)
 
 
 class DCHeatmapArgmax(DCModule):

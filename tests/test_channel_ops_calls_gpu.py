@@ -1,0 +1,140 @@
+"""Calls of the layer norm and MXFP4 operators that a program makes around them: modules whose weights change, gradients of
+gradients, forward-mode tangents, saved-tensor hooks, skip connections, tensors of other dimensions and of more than 2^31 elements.
+
+Where values are compared, both sides are the same kernels on the same inputs (equal bits), or whole numbers whose sums
+float32 holds exactly, or the tolerance is derived beside the comparison."""
+import copy
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+EPS = 1e-5
+
+
+def dc():
+    import deltacnn_b200
+    return deltacnn_b200
+
+
+def gen(seed=0):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def randn(shape, g, dtype=F32, scale=1.0, shift=0.0):
+    return (torch.randn(shape, generator=g, device="cuda") * scale + shift).to(dtype)
+
+
+# ---- DCMX4Linear and its packed weight -------------------------------------------------------------------------
+
+@pytest.fixture
+def packings(monkeypatch):
+    """A list that grows by one entry for every matrix that is packed outside a product."""
+    from deltacnn_b200 import channel_ops
+    calls, quantize = [], channel_ops._quantize
+    monkeypatch.setattr(channel_ops, "_quantize", lambda *a: calls.append(a) or quantize(*a))
+    return calls
+
+
+def packed_layer(seed):
+    g = gen(seed)
+    layer = dc().DCMX4Linear(64, 48).cuda().half()
+    with torch.no_grad():
+        layer.weight.copy_(randn((48, 64), g))
+        layer.bias.copy_(randn((48,), g))
+    layer.process_filters()
+    return layer, randn((9, 64), g, F16)
+
+
+def load(layer):
+    layer.load_state_dict({k: torch.flip(v, (0,)) for k, v in layer.state_dict().items()})
+
+
+def optimizer_step(layer):
+    for p in layer.parameters():
+        p.grad = torch.ones_like(p)
+    torch.optim.SGD(layer.parameters(), lr=1.0).step()
+
+
+def new_data(layer):
+    layer.weight.data = torch.flip(layer.weight.data, (0,))
+
+
+def new_parameter(layer):
+    layer.weight = torch.nn.Parameter(torch.flip(layer.weight.detach(), (0,)))
+
+
+def in_place(layer):
+    with torch.no_grad():
+        layer.weight.mul_(-2)
+
+
+def coarser_and_back(layer):
+    layer.bfloat16().half()                 # eleven bits become eight: other values at what may be the old address
+
+
+@pytest.mark.parametrize("change", [load, optimizer_step, new_data, new_parameter, in_place, coarser_and_back])
+def test_a_packed_layer_answers_with_the_weight_it_has(change, packings):
+    layer, x = packed_layer(1)
+    with torch.no_grad():
+        before = layer(x)
+        assert len(packings) == 1, "a packed layer packs its weight once"
+        change(layer)
+        want = dc().mx4_linear(x, layer.weight, layer.bias)
+        assert not torch.equal(want, before)
+        assert torch.equal(layer(x), want)
+        layer.process_filters()
+        count = len(packings)
+        assert torch.equal(layer(x), want) and len(packings) == count
+
+
+def test_a_packed_layer_moves_and_copies(packings):
+    layer, x = packed_layer(2)
+    with torch.no_grad():
+        want = layer(x)
+        twin = copy.deepcopy(layer)
+        count = len(packings)
+        assert torch.equal(twin(x), want) and len(packings) == count        # a copy keeps what it has packed
+        twin.weight.neg_()
+        assert torch.equal(twin(x), dc().mx4_linear(x, twin.weight, twin.bias)) and torch.equal(layer(x), want)
+        layer.cpu().cuda()
+        assert torch.equal(layer(x), want)
+
+
+def test_a_packed_layer_trains():
+    """Packing does not take a layer out of training: input without a gradient (a first layer), frozen weights before an input
+    that needs one, and both."""
+    layer, x = packed_layer(3)
+    dy = randn((9, 48), gen(4), F16)
+    for x_grad, w_grad, b_grad in ((False, True, True), (False, False, True), (True, False, False), (True, True, True)):
+        layer.weight.requires_grad_(w_grad), layer.bias.requires_grad_(b_grad)
+        inputs = x.clone().requires_grad_(x_grad)
+        leaves = [t for t in (inputs, layer.weight, layer.bias) if t.requires_grad]
+        y = layer(inputs)
+        assert y.requires_grad
+        want = torch.autograd.grad(dc().mx4_linear(inputs, layer.weight, layer.bias), leaves, dy)
+        assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+    layer.requires_grad_(False)
+    assert not layer(x).requires_grad
+
+
+def test_a_packed_layer_under_inference_mode(packings):
+    layer, x = packed_layer(5)
+    want = layer(x).detach()
+    count = len(packings)
+    with torch.inference_mode():
+        assert torch.equal(layer(x), want)
+        born = dc().DCMX4Linear(64, 48).cuda().half()                           # its tensors keep no version
+        born.weight.copy_(layer.weight), born.bias.copy_(layer.bias)
+        born.process_filters()
+        count += 1
+        assert torch.equal(born(x), want)
+    assert len(packings) == count
+    with torch.no_grad():
+        square = dc().DCMX4Linear(48, 48).cuda().half()
+        square.process_filters()
+        square.weight.data = square.weight.data.t()                             # the same memory, other strides: not the packed matrix
+        with pytest.raises(RuntimeError, match="contiguous"):
+            square(x[:, :48].contiguous())
