@@ -329,12 +329,20 @@ def mx4_matmul(a, b, bias=None, dtype=torch.float16, out=None):
     return out
 
 
-def _unrows(out, x):
-    """A (rows, n) result in the shape of x with n channels."""
-    if x.dim() == 4:
-        n, _, h, w = x.shape
-        return out.view(n, h, w, out.shape[1]).permute(0, 3, 1, 2)
-    return out.view(*x.shape[:-1], out.shape[1]) if x.dim() != 2 else out
+def _empty(like, shape, dtype):
+    """A new tensor of rows: a 4-D one is a channels-last map. No view of another: what an autograd function returns has to be its
+    own tensor, or nothing may write to it in place."""
+    if len(shape) == 4:
+        return torch.empty(shape, dtype=dtype, device=like.device, memory_format=torch.channels_last)
+    return like.new_empty(shape, dtype=dtype)
+
+
+def _result(x, rows, c):
+    """A new tensor of x's type and shape with c channels."""
+    if x.dim() == 2:
+        return x.new_empty((rows, c))
+    shape = x.shape
+    return _empty(x, (shape[0], c, *shape[2:]) if len(shape) == 4 else (*shape[:-1], c), x.dtype)
 
 
 class _MX4Linear(torch.autograd.Function):
@@ -348,7 +356,7 @@ class _MX4Linear(torch.autograd.Function):
         need_x, need_w, _ = ctx.needs_input_grad
         ctx.sizes = rows, cols, outs
         ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        out = x.new_empty((rows, outs))
+        out = _result(x, rows, outs)
         ctx.kept, ctx.at = None, (None, None)
         if rows > 0:
             # the packed x^T and w^T that the backward pass reads, in one piece
@@ -360,7 +368,7 @@ class _MX4Linear(torch.autograd.Function):
             ws = x.new_empty(nbytes, dtype=torch.uint8)
             _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), *ctx.at, rows, outs, cols,
                     _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype], ws.data_ptr(), nbytes)
-        return _unrows(out, x)
+        return out
 
     @staticmethod
     def backward(ctx, dy):
@@ -378,20 +386,14 @@ class _MX4Linear(torch.autograd.Function):
         dy = _like_rows(dy, dy)
         db = dy.new_empty(outs, dtype=ctx.dtypes[2]) if need_b else None
         if rows == 0:
-            dx = dy.new_zeros(ctx.x_shape, dtype=ctx.dtypes[0]) if need_x else None
+            dx = _empty(dy, ctx.x_shape, ctx.dtypes[0]) if need_x else None
             return dx, dy.new_zeros((outs, cols), dtype=ctx.dtypes[1]) if need_w else None, None if db is None else db.zero_()
-        dx = dy.new_empty((rows, cols), dtype=ctx.dtypes[0]) if need_x else None
+        dx = _empty(dy, ctx.x_shape, ctx.dtypes[0]) if need_x else None
         dw = dy.new_empty((outs, cols), dtype=ctx.dtypes[1]) if need_w else None
         nbytes = _bytes_wanted("dc_mx4_linear_backward_workspace_bytes", dy.get_device(), rows, outs, cols)
         ws = dy.new_empty(nbytes, dtype=torch.uint8)
         _launch("mx4_linear_backward", lib.dc_mx4_linear_backward, dy, dy.data_ptr(), *ctx.at, _ptr(dx), _ptr(dw), _ptr(db), rows, outs, cols, _CODES[dy.dtype],
                 _CODES[ctx.dtypes[1]], 0 if db is None else _CODES[db.dtype], ws.data_ptr(), nbytes)
-        if need_x:
-            if len(ctx.x_shape) == 4:
-                n, _, h, w = ctx.x_shape
-                dx = dx.view(n, h, w, cols).permute(0, 3, 1, 2)
-            elif len(ctx.x_shape) != 2:
-                dx = dx.view(ctx.x_shape)
         return dx, dw, db
 
 
@@ -419,10 +421,10 @@ def mx4_linear(x, weight, bias=None):
         if grad:
             return _MX4Linear.apply(x, weight, bias)
         weight = _quantize(weight, outs, cols, False)[0]
-    out = x.new_empty((rows, outs))
+    out = _result(x, rows, outs)
     if rows > 0 and outs > 0:
         nbytes = _bytes_wanted("dc_mx4_linear_workspace_bytes", x.get_device(), rows, outs, cols)
         ws = x.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
         _launch(op, lib.dc_mx4_linear, x, x.data_ptr(), *weight._ptrs(), _ptr(bias), out.data_ptr(), rows, outs, cols, code,
                 0 if bias is None else _CODES[bias.dtype], _ptr(ws), nbytes)
-    return _unrows(out, x)
+    return out

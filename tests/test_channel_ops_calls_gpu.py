@@ -27,6 +27,10 @@ def randn(shape, g, dtype=F32, scale=1.0, shift=0.0):
     return (torch.randn(shape, generator=g, device="cuda") * scale + shift).to(dtype)
 
 
+def channels_last(t):
+    return t.contiguous(memory_format=torch.channels_last)
+
+
 # ---- DCMX4Linear and its packed weight -------------------------------------------------------------------------
 
 @pytest.fixture
@@ -138,3 +142,38 @@ def test_a_packed_layer_under_inference_mode(packings):
         square.weight.data = square.weight.data.t()                             # the same memory, other strides: not the packed matrix
         with pytest.raises(RuntimeError, match="contiguous"):
             square(x[:, :48].contiguous())
+
+
+# ---- tensors of other dimensions --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("shape", [(96,), (6, 7, 96), (2, 3, 2, 5, 96), (3, 96, 5, 7), (1, 96, 1, 1), (5, 96, 1, 1)])
+def test_linear_of_other_dimensions(shape):
+    d, g = dc(), gen(50)
+    x = randn(shape, g, F16)
+    w, b = randn((40, 96), g, F16).requires_grad_(), randn((40,), g, F16).requires_grad_()
+    maps = len(shape) == 4
+    out_shape = (shape[0], 40, *shape[2:]) if maps else (*shape[:-1], 40)
+    dy = randn(out_shape, g, F16)                                               # maps: NCHW memory, brought into the layer's layout
+    rows = lambda t: t.permute(0, 2, 3, 1).reshape(-1, t.shape[1]) if maps else t.reshape(-1, t.shape[-1])      # noqa: E731
+    x = (channels_last(x) if maps else x).requires_grad_()
+    flat = rows(x.detach()).contiguous().requires_grad_()
+    y, want = d.mx4_linear(x, w, b), d.mx4_linear(flat, w, b)
+    assert y.shape == out_shape and torch.equal(rows(y), want)
+    assert not maps or y.is_contiguous(memory_format=torch.channels_last)
+    got = torch.autograd.grad(y, (x, w, b), dy, retain_graph=True)
+    ref = torch.autograd.grad(want, (flat, w, b), rows(dy).contiguous())
+    assert got[0].shape == shape and torch.equal(rows(got[0]), ref[0]) and torch.equal(got[1], ref[1]) and torch.equal(got[2], ref[2])
+    with torch.no_grad():
+        assert torch.equal(d.mx4_linear(x, d.mx4_quantize(w), b), y)
+        assert d.mx4_linear(x, d.mx4_quantize(w), b).stride() == y.stride()
+    y.relu_()                                                                   # as an activation in place does
+
+
+def test_linear_of_no_rows():
+    x, w, b = torch.empty((0, 5, 64), device="cuda", requires_grad=True), torch.randn((8, 64), device="cuda", requires_grad=True), torch.randn(8, device="cuda", requires_grad=True)
+    y = dc().mx4_linear(x, w, b)
+    assert y.shape == (0, 5, 8)
+    dx, dw, db = torch.autograd.grad(y.sum(), (x, w, b))
+    assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all() and dw.shape == w.shape
+    for t in torch.autograd.grad(dc().mx4_linear(torch.randn((3, 64), device="cuda"), w, b).sum(), (w, b)):
+        assert t.isfinite().all()
