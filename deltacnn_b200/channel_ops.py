@@ -10,7 +10,6 @@ copied to make it fit, except an incoming gradient, whose layout the caller cann
 import functools
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from ._lib import lib, check
@@ -82,6 +81,24 @@ def _ptr(t):
     return None if t is None else t.data_ptr()
 
 
+class _Once(torch.autograd.Function):
+    """The gradients of an operator that is differentiable once, tied to what they depend on (``of``): whoever asks for their own
+    gradients comes through here and is refused, instead of getting a sum without its second-order part."""
+
+    @staticmethod
+    def forward(ctx, op, count, *grads_and_of):
+        ctx.op = op
+        return grads_and_of[:count]
+
+    @staticmethod
+    def backward(ctx, *_):
+        _fail(ctx.op, "differentiable once: the gradients have no gradients")
+
+
+def _once(op, grads, *of):
+    return _Once.apply(op, len(grads), *grads, *of)
+
+
 # ---- layer norm ------------------------------------------------------------------------------------------------
 
 def _ln_params(x, c, code, weight, bias, op):
@@ -131,11 +148,15 @@ class _LayerNorm(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        return _LayerNorm._again(ctx, dy) if torch.is_grad_enabled() else _LayerNorm._backward(ctx, dy)
+        x, weight, stats = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return (*_LayerNorm._backward(ctx, dy, x, weight, stats), None)
+        with torch.no_grad():                                # create_graph
+            grads = _LayerNorm._backward(ctx, dy, x, weight, stats)
+        return (*_once("layer_norm", grads, dy, x, weight), None)
 
     @staticmethod
-    def _backward(ctx, dy):
-        x, weight, stats = ctx.saved_tensors
+    def _backward(ctx, dy, x, weight, stats):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         rows, c = ctx.sizes
         dy = _like_rows(dy, x)
@@ -148,19 +169,13 @@ class _LayerNorm(torch.autograd.Function):
         mean = stats.data_ptr()
         _launch("layer_norm_backward", lib.dc_layer_norm_backward, x, dy.data_ptr(), x.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw),
                 _ptr(db), rows, c, code, _CODES[wtype], ws.data_ptr(), nbytes)
-        return dx, dw, db, None
-
-    @staticmethod
-    @once_differentiable
-    def _again(ctx, dy):
-        # under create_graph: the gradients' own gradients raise instead of being wrong
-        return _LayerNorm._backward(ctx, dy)
+        return dx, dw, db
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the channels, statistics and arithmetic in float32. ``weight`` and
-    ``bias``: (C,) in x's type or float32, or None. Differentiable in x, weight and bias (once); the sums over rows are added
-    in a fixed order, so equal inputs give equal bits. No reference counterpart."""
+    ``bias``: (C,) in x's type or float32, or None. Differentiable in x, weight and bias, once: gradients of the gradients are
+    refused. The sums over rows are added in a fixed order, so equal inputs give equal bits. No reference counterpart."""
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
     rows, c = _rows(x, "layer_norm")
@@ -347,7 +362,8 @@ def _result(x, rows, c):
 
 class _MX4Linear(torch.autograd.Function):
     """y = Q(x) Q(w)^T + b; dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, db = sum dy: every operand is rounded along the axis that
-    its product sums over, the rounding's own gradient is taken as 1. What is kept for the backward pass is 4-bit."""
+    its product sums over, the rounding's own gradient is taken as 1. What is kept for the backward pass is 4-bit. The second
+    result is empty: dx depends on the weight and dw on x, and it keeps the way to both without keeping either."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -356,7 +372,8 @@ class _MX4Linear(torch.autograd.Function):
         need_x, need_w, _ = ctx.needs_input_grad
         ctx.sizes = rows, cols, outs
         ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        out = _result(x, rows, outs)
+        ctx.set_materialize_grads(False)
+        out, origin = _result(x, rows, outs), x.new_empty(0)
         ctx.kept, ctx.at = None, (None, None)
         if rows > 0:
             # the packed x^T and w^T that the backward pass reads, in one piece
@@ -368,16 +385,20 @@ class _MX4Linear(torch.autograd.Function):
             ws = x.new_empty(nbytes, dtype=torch.uint8)
             _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), *ctx.at, rows, outs, cols,
                     _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype], ws.data_ptr(), nbytes)
-        return out
+        ctx.save_for_backward(origin)
+        return out, origin
 
     @staticmethod
-    def backward(ctx, dy):
-        return _MX4Linear._again(ctx, dy) if torch.is_grad_enabled() else _MX4Linear._backward(ctx, dy)
-
-    @staticmethod
-    @once_differentiable
-    def _again(ctx, dy):
-        return _MX4Linear._backward(ctx, dy)
+    def backward(ctx, dy, _):
+        if dy is None:
+            return None, None, None
+        origin, = ctx.saved_tensors
+        if not torch.is_grad_enabled():
+            return _MX4Linear._backward(ctx, dy)
+        with torch.no_grad():                                # create_graph
+            grads = _MX4Linear._backward(ctx, dy)
+        need_x, need_w, _ = ctx.needs_input_grad
+        return _once("mx4_linear", grads, dy, origin if need_x and need_w else None)
 
     @staticmethod
     def _backward(ctx, dy):
@@ -419,7 +440,7 @@ def mx4_linear(x, weight, bias=None):
         if not weight.is_contiguous() or weight.device != x.device or weight.dtype not in _CODES or outs == 0:
             _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
         if grad:
-            return _MX4Linear.apply(x, weight, bias)
+            return _MX4Linear.apply(x, weight, bias)[0]
         weight = _quantize(weight, outs, cols, False)[0]
     out = _result(x, rows, outs)
     if rows > 0 and outs > 0:

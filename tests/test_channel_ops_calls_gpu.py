@@ -177,3 +177,49 @@ def test_linear_of_no_rows():
     assert dx.shape == x.shape and (dw == 0).all() and (db == 0).all() and dw.shape == w.shape
     for t in torch.autograd.grad(dc().mx4_linear(torch.randn((3, 64), device="cuda"), w, b).sum(), (w, b)):
         assert t.isfinite().all()
+
+
+# ---- what is not differentiated is refused ---------------------------------------------------------------------
+
+def once_only(kind, g):
+    """(function of x, x, what else it depends on) of an operator that is differentiable once."""
+    x = randn((8, 64), g).requires_grad_()
+    w, b = randn((64,), g).requires_grad_(), randn((64,), g).requires_grad_()
+    m, c = randn((32, 64), g).requires_grad_(), randn((32,), g).requires_grad_()
+    return {"norm": (lambda: dc().layer_norm(x, w, b), x, (w, b)), "bare norm": (lambda: dc().layer_norm(x), x, ()),
+            "linear": (lambda: dc().mx4_linear(x, m, c), x, (m, c)), "frozen linear": (lambda: dc().mx4_linear(x, m.detach()), x, ()),
+            "behind another": (lambda: dc().mx4_linear(dc().layer_norm(x * 2, w, b), m), x, (w, b, m))}[kind]
+
+
+@pytest.mark.parametrize("through_dy", [False, True])
+@pytest.mark.parametrize("kind", ["norm", "bare norm", "linear", "frozen linear", "behind another"])
+def test_a_gradient_penalty_is_refused(kind, through_dy):
+    """total = loss + |d loss / d x|^2 has a second-order term that these operators do not give: every way to ask for it raises."""
+    f, x, others = once_only(kind, gen(10))
+
+    def total():
+        y = f()
+        loss = y.square().sum() if through_dy else y.sum()
+        g, = torch.autograd.grad(loss, x, create_graph=True)
+        return loss + g.square().sum()
+
+    if kind == "frozen linear" and not through_dy:          # its gradient depends on nothing that wants one: no second-order term
+        assert torch.equal(torch.autograd.grad(total(), x)[0], torch.autograd.grad(f().sum(), x)[0])
+        return
+    for ask in (lambda t: torch.autograd.grad(t, x), lambda t: t.backward(), lambda t: torch.autograd.grad(t, (x, *others), allow_unused=True)):
+        t = total()
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            ask(t)
+
+
+@pytest.mark.parametrize("kind", ["norm", "linear"])
+def test_first_gradients_under_create_graph(kind):
+    f, x, others = once_only(kind, gen(11))
+    leaves = (x, *others)
+    dy = randn(f().shape, gen(12))
+    want = torch.autograd.grad(f(), leaves, dy)
+    got = torch.autograd.grad(f(), leaves, dy, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(p.requires_grad for p in got)
+    for p in got:                                  # each of them knows that it depends on x
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(p.sum(), x, retain_graph=True)
