@@ -5,11 +5,13 @@ A tensor is seen as rows x channels: a 4-D tensor is a feature map (N, C, H, W) 
 any other tensor is (..., C), contiguous, one row per token. Types are float32, float16 and bfloat16 (the delta form: those of
 the delta path, float32 and float16). As everywhere in this package there is no CPU path, a wrong device, type or
 memory format raises before a launch, and launches go to torch's current stream on the tensor's device; an argument is never
-copied to make it fit, except an incoming gradient, whose layout the caller cannot choose.
+copied to make it fit, except an incoming gradient, whose layout the caller cannot choose. Gradients are those of a backward pass,
+once; forward-mode tangents are refused.
 """
 import functools
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import lib, check
@@ -42,6 +44,15 @@ def _bytes_wanted(query, index, *sizes):
 
 def _fail(op, text):
     raise RuntimeError(f"deltacnn_b200.{op}: {text}")
+
+
+def _no_tangent(op, *tensors):
+    """A dual tensor does not ask for a gradient: without this its tangent would be dropped and read as a derivative of zero."""
+    if _forward_ad._current_level < 0:
+        return
+    for t in tensors:
+        if t is not None and _forward_ad.unpack_dual(t).tangent is not None:
+            _fail(op, "there is no forward-mode derivative")
 
 
 def _code(t, op, name):
@@ -176,6 +187,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the channels, statistics and arithmetic in float32. ``weight`` and
     ``bias``: (C,) in x's type or float32, or None. Differentiable in x, weight and bias, once: gradients of the gradients are
     refused. The sums over rows are added in a fixed order, so equal inputs give equal bits. No reference counterpart."""
+    _no_tangent("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)
     rows, c = _rows(x, "layer_norm")
@@ -190,6 +202,7 @@ def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, thr
     ``delta`` and ``out_mask`` may be ``mask``; new tensors where None. At most 8192 channels. Returns (out, out_mask). No
     reference counterpart."""
     op = "layer_norm_delta"
+    _no_tangent(op, delta, prev_in, prev_out, weight, bias)
     _check_feature(delta, "delta")
     if delta.dtype not in (torch.float32, torch.float16):
         _fail(op, f"unsupported dtype {delta.dtype} (float32 and float16 only)")
@@ -289,6 +302,7 @@ def mx4_quantize(x):
     """x packed along its channels: an ``MX4Tensor`` of rows x channels. Blocks of 32 values share the scale
     2^(floor(log2 max|v|) - 2); values are rounded to the nearest of +-{0, 1/2, 1, 3/2, 2, 3, 4, 6} times the scale (ties to
     even, saturating); a block with an infinity or a NaN becomes NaN. No gradient, no reference counterpart."""
+    _no_tangent("mx4_quantize", x)
     rows, cols = _rows(x, "mx4_quantize")
     return _quantize(x, rows, cols, False)[0]
 
@@ -296,6 +310,7 @@ def mx4_quantize(x):
 def mx4_quantize_both(x):
     """(packed x, packed x^T) from one read of x; the second is cols x rows with blocks along x's columns (what the products
     of a backward pass contract over)."""
+    _no_tangent("mx4_quantize_both", x)
     rows, cols = _rows(x, "mx4_quantize_both")
     if rows == 0:
         _fail("mx4_quantize_both", "x has no rows")
@@ -325,6 +340,7 @@ def mx4_matmul(a, b, bias=None, dtype=torch.float16, out=None):
     """``a @ b.T + bias`` of two packed matrices (m x k and n x k, a weight in nn.Linear's layout): products and sums in float32,
     one rounding to ``dtype``. ``bias``: (n,) or None. ``out``: a contiguous (m, n) tensor to write to."""
     op = "mx4_matmul"
+    _no_tangent(op, bias)
     (m, k), (n, k2) = a.shape, b.shape
     if k != k2:
         _fail(op, f"the matrices have {k} and {k2} columns")
@@ -426,6 +442,7 @@ def mx4_linear(x, weight, bias=None):
     rows, cols = _rows(x, op)
     code = _code(x, op, "x")
     packed = isinstance(weight, MX4Tensor)
+    _no_tangent(op, x, None if packed else weight, bias)
     outs, k = weight.shape
     if k != cols:
         _fail(op, f"x has {cols} channels, the weight {k} columns")

@@ -937,6 +937,7 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
         if self.first_iter:
             K._check_feature(val, "input")
             K._dtype(val)
+            C._no_tangent("layer_norm_delta", val, self.weight, self.bias)
             self.first_iter = False
             if self not in DCThreshold.t:
                 DCThreshold.set(self, self.delta_threshold)

@@ -223,3 +223,27 @@ def test_first_gradients_under_create_graph(kind):
     for p in got:                                  # each of them knows that it depends on x
         with pytest.raises(RuntimeError, match="differentiable once"):
             torch.autograd.grad(p.sum(), x, retain_graph=True)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A tangent that nothing carries on would read as a derivative of zero."""
+    import torch.autograd.forward_ad as fwd
+    d, g = dc(), gen(13)
+    x, w, m, c = randn((6, 64), g), randn((64,), g), randn((32, 64), g), randn((32,), g)
+    q = d.mx4_quantize(m)
+    cl = channels_last(randn((1, 64, 4, 4), g))
+    mask = torch.ones((1, 1, 4, 4), dtype=torch.int32, device="cuda")
+    with fwd.dual_level():
+        dual = lambda t: fwd.make_dual(t, torch.ones_like(t))      # noqa: E731
+        calls = [lambda: d.layer_norm(dual(x)), lambda: d.layer_norm(x, dual(w)), lambda: d.layer_norm(x, w, dual(w)),
+                 lambda: d.layer_norm(dual(x.clone().requires_grad_()), w),
+                 lambda: d.mx4_linear(dual(x), m), lambda: d.mx4_linear(x, dual(m)), lambda: d.mx4_linear(x, q, dual(c)), lambda: d.mx4_linear(dual(x), q),
+                 lambda: d.mx4_quantize(dual(x)), lambda: d.mx4_quantize_both(dual(x)), lambda: d.mx4_matmul(d.mx4_quantize(x), q, dual(c)),
+                 lambda: d.layer_norm_delta(dual(cl), mask, cl.clone(), cl.clone()), lambda: d.layer_norm_delta(cl, mask, cl.clone(), cl.clone(), dual(w)),
+                 lambda: d.DCLayerNorm(64).cuda()((dual(cl), mask))]
+        for i, call in enumerate(calls):
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                call()
+                pytest.fail(f"call {i} was not refused")
+        inside = d.mx4_linear(d.layer_norm(x, w), m, c)             # nothing dual about it
+    assert torch.equal(inside, d.mx4_linear(d.layer_norm(x, w), m, c))
