@@ -170,6 +170,8 @@ class _LayerNorm(torch.autograd.Function):
     def _backward(ctx, dy, x, weight, stats):
         need_x, need_w, need_b, _ = ctx.needs_input_grad
         rows, c = ctx.sizes
+        # saved-tensor hooks may bring x back in another layout (offloading to pinned memory loses that of a map)
+        x = _like_rows(x, x)
         dy = _like_rows(dy, x)
         code, wtype = _CODES[x.dtype], ctx.wtype
         dx = torch.empty_like(x) if need_x else None

@@ -247,3 +247,35 @@ def test_forward_mode_tangents_are_refused():
                 pytest.fail(f"call {i} was not refused")
         inside = d.mx4_linear(d.layer_norm(x, w), m, c)             # nothing dual about it
     assert torch.equal(inside, d.mx4_linear(d.layer_norm(x, w), m, c))
+
+
+# ---- saved tensors ---------------------------------------------------------------------------------------------
+
+def map_step(g):
+    """A map's norm and linear layer with their gradients."""
+    x, w, b = channels_last(randn((2, 32, 5, 7), g)).requires_grad_(), randn((32,), g).requires_grad_(), randn((32,), g).requires_grad_()
+    m = randn((24, 32), g).requires_grad_()
+
+    def run():
+        y = dc().mx4_linear(dc().layer_norm(x, w, b), m)
+        return (y, *torch.autograd.grad(y.square().sum(), (x, w, b, m)))
+    return run
+
+
+def in_other_memory(t):
+    """The same values where offloading may leave them: another layout, another address."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    return flat[1:].view(t.shape).copy_(t.detach())
+
+
+def test_saved_tensors_may_be_moved():
+    run = map_step(gen(20))
+    want = run()
+    for hooks in (torch.autograd.graph.saved_tensors_hooks(in_other_memory, lambda t: t), torch.autograd.graph.save_on_cpu(),
+                  torch.autograd.graph.save_on_cpu(pin_memory=True)):
+        with hooks:
+            got = run()
+        # other addresses, so other widths of access and another order of float32 sums: of 70 rows or 32 channels of values of order
+        # one, a few hundred in dx's and dw's own sums
+        for p, q in zip(got, want):
+            assert (p - q).abs().max() <= 2.0 ** -24 * 200 * q.abs().max()
