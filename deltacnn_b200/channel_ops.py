@@ -392,34 +392,40 @@ class _MX4Linear(torch.autograd.Function):
         ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
         ctx.set_materialize_grads(False)
         out, origin = _result(x, rows, outs), x.new_empty(0)
-        ctx.kept, ctx.at = None, (None, None)
+        kept = None
         if rows > 0:
             # the packed x^T and w^T that the backward pass reads, in one piece
             x_bytes, w_bytes = _packed_bytes(cols, rows) if need_w else 0, _packed_bytes(cols, outs) if need_x else 0
-            ctx.kept = x.new_empty(x_bytes + w_bytes, dtype=torch.uint8)
-            at = ctx.kept.data_ptr()
-            ctx.at = at if need_w else None, at + x_bytes if need_x else None
+            kept = x.new_empty(x_bytes + w_bytes, dtype=torch.uint8)
             nbytes = _packed_bytes(rows, cols) + _packed_bytes(outs, cols)
             ws = x.new_empty(nbytes, dtype=torch.uint8)
-            _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), *ctx.at, rows, outs, cols,
-                    _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype], ws.data_ptr(), nbytes)
-        ctx.save_for_backward(origin)
+            _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), *_MX4Linear._at(ctx, kept), rows, outs,
+                    cols, _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype], ws.data_ptr(), nbytes)
+        ctx.save_for_backward(kept, origin)
         return out, origin
+
+    @staticmethod
+    def _at(ctx, kept):
+        """Where the packed x^T and w^T stand (None: not wanted)."""
+        need_x, need_w, _ = ctx.needs_input_grad
+        rows, cols, _ = ctx.sizes
+        at = kept.data_ptr()
+        return at if need_w else None, at + (_packed_bytes(cols, rows) if need_w else 0) if need_x else None
 
     @staticmethod
     def backward(ctx, dy, _):
         if dy is None:
             return None, None, None
-        origin, = ctx.saved_tensors
+        kept, origin = ctx.saved_tensors
         if not torch.is_grad_enabled():
-            return _MX4Linear._backward(ctx, dy)
+            return _MX4Linear._backward(ctx, dy, kept)
         with torch.no_grad():                                # create_graph
-            grads = _MX4Linear._backward(ctx, dy)
+            grads = _MX4Linear._backward(ctx, dy, kept)
         need_x, need_w, _ = ctx.needs_input_grad
         return _once("mx4_linear", grads, dy, origin if need_x and need_w else None)
 
     @staticmethod
-    def _backward(ctx, dy):
+    def _backward(ctx, dy, kept):
         need_x, need_w, need_b = ctx.needs_input_grad
         rows, cols, outs = ctx.sizes
         dy = _like_rows(dy, dy)
@@ -427,11 +433,13 @@ class _MX4Linear(torch.autograd.Function):
         if rows == 0:
             dx = _empty(dy, ctx.x_shape, ctx.dtypes[0]) if need_x else None
             return dx, dy.new_zeros((outs, cols), dtype=ctx.dtypes[1]) if need_w else None, None if db is None else db.zero_()
+        if kept.data_ptr() % 16:
+            kept = kept.clone()                              # saved-tensor hooks may bring it back at any address
         dx = _empty(dy, ctx.x_shape, ctx.dtypes[0]) if need_x else None
         dw = dy.new_empty((outs, cols), dtype=ctx.dtypes[1]) if need_w else None
         nbytes = _bytes_wanted("dc_mx4_linear_backward_workspace_bytes", dy.get_device(), rows, outs, cols)
         ws = dy.new_empty(nbytes, dtype=torch.uint8)
-        _launch("mx4_linear_backward", lib.dc_mx4_linear_backward, dy, dy.data_ptr(), *ctx.at, _ptr(dx), _ptr(dw), _ptr(db), rows, outs, cols, _CODES[dy.dtype],
+        _launch("mx4_linear_backward", lib.dc_mx4_linear_backward, dy, dy.data_ptr(), *_MX4Linear._at(ctx, kept), _ptr(dx), _ptr(dw), _ptr(db), rows, outs, cols, _CODES[dy.dtype],
                 _CODES[ctx.dtypes[1]], 0 if db is None else _CODES[db.dtype], ws.data_ptr(), nbytes)
         return dx, dw, db
 

@@ -279,3 +279,31 @@ def test_saved_tensors_may_be_moved():
         # one, a few hundred in dx's and dw's own sums
         for p, q in zip(got, want):
             assert (p - q).abs().max() <= 2.0 ** -24 * 200 * q.abs().max()
+
+
+def test_what_the_linear_layer_keeps_is_seen_and_freed():
+    g = gen(21)
+    x, w = randn((300, 256), g).requires_grad_(), randn((128, 256), g).requires_grad_()
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.numel() * t.element_size()) or t, lambda t: t):
+        y = dc().mx4_linear(x, w)
+    packed = sum(r * -(-c // 32) * 16 + -(-r // 128) * -(-c // 128) * 512 for r, c in ((256, 300), (256, 128)))
+    assert packed in seen
+    y = dc().mx4_linear(x, w)
+    before = torch.cuda.memory_allocated()
+    y.sum().backward(inputs=[x])
+    assert torch.cuda.memory_allocated() <= before + 300 * 256 * 4 - packed + 4096          # x.grad came, the packed matrices went
+    with pytest.raises(RuntimeError, match="second time"):
+        y.sum().backward(inputs=[x])
+
+
+def test_checkpointed_block():
+    from torch.utils.checkpoint import checkpoint
+    g = gen(22)
+    x, w, b, m = (randn(s, g).requires_grad_() for s in ((40, 64), (64,), (64,), (64, 64)))
+
+    def block(v):
+        return dc().mx4_linear(dc().layer_norm(v, w, b), m)
+    want = torch.autograd.grad(block(block(x)).square().sum(), (x, w, b, m))
+    got = torch.autograd.grad(checkpoint(block, checkpoint(block, x, use_reentrant=False), use_reentrant=False).square().sum(), (x, w, b, m))
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
