@@ -1010,6 +1010,8 @@ static LnShape ln_shape(int c, int64_t rows, int elem_bytes, int access, int war
 }
 
 // CTAs of a kernel that an SM holds; the grid is sized by it, so that every CTA's rows, and its one read of the parameters, start at once.
+// The first query of a kernel and CTA size also raises the kernel's limit of dynamic shared memory, whatever this launch needs of it:
+// without that a launch gets 48 KB together with the kernel's static memory, and the rings of some widths are 48 KB by themselves.
 template <auto KERNEL>
 static int resident_ctas(int threads, size_t smem) {
     static int known[64][33] = {};
@@ -1018,9 +1020,12 @@ static int resident_ctas(int threads, size_t smem) {
     int& n = known[dev][threads / 32];
     if (n == 0) {
         int v = 0;
-        if (smem > 48 * 1024) (void)cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem);
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, KERNEL, threads, smem) != cudaSuccess) (void)cudaGetLastError();
-        n = v > 0 ? v : 1;
+        if ((smem > 0 && cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, kLongSmem) != cudaSuccess) ||
+            cudaOccupancyMaxActiveBlocksPerMultiprocessor(&v, KERNEL, threads, smem) != cudaSuccess || v < 1) {
+            (void)cudaGetLastError();
+            return 1;          // not remembered: the launch tells what is wrong, the next call asks again
+        }
+        n = v;
     }
     return n;
 }

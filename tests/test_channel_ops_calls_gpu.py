@@ -4,6 +4,8 @@ gradients, forward-mode tangents, saved-tensor hooks, skip connections, tensors 
 Where values are compared, both sides are the same kernels on the same inputs (equal bits), or whole numbers whose sums
 float32 holds exactly, or the tolerance is derived beside the comparison."""
 import copy
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -307,3 +309,34 @@ def test_checkpointed_block():
     want = torch.autograd.grad(block(block(x)).square().sum(), (x, w, b, m))
     got = torch.autograd.grad(checkpoint(block, checkpoint(block, x, use_reentrant=False), use_reentrant=False).square().sum(), (x, w, b, m))
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+# ---- widths ----------------------------------------------------------------------------------------------------
+
+FRESH = """
+import torch, deltacnn_b200 as dc
+torch.manual_seed(0)
+t = torch.{dtype}
+x, dy = torch.randn(5, {c}, device="cuda").to(t), torch.randn(5, {c}, device="cuda").to(t)
+w, b = torch.randn({c}, device="cuda").to(t), torch.randn({c}, device="cuda").to(t)
+x64, w64 = x.double(), w.double()
+n = (x64 - x64.mean(-1, keepdim=True)) / (x64.var(-1, unbiased=False, keepdim=True) + 1e-5).sqrt()
+u = torch.finfo(t).eps / 2
+y64 = n * w64 + b.double()
+# one rounding at the end, and 64 steps of float32 in sums of values of order ten at most
+assert ((dc.layer_norm(x, w, b) - y64).abs() <= u * y64.abs() + 64 * 2.0 ** -24 * 10).all()
+if {train}:
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    dx, dw, db = torch.autograd.grad(dc.layer_norm(*leaves), leaves, dy)
+    db64 = dy.double().sum(0)
+    assert ((db - db64).abs() <= u * db64.abs() + 64 * 2.0 ** -24 * 10).all() and dx.isfinite().all() and dw.isfinite().all()
+torch.cuda.synchronize()
+"""
+
+
+@pytest.mark.parametrize("dtype,c,train", [("float16", 6000, False), ("bfloat16", 5640, False), ("float32", 2900, False), ("float16", 2600, True),
+                                           ("bfloat16", 3000, True), ("float32", 1500, True), ("float32", 1284, True)])
+def test_a_width_is_taken_whatever_ran_before(dtype, c, train):
+    """Rows whose ring fills 48 KB of shared memory exactly, as the first call of a process: no wider row has asked for more yet."""
+    run = subprocess.run([sys.executable, "-c", FRESH.format(dtype=dtype, c=c, train=train)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stderr[-1500:]
