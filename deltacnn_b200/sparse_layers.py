@@ -913,11 +913,13 @@ class DCLinear(nn.Linear, DCModule):
 class DCLayerNorm(nn.LayerNorm, DCModule):
     """Layer norm over the channels of a feature map. On a (delta, mask) pair it keeps the accumulated input and what it has
     handed on so far, and hands on the change of the norm where any channel's change is above ``delta_threshold`` (the same
-    truncation as ``DCActivation``, mask cleared in place); the first frame is normalised as a whole. A dense tensor
-    (N, C, H, W channels-last, or (..., C)) is normalised by the same arithmetic and has gradients. No reference counterpart
-    (the reference's only norm is DCBatchNorm2d, src/deltacnn/sparse_layers.py:1516-1585)."""
+    truncation as ``DCActivation``); the first frame is normalised as a whole. The result stands in buffers of the layer's own, which
+    the next frame overwrites (as a convolution's), so that a skip connection may read the input again; ``inplace=True`` writes it
+    over the input and clears the input's mask. A dense tensor (N, C, H, W channels-last, or (..., C)) is normalised by the same
+    arithmetic and has gradients. No reference counterpart (the reference's only norm is DCBatchNorm2d,
+    src/deltacnn/sparse_layers.py:1516-1585)."""
 
-    def __init__(self, num_features, eps=1e-5, elementwise_affine=True, bias=True, delta_threshold=None, name="", inplace=True):
+    def __init__(self, num_features, eps=1e-5, elementwise_affine=True, bias=True, delta_threshold=None, name="", inplace=False):
         nn.LayerNorm.__init__(self, num_features, eps=eps, elementwise_affine=elementwise_affine, bias=bias)
         if len(self.normalized_shape) != 1:
             raise RuntimeError("DCLayerNorm normalises over the channels: num_features must be one number")
@@ -927,6 +929,8 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
         self.first_iter = True
         self.prev_in = None
         self.prev_out = None
+        self._out = None
+        self._out_mask = None
 
     def forward(self, input):
         if type(input) != tuple:
@@ -945,21 +949,32 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
             self.prev_out = C.layer_norm(self.prev_in, weight, bias, self.eps)
             DCModule.temp_buffers.append(self.prev_in)
             DCModule.temp_buffers.append(self.prev_out)
-            return self.prev_out.clone(), mask
-        if not self.inplace:
-            val = val.clone()
-            mask = mask.clone()
-        mask_before = mask.clone() if K.DCPerformanceMetricsManager.enabled else None
-        C.layer_norm_delta(val, mask, self.prev_in, self.prev_out, weight, bias, DCThreshold.get(self), self.eps, out=val, out_mask=mask)
-        if mask_before is not None:
-            K.DCPerformanceMetricsManager.add_activation(mask_before, val.shape[1], DCTruncation.max.value, mask)
-        return val, mask
+            first = self.prev_out.clone()
+            if not self.inplace:
+                self._out = first
+            return first, mask
+        if self.inplace:
+            out, out_mask = val, mask
+        else:
+            reuse = DCConv2d.reuse_buffers
+            if self._out is None or self._out.shape != val.shape or not reuse:
+                self._out = torch.empty_like(val)
+            if self._out_mask is None or self._out_mask.shape != mask.shape or not reuse:
+                self._out_mask = torch.empty_like(mask)
+            out, out_mask = self._out, self._out_mask
+        mask_before = mask.clone() if K.DCPerformanceMetricsManager.enabled and self.inplace else mask
+        C.layer_norm_delta(val, mask, self.prev_in, self.prev_out, weight, bias, DCThreshold.get(self), self.eps, out=out, out_mask=out_mask)
+        if K.DCPerformanceMetricsManager.enabled:
+            K.DCPerformanceMetricsManager.add_activation(mask_before, val.shape[1], DCTruncation.max.value, out_mask)
+        return out, out_mask
 
     def reset(self):
         DCModule.reset(self)
         self.first_iter = True
         self.prev_in = None
         self.prev_out = None
+        self._out = None
+        self._out_mask = None
 
 
 class DCMX4Linear(nn.Linear, DCModule):

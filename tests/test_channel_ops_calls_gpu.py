@@ -340,3 +340,115 @@ def test_a_width_is_taken_whatever_ran_before(dtype, c, train):
     """Rows whose ring fills 48 KB of shared memory exactly, as the first call of a process: no wider row has asked for more yet."""
     run = subprocess.run([sys.executable, "-c", FRESH.format(dtype=dtype, c=c, train=train)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stderr[-1500:]
+
+
+# ---- the delta norm in a network -------------------------------------------------------------------------------
+
+def frames(g, dtype, n=4, shape=(2, 24, 9, 7)):
+    frame = channels_last(randn(shape, g, dtype))
+    for t in range(n):
+        yield frame
+        frame = frame.clone(memory_format=torch.preserve_format)
+        frame[:, :, t:t + 3, 1:4] += randn((*shape[:2], 3, 3), g, dtype)
+
+
+def norm_layer(g, dtype, channels=24, **args):
+    ln = dc().DCLayerNorm(channels, delta_threshold=0.0, **args).cuda().to(dtype)
+    with torch.no_grad():
+        ln.weight.copy_(randn((channels,), g, dtype, 0.2, 1.0))
+        ln.bias.copy_(randn((channels,), g, dtype))
+    return ln
+
+
+@pytest.mark.parametrize("dtype", [F32, F16])
+def test_delta_norm_beside_a_skip_connection(dtype):
+    """x + norm(x), the norm's usual place, over some frames against the dense block."""
+    d, g = dc(), gen(30)
+    sp, ln, add, de = d.DCSparsify(delta_threshold=0.0), norm_layer(g, dtype), d.DCAdd(), d.DCDensify()
+    with torch.no_grad():
+        for t, frame in enumerate(frames(g, dtype)):
+            x = sp(frame.clone(memory_format=torch.preserve_format))
+            held = [v.clone() for v in x]
+            y = ln(x)
+            for p, q in zip(x, held):                                           # bits: what lies at pixels without a mask may be a NaN
+                whole = {2: torch.int16, 4: torch.int32}[p.element_size()]
+                assert torch.equal(p.view(whole), q.view(whole)), "the norm wrote to its input"
+            got = de(add(x, y))
+            want = frame.double() + d.layer_norm(frame, ln.weight, ln.bias, EPS).double()
+            # a frame rounds the two inputs' sums, the norm, its change, the add and the sum of adds: six values below 16
+            assert (got.double() - want).abs().max().item() <= 6 * (t + 1) * 16 * torch.finfo(dtype).eps / 2
+
+
+def test_delta_norm_behind_a_convolution():
+    """The convolution's own output buffer is read again by a skip behind the norm. Weights of one power of two per output: exact."""
+    d, g = dc(), gen(31)
+    conv = d.DCConv2d(24, 24, 1, bias=False).cuda().half()
+    with torch.no_grad():
+        conv.weight.copy_(torch.eye(24, device="cuda").flip(0)[:, :, None, None] * 0.5)
+    model = torch.nn.ModuleList([conv])
+    conv.to(memory_format=torch.channels_last)
+    for c in model:
+        c.process_filters()
+    sp, ln, add, de = d.DCSparsify(delta_threshold=0.0), norm_layer(g, F16), d.DCAdd(), d.DCDensify()
+    with torch.no_grad():
+        for t, frame in enumerate(frames(g, F16)):
+            x = conv(sp(frame.clone(memory_format=torch.preserve_format)))
+            got = de(add(x, ln(x)))
+            dense = channels_last(frame.flip(1) * 0.5)
+            want = dense.double() + d.layer_norm(dense, ln.weight, ln.bias, EPS).double()
+            assert (got.double() - want).abs().max().item() <= 6 * (t + 1) * 16 * torch.finfo(F16).eps / 2
+
+
+@pytest.mark.parametrize("reuse", [False, True])
+def test_delta_norm_in_place_and_in_buffers_of_its_own(reuse, monkeypatch):
+    d = dc()
+    monkeypatch.setattr(d.DCConv2d, "reuse_buffers", reuse)
+    a, b = norm_layer(gen(32), F16), norm_layer(gen(32), F16, inplace=True)
+    sp, outs = d.DCSparsify(delta_threshold=0.0), []
+    with torch.no_grad():
+        for t, frame in enumerate(frames(gen(33), F16)):
+            val, mask = (v.clone() for v in sp(frame.clone(memory_format=torch.preserve_format)))
+            out, out_mask = a((val, mask))
+            outs.append(out.data_ptr())
+            mine, mine_mask = b((val, mask))
+            assert t == 0 or (mine is val and mine_mask is mask)
+            on = (out_mask != 0).expand_as(out)
+            assert torch.equal(out_mask, mine_mask) and torch.equal(out[on], mine[on])
+            assert torch.equal(a.prev_in, b.prev_in) and torch.equal(a.prev_out, b.prev_out)
+            if t == 0 or not reuse:
+                kept = out, out_mask                        # still referenced: a new tensor cannot stand where it does
+    assert (len(set(outs)) == 1) if reuse else (outs[-1] != outs[-2])
+    with pytest.raises(RuntimeError, match="reset_layers"):
+        a((channels_last(torch.zeros((3, 24, 9, 7), dtype=F16, device="cuda")), torch.ones((3, 1, 9, 7), dtype=torch.int32, device="cuda")))
+    a.reset()
+    val = channels_last(randn((3, 24, 4, 4), gen(34), F16))
+    with torch.no_grad():
+        assert torch.equal(a((val, torch.ones((3, 1, 4, 4), dtype=torch.int32, device="cuda")))[0], d.layer_norm(val, a.weight, a.bias, EPS))
+
+
+def test_delta_norm_replayed_from_a_graph():
+    d, g = dc(), gen(35)
+    sp, ln, add, de = d.DCSparsify(delta_threshold=0.0), norm_layer(g, F16), d.DCAdd(), d.DCDensify()
+    sequence = list(frames(g, F16, 6))
+    static = sequence[0].clone(memory_format=torch.preserve_format)
+
+    def block():
+        x = sp(static)
+        return de(add(x, ln(x)))
+
+    with torch.no_grad():
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            for frame in sequence[:2]:
+                static.copy_(frame)
+                block()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = block()
+        for t, frame in enumerate(sequence[2:], 2):
+            static.copy_(frame)
+            graph.replay()
+            want = frame.double() + d.layer_norm(frame, ln.weight, ln.bias, EPS).double()
+            assert (out.double() - want).abs().max().item() <= 6 * (t + 1) * 16 * torch.finfo(F16).eps / 2
