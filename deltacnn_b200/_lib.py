@@ -82,6 +82,7 @@ _SIGNATURES = {
     "dc_layer_norm_backward_workspace_bytes": (c_size_t, [c_i64, c_int, c_int]),
     "dc_layer_norm_backward": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_i64, c_int, c_int, c_int, _P, c_size_t, _P]),
     "dc_layer_norm_delta": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, c_i64, c_int, c_int, c_int, c_float, c_float, _P]),
+    "dc_layer_norm_delta_first": (c_int, [_P, _P, _P, _P, c_i64, c_int, c_int, c_int, c_float, _P]),
     "dc_mx4_data_bytes": (c_size_t, [c_i64, c_i64]),
     "dc_mx4_scale_bytes": (c_size_t, [c_i64, c_i64]),
     "dc_mx4_colsum_workspace_bytes": (c_size_t, [c_i64, c_i64]),

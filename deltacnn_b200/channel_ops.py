@@ -196,26 +196,42 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     return _ln_forward(x, rows, c, weight, bias, eps, False)[0]
 
 
+def _delta_map(x, name, weight, bias, op):
+    """(pixels, channels, type code, weight's type code) of a feature map in the delta path."""
+    _no_tangent(op, x, weight, bias)
+    _check_feature(x, name)
+    if x.dtype not in (torch.float32, torch.float16):
+        _fail(op, f"unsupported dtype {x.dtype} (float32 and float16 only)")
+    n, c, h, w = x.shape
+    if c == 0:
+        _fail(op, f"{name} has no channels")
+    code = _CODES[x.dtype]
+    return n * h * w, c, code, _ln_params(x, c, code, weight, bias, op)
+
+
+def _layer_norm_delta_first(x, weight, bias, eps):
+    """The norm of a whole first frame as ``prev_out`` of the delta form: bit for bit what ``layer_norm_delta`` computes for a pixel that
+    does not change afterwards (``layer_norm`` may add a row's sums in another order)."""
+    op = "layer_norm_delta"
+    pixels, c, code, wcode = _delta_map(x, "x", weight, bias, op)
+    y = torch.empty_like(x)
+    _launch(op, lib.dc_layer_norm_delta_first, x, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), pixels, c, code, wcode, eps)
+    return y
+
+
 def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, threshold=0.0, eps=1e-5, out=None, out_mask=None):
     """Layer norm over the channels of a (delta, mask) pair with its caches (no gradient): on masked pixels
     ``prev_in += delta`` and ``e = layer_norm(prev_in) - prev_out``; where any ``|e| > threshold`` the pixel stays in the mask,
     ``out = e`` and ``prev_out += e``; elsewhere the out-mask is 0 and ``out`` and ``prev_out`` keep what they hold.
     ``prev_in``: the accumulated input, ``prev_out``: the sum of what was handed on, both updated in place. ``out`` may be
-    ``delta`` and ``out_mask`` may be ``mask``; new tensors where None. At most 8192 channels. Returns (out, out_mask). No
-    reference counterpart."""
+    ``delta`` and ``out_mask`` may be ``mask``; new tensors where None. Before the first frame both caches are zeros, and the frame
+    itself is the delta, every pixel masked. At most 8192 channels. Returns (out, out_mask). No reference counterpart."""
     op = "layer_norm_delta"
-    _no_tangent(op, delta, prev_in, prev_out, weight, bias)
-    _check_feature(delta, "delta")
-    if delta.dtype not in (torch.float32, torch.float16):
-        _fail(op, f"unsupported dtype {delta.dtype} (float32 and float16 only)")
+    _no_tangent(op, prev_in, prev_out)
+    pixels, c, code, wcode = _delta_map(delta, "delta", weight, bias, op)
     _check_mask(mask, delta, "mask")
     _check_like(prev_in, delta, "prev_in")
     _check_like(prev_out, delta, "prev_out")
-    n, c, h, w = delta.shape
-    if c == 0:
-        _fail(op, "delta has no channels")
-    code = _CODES[delta.dtype]
-    wcode = _ln_params(delta, c, code, weight, bias, op)
     if out is None:
         out = torch.empty_like(delta)
     else:
@@ -231,7 +247,7 @@ def layer_norm_delta(delta, mask, prev_in, prev_out, weight=None, bias=None, thr
         if delta.numel() > 0:
             _fail(op, "delta, prev_in and prev_out must be three tensors, and out none of the caches")
     _launch(op, lib.dc_layer_norm_delta, delta, delta.data_ptr(), mask.data_ptr(), prev_in.data_ptr(), prev_out.data_ptr(), _ptr(weight), _ptr(bias),
-            out.data_ptr(), out_mask.data_ptr(), n * h * w, c, code, wcode, float(threshold), eps)
+            out.data_ptr(), out_mask.data_ptr(), pixels, c, code, wcode, float(threshold), eps)
     return out, out_mask
 
 

@@ -879,7 +879,8 @@ __device__ __forceinline__ bool ln_delta_pixel(const LnDeltaParams& p, const Tea
         bb.from(b[k]);
 #pragma unroll
         for (int i = 0; i < N; ++i) x[k].v[i] = fma(mul(x[k].v[i], rr), ww.v[i], bb.v[i]);
-        x[k].to(d[k]);               // the norm is rounded to the storage type first, then the difference: e = 0 exactly where nothing changed
+        x[k].to(d[k]);               // the norm is rounded to the storage type first, then the difference: e = 0 exactly where nothing changed since this
+                                   // kernel, or dc_layer_norm_delta_first with the same split of the row, wrote prev_out
         frag_sub(d[k], o[k]);
         hit |= frag_any_above(d[k], p.thr);
     }
@@ -1197,6 +1198,7 @@ static int ln_access(std::initializer_list<const void*> arrays, const void* weig
 static int bwd_cta_packs(int elem_bytes) { return elem_bytes == 2 ? 2 : 4; }
 constexpr int kLnMaxC = 1 << 30;          // a row's places are 32-bit
 constexpr int kFwdWarpPacks = 4, kBwdWarpPacks = 2, kDeltaWarpPacks = 4;
+static LnShape ln_delta_shape(int c, int dtype, int access) { return ln_shape(c, 0, ln_elem(dtype), access, kDeltaWarpPacks, 4); }
 
 }  // namespace dc
 
@@ -1253,6 +1255,20 @@ int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, co
     return col_reduce(partial, (int)t.slices, c, 2 * (int64_t)c, dweight, dbias, weight_dtype, st);
 }
 
+// The row is split as below: a pixel that does not change afterwards has the same norm bit for bit. dc_layer_norm's own split may be
+// another, since it looks at the number of rows too.
+int dc_layer_norm_delta_first(const void* x, const void* weight, const void* bias, void* prev_out, int64_t npix, int32_t c, int32_t dtype,
+                              int32_t weight_dtype, float eps, void* stream) {
+    if (x == nullptr || prev_out == nullptr) return DC_ERR_NULL_POINTER;
+    if (npix < 0 || c <= 0 || c > kLnMaxC) return DC_ERR_SHAPE;
+    if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;
+    if (npix == 0) return DC_OK;
+    const LnShape s = ln_delta_shape(c, dtype, ln_access({x, prev_out}, weight, bias));
+    if (s.p == 0) return DC_ERR_UNSUPPORTED;
+    LnParams p{x, weight, bias, prev_out, nullptr, nullptr, npix, c, c / s.w, s.g, eps, 1.f / (float)c};
+    DC_LN_TYPES(ln_forward_t, s, p, (cudaStream_t)stream)
+}
+
 int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, void* prev_out, const void* weight, const void* bias,
                         void* out, int32_t* mask_out, int64_t npix, int32_t c, int32_t dtype, int32_t weight_dtype, float threshold,
                         float eps, void* stream) {
@@ -1261,7 +1277,7 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
     if (npix < 0 || c <= 0 || c > kLnMaxC) return DC_ERR_SHAPE;
     if (dtype == DC_BF16 || !ln_dtypes_ok(dtype, weight_dtype)) return DC_ERR_DTYPE;      // the caches are those of the delta path
     if (npix == 0) return DC_OK;
-    const LnShape s = ln_shape(c, 0, ln_elem(dtype), ln_access({delta, prev_in, prev_out, out}, weight, bias), kDeltaWarpPacks, 4);
+    const LnShape s = ln_delta_shape(c, dtype, ln_access({delta, prev_in, prev_out, out}, weight, bias));
     if (s.p == 0) return DC_ERR_UNSUPPORTED;      // more channels than the registers of a CTA hold
     const float thr = dtype == DC_F16 ? host_round_threshold<__half>(threshold) : threshold;
     LnDeltaParams p{delta, weight, bias, mask, prev_in, prev_out, out, mask_out, npix, c, c / s.w, s.g, thr, eps, 1.f / (float)c, 32};

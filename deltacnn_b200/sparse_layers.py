@@ -936,17 +936,13 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
         if type(input) != tuple:
             return C.layer_norm(input, self.weight, self.bias, self.eps)
         val, mask = input
-        weight = None if self.weight is None else self.weight.detach()
-        bias = None if self.bias is None else self.bias.detach()
         if self.first_iter:
-            K._check_feature(val, "input")
-            K._dtype(val)
-            C._no_tangent("layer_norm_delta", val, self.weight, self.bias)
+            whole = val.clone()
+            self.prev_out = C._layer_norm_delta_first(whole, self.weight, self.bias, self.eps)
+            self.prev_in = whole.detach()
             self.first_iter = False
             if self not in DCThreshold.t:
                 DCThreshold.set(self, self.delta_threshold)
-            self.prev_in = val.detach().clone()
-            self.prev_out = C.layer_norm(self.prev_in, weight, bias, self.eps)
             DCModule.temp_buffers.append(self.prev_in)
             DCModule.temp_buffers.append(self.prev_out)
             first = self.prev_out.clone()
@@ -963,7 +959,7 @@ class DCLayerNorm(nn.LayerNorm, DCModule):
                 self._out_mask = torch.empty_like(mask)
             out, out_mask = self._out, self._out_mask
         mask_before = mask.clone() if K.DCPerformanceMetricsManager.enabled and self.inplace else mask
-        C.layer_norm_delta(val, mask, self.prev_in, self.prev_out, weight, bias, DCThreshold.get(self), self.eps, out=out, out_mask=out_mask)
+        C.layer_norm_delta(val, mask, self.prev_in, self.prev_out, self.weight, self.bias, DCThreshold.get(self), self.eps, out=out, out_mask=out_mask)
         if K.DCPerformanceMetricsManager.enabled:
             K.DCPerformanceMetricsManager.add_activation(mask_before, val.shape[1], DCTruncation.max.value, out_mask)
         return out, out_mask

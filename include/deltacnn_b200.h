@@ -353,6 +353,12 @@ int dc_layer_norm_delta(const void* delta, const int32_t* mask, void* prev_in, v
                         void* out, int32_t* mask_out, int64_t npix, int32_t c, int32_t dtype, int32_t weight_dtype, float threshold,
                         float eps, void* stream);
 
+/* The norm of a whole first frame x, for prev_out before the calls above (prev_in = x): the sums are added in dc_layer_norm_delta's
+ * order (that of arrays at 16-byte addresses, where x and prev_out are), so that at threshold 0 a pixel that has not changed leaves the
+ * mask. dc_layer_norm's order also depends on the number of rows. */
+int dc_layer_norm_delta_first(const void* x, const void* weight, const void* bias, void* prev_out, int64_t npix, int32_t c, int32_t dtype,
+                              int32_t weight_dtype, float eps, void* stream);
+
 /* ---- MXFP4: quantisation and products ----------------------------------------------------------------------
  * No counterpart in the reference. A row of a matrix is cut into blocks of 32 values; a block is 32 e2m1 codes (+-{0, 1/2, 1,
  * 3/2, 2, 3, 4, 6}) under one scale 2^(s - 127). With E the biased float32 exponent of the block's largest magnitude,

@@ -452,3 +452,55 @@ def test_delta_norm_replayed_from_a_graph():
             graph.replay()
             want = frame.double() + d.layer_norm(frame, ln.weight, ln.bias, EPS).double()
             assert (out.double() - want).abs().max().item() <= 6 * (t + 1) * 16 * torch.finfo(F16).eps / 2
+
+
+@pytest.mark.parametrize("dtype,shape", [(F16, (8, 96, 160, 160)), (F32, (4, 101, 130, 160)), (F16, (4, 82, 130, 160)), (F16, (2, 1200, 9, 7)), (F32, (1, 2000, 9, 7))])
+def test_an_unchanged_pixel_leaves_the_mask(dtype, shape):
+    """At threshold 0 a masked pixel whose delta is 0 has no change, from the first frame on: the first frame's norm has to be the
+    delta form's own, bit for bit, on maps of many pixels too."""
+    g = gen(40)
+    ln = norm_layer(g, dtype, shape[1])
+    frame = channels_last(randn(shape, g, dtype, 1.5, 0.7))
+    ones = torch.ones((shape[0], 1, *shape[2:]), dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        first, mask = ln((frame, ones))
+        assert (mask == 1).all() and torch.equal(first, ln.prev_out)
+        first = first.clone()
+        _, mask = ln((torch.zeros_like(frame), ones.clone()))
+        assert int(mask.sum()) == 0
+        assert torch.equal(ln.prev_out, first) and torch.equal(ln.prev_in, frame)
+
+
+def test_first_frame_of_hard_values_and_refusals():
+    d, g = dc(), gen(41)
+    ln = norm_layer(g, F32)
+    frame = channels_last(randn((1, 24, 2, 3), g))
+    frame[0, 3, 0, 0], frame[0, 5, 1, 1], frame[0, :, 0, 2] = float("nan"), float("inf"), 2.0
+    ones = torch.ones((1, 1, 2, 3), dtype=torch.int32, device="cuda")
+    with torch.no_grad():
+        y = ln((frame, ones))[0]
+    assert y[0, :, 0, 0].isnan().all() and y[0, :, 1, 1].isnan().all() and torch.equal(y[0, :, 0, 2], ln.bias)
+    assert int(y.isnan().sum()) == 48
+    for bad in (torch.zeros((1, 24, 2, 3), device="cuda"), channels_last(torch.zeros((1, 24, 2, 3), device="cuda").bfloat16()),
+                channels_last(torch.zeros((1, 25, 2, 3), device="cuda"))):
+        with pytest.raises(RuntimeError):
+            norm_layer(g, F32)((bad, ones))
+    wide = norm_layer(g, F32, 9001)
+    with pytest.raises(RuntimeError):                                           # no delta kernel for so many channels: at once, not a frame later
+        wide((channels_last(torch.zeros((1, 9001, 1, 1), device="cuda")), torch.ones((1, 1, 1, 1), dtype=torch.int32, device="cuda")))
+    assert wide.first_iter and d.layer_norm(torch.zeros((2, 9001), device="cuda"), wide.weight, wide.bias).shape == (2, 9001)
+
+
+def test_a_first_frame_through_the_delta_call_itself():
+    """From caches of zeros, as the call documents: the same norm, and nothing changes behind it."""
+    d, g = dc(), gen(42)
+    x, w, b = channels_last(randn((2, 96, 40, 50), g, F16)), randn((96,), g, F16), randn((96,), g, F16)
+    ones = torch.ones((2, 1, 40, 50), dtype=torch.int32, device="cuda")
+    prev_in, prev_out = torch.zeros_like(x), torch.zeros_like(x)
+    out, mask = d.layer_norm_delta(x, ones, prev_in, prev_out, w, b)
+    ln = norm_layer(g, F16, 96)
+    with torch.no_grad():
+        ln.weight.copy_(w), ln.bias.copy_(b)
+        first = ln((x, ones))[0]
+    assert torch.equal(out, first) and torch.equal(prev_out, first) and torch.equal(prev_in, x) and int(mask.sum()) == mask.numel()
+    assert int(d.layer_norm_delta(torch.zeros_like(x), ones, prev_in, prev_out, w, b)[1].sum()) == 0
