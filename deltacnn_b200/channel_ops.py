@@ -20,13 +20,14 @@ from .cuda_kernels import _check_feature, _check_like, _check_mask
 _CODES = {torch.float32: _lib.DC_F32, torch.float16: _lib.DC_F16, torch.bfloat16: _lib.DC_BF16}
 
 
-_raw_stream = torch._C._cuda_getCurrentRawStream      # what torch.cuda.current_stream(i).cuda_stream gives, at a fortieth of the time
+# what torch.cuda.current_stream(i).cuda_stream and torch.cuda.current_device() give, at a fortieth and half of the time
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def _launch(op, fn, t, *args):
     """Calls a library entry point on t's device and that device's current stream."""
     index = t.get_device()
-    if index == torch.cuda.current_device():
+    if index == _current_device():
         status = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -394,69 +395,69 @@ def _result(x, rows, c):
     return _empty(x, (shape[0], c, *shape[2:]) if len(shape) == 4 else (*shape[:-1], c), x.dtype)
 
 
+@functools.lru_cache(maxsize=4096)
+def _train_bytes(rows, cols, outs):
+    """Bytes of the packed x^T and w^T that a backward pass reads, and of the packed x and w of the forward product."""
+    return _packed_bytes(cols, rows), _packed_bytes(cols, outs), _packed_bytes(rows, cols) + _packed_bytes(outs, cols)
+
+
 class _MX4Linear(torch.autograd.Function):
     """y = Q(x) Q(w)^T + b; dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, db = sum dy: every operand is rounded along the axis that
     its product sums over, the rounding's own gradient is taken as 1. What is kept for the backward pass is 4-bit. The second
     result is empty: dx depends on the weight and dw on x, and it keeps the way to both without keeping either."""
 
     @staticmethod
-    def forward(ctx, x, weight, bias):
-        rows, cols = _rows(x, "mx4_linear")
+    def forward(ctx, x, weight, bias, rows, cols):
         outs = weight.shape[0]
-        need_x, need_w, _ = ctx.needs_input_grad
-        ctx.sizes = rows, cols, outs
-        ctx.x_shape, ctx.dtypes = x.shape, (x.dtype, weight.dtype, None if bias is None else bias.dtype)
-        ctx.set_materialize_grads(False)
-        out, origin = _result(x, rows, outs), x.new_empty(0)
-        kept = None
+        need_x, need_w = ctx.needs_input_grad[:2]
+        out = _result(x, rows, outs)
+        codes = _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype]
+        kept, x_at, w_at = None, None, None
         if rows > 0:
             # the packed x^T and w^T that the backward pass reads, in one piece
-            x_bytes, w_bytes = _packed_bytes(cols, rows) if need_w else 0, _packed_bytes(cols, outs) if need_x else 0
+            x_bytes, w_bytes, nbytes = _train_bytes(rows, cols, outs)
+            x_bytes, w_bytes = x_bytes if need_w else 0, w_bytes if need_x else 0
+            x_at, w_at = 0 if need_w else None, x_bytes if need_x else None
             kept = x.new_empty(x_bytes + w_bytes, dtype=torch.uint8)
-            nbytes = _packed_bytes(rows, cols) + _packed_bytes(outs, cols)
             ws = x.new_empty(nbytes, dtype=torch.uint8)
-            _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), *_MX4Linear._at(ctx, kept), rows, outs,
-                    cols, _CODES[x.dtype], _CODES[weight.dtype], 0 if bias is None else _CODES[bias.dtype], ws.data_ptr(), nbytes)
+            at = kept.data_ptr()
+            _launch("mx4_linear", lib.dc_mx4_linear_train, x, x.data_ptr(), weight.data_ptr(), _ptr(bias), out.data_ptr(), at if need_w else None,
+                    at + x_bytes if need_x else None, rows, outs, cols, *codes, ws.data_ptr(), nbytes)
+        ctx.plan = rows, cols, outs, x.shape, x.dtype, weight.dtype, None if bias is None else bias.dtype, codes, x_at, w_at
+        origin = x.new_empty(0) if need_x and need_w else None
+        ctx.set_materialize_grads(False)
         ctx.save_for_backward(kept, origin)
         return out, origin
 
     @staticmethod
-    def _at(ctx, kept):
-        """Where the packed x^T and w^T stand (None: not wanted)."""
-        need_x, need_w, _ = ctx.needs_input_grad
-        rows, cols, _ = ctx.sizes
-        at = kept.data_ptr()
-        return at if need_w else None, at + (_packed_bytes(cols, rows) if need_w else 0) if need_x else None
-
-    @staticmethod
     def backward(ctx, dy, _):
         if dy is None:
-            return None, None, None
+            return None, None, None, None, None
         kept, origin = ctx.saved_tensors
         if not torch.is_grad_enabled():
-            return _MX4Linear._backward(ctx, dy, kept)
+            return (*_MX4Linear._backward(ctx, dy, kept), None, None)
         with torch.no_grad():                                # create_graph
             grads = _MX4Linear._backward(ctx, dy, kept)
-        need_x, need_w, _ = ctx.needs_input_grad
-        return _once("mx4_linear", grads, dy, origin if need_x and need_w else None)
+        return (*_once("mx4_linear", grads, dy, origin), None, None)
 
     @staticmethod
     def _backward(ctx, dy, kept):
-        need_x, need_w, need_b = ctx.needs_input_grad
-        rows, cols, outs = ctx.sizes
+        need_x, need_w, need_b, _, _ = ctx.needs_input_grad
+        rows, cols, outs, x_shape, x_dtype, w_dtype, b_dtype, codes, x_at, w_at = ctx.plan
         dy = _like_rows(dy, dy)
-        db = dy.new_empty(outs, dtype=ctx.dtypes[2]) if need_b else None
+        dx = _empty(dy, x_shape, x_dtype) if need_x else None
         if rows == 0:
-            dx = _empty(dy, ctx.x_shape, ctx.dtypes[0]) if need_x else None
-            return dx, dy.new_zeros((outs, cols), dtype=ctx.dtypes[1]) if need_w else None, None if db is None else db.zero_()
-        if kept.data_ptr() % 16:
+            return dx, dy.new_zeros((outs, cols), dtype=w_dtype) if need_w else None, dy.new_zeros(outs, dtype=b_dtype) if need_b else None
+        dw = dy.new_empty((outs, cols), dtype=w_dtype) if need_w else None
+        db = dy.new_empty(outs, dtype=b_dtype) if need_b else None
+        at = kept.data_ptr()
+        if at % 16:
             kept = kept.clone()                              # saved-tensor hooks may bring it back at any address
-        dx = _empty(dy, ctx.x_shape, ctx.dtypes[0]) if need_x else None
-        dw = dy.new_empty((outs, cols), dtype=ctx.dtypes[1]) if need_w else None
+            at = kept.data_ptr()
         nbytes = _bytes_wanted("dc_mx4_linear_backward_workspace_bytes", dy.get_device(), rows, outs, cols)
         ws = dy.new_empty(nbytes, dtype=torch.uint8)
-        _launch("mx4_linear_backward", lib.dc_mx4_linear_backward, dy, dy.data_ptr(), *_MX4Linear._at(ctx, kept), _ptr(dx), _ptr(dw), _ptr(db), rows, outs, cols, _CODES[dy.dtype],
-                _CODES[ctx.dtypes[1]], 0 if db is None else _CODES[db.dtype], ws.data_ptr(), nbytes)
+        _launch("mx4_linear_backward", lib.dc_mx4_linear_backward, dy, dy.data_ptr(), None if x_at is None else at + x_at, None if w_at is None else at + w_at,
+                _ptr(dx), _ptr(dw), _ptr(db), rows, outs, cols, *codes, ws.data_ptr(), nbytes)
         return dx, dw, db
 
 
@@ -483,7 +484,7 @@ def mx4_linear(x, weight, bias=None):
         if not weight.is_contiguous() or weight.device != x.device or weight.dtype not in _CODES or outs == 0:
             _fail(op, f"weight must be a contiguous (outputs, {cols}) tensor on {x.device}")
         if grad:
-            return _MX4Linear.apply(x, weight, bias)[0]
+            return _MX4Linear.apply(x, weight, bias, rows, cols)[0]
         weight = _quantize(weight, outs, cols, False)[0]
     out = _result(x, rows, outs)
     if rows > 0 and outs > 0:
