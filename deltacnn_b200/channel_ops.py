@@ -6,7 +6,8 @@ any other tensor is (..., C), contiguous, one row per token. Types are float32, 
 the delta path, float32 and float16). As everywhere in this package there is no CPU path, a wrong device, type or
 memory format raises before a launch, and launches go to torch's current stream on the tensor's device; an argument is never
 copied to make it fit, except an incoming gradient, whose layout the caller cannot choose. Gradients are those of a backward pass,
-once; forward-mode tangents are refused.
+once; forward-mode tangents are refused. Every wait inside a product is bounded: one that runs out makes ``lib.dc_umma_error()``
+non-zero (which synchronises), and leaves its tile of the result unwritten, or NaN where the tile is shared along k.
 """
 import functools
 

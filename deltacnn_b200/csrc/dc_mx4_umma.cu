@@ -214,6 +214,12 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
         const int quarter = warp & 3;
         int it = 0;
         [[maybe_unused]] uint32_t seq = 0;         // steps so far
+        // A wait that ran out: a tile that is shared along k becomes NaN in the columns of every rank, instead of a sum without
+        // this rank's share. (The accumulator of a failed copy or MMA never arrives, so that the draining warps come through here.)
+        [[maybe_unused]] auto spoil = [&] {
+            float* part = reinterpret_cast<float*>(raw + (ring - smem_u32(raw)));
+            for (int c = 0; c < NT; ++c) part[c * 128 + quarter * 32 + lane] = __uint_as_float(0x7fffffffu);
+        };
         for (int tile = blockIdx.x; tile < p.tiles; tile += gridDim.x, ++it) {
             const int a = it & 1, use = it >> 1;
             const int tf = tile % p.tiles_f, tt = tile / p.tiles_f;
@@ -255,12 +261,20 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
                         if (lane == 0) mbar_arrive(full(s));
                     }
                 }
-                if (!ok) break;
+                if (!ok) {
+                    if constexpr (SPLIT) if (warp < 6) spoil();
+                    break;
+                }
                 if (warp >= 6) continue;
             }
             const int f = tf * 128 + quarter * 32 + lane;
             const float bias = f < p.n && !SPLIT ? mx_bias(p, f) : 0.f;
-            if (!mbar_wait_warp(acc_full(a), (uint32_t)(use & 1), ok_flag)) { *ok_flag = 0; atomicExch(&g_mx4_error, 4); break; }
+            if (!mbar_wait_warp(acc_full(a), (uint32_t)(use & 1), ok_flag)) {
+                *ok_flag = 0;
+                atomicExch(&g_mx4_error, 4);
+                if constexpr (SPLIT) spoil();
+                break;
+            }
             tc_fence_after();
             const uint32_t src = tmem + a * NT + ((uint32_t)quarter << 21);
             const int64_t t0 = (int64_t)tt * NT;
@@ -291,10 +305,9 @@ __global__ void __launch_bounds__(QUANT ? kMxQuantThreads : kMxThreads, 1) k_mx4
         const int tile = blockIdx.x, tf = tile % p.tiles_f, tt = tile / p.tiles_f;
         const int64_t t0 = (int64_t)tt * NT;
         const int cols = (int)(p.m - t0 < NT ? p.m - t0 : NT);
-        const bool good = *ok_flag != 0;
         // four features at a time, every rank's share of them in flight together
         const int mine = 32 * ((cols - rank + ranks - 1) / ranks);
-        for (int i = threadIdx.x; i < mine && good; i += blockDim.x) {
+        for (int i = threadIdx.x; i < mine; i += blockDim.x) {
             const int col = rank + (i >> 5) * ranks, f = tf * 128 + (i & 31) * 4;
             float4 x[8];
 #pragma unroll

@@ -181,8 +181,8 @@ int dc_pack_filter_umma(const dc_conv_desc* desc, int32_t transposed, const void
                         void* filter_umma, void* stream);
 
 /* Sticky device-side error code of the tensor-core kernels on the current device: 0 = none,
- * otherwise the bounded wait that gave up (1 stage ring, 2 filter copy, 3 accumulator). The
- * call synchronises with the device. No reference counterpart. */
+ * otherwise the bounded wait that gave up (convolutions: 1 stage ring, 2 filter copy, 3 accumulator; the MXFP4 products use 1 to 9
+ * for their own). What the kernel still had to write is then left unwritten (MXFP4 tiles shared along k: NaN). The call synchronises with the device. No reference counterpart. */
 int dc_umma_error(void);
 
 /* Accumulate + activation delta + truncation, in place on delta, mask and both caches.
