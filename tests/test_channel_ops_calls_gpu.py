@@ -504,3 +504,114 @@ def test_a_first_frame_through_the_delta_call_itself():
         first = ln((x, ones))[0]
     assert torch.equal(out, first) and torch.equal(prev_out, first) and torch.equal(prev_in, x) and int(mask.sum()) == mask.numel()
     assert int(d.layer_norm_delta(torch.zeros_like(x), ones, prev_in, prev_out, w, b)[1].sum()) == 0
+
+
+# ---- tensors of many rows, of float32 weights, of more than 2^31 elements --------------------------------------
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,c", [(160001, 24), (80001, 96), (30000, 512), (20000, 101), (19001, 33), (20000, 25), (1500, 8), (16001, 1000), (4097, 2600),
+                                    (5001, 255), (4800, 129), (5000, 202), (700, 257), (2100, 5000), (1000, 9006), (450, 8200), (901, 12001), (333, 20000)])
+def test_no_row_is_missing_from_the_column_sums(rows, c, dtype):
+    """Odd whole numbers over mean 0 and rstd 1/2: every term is a multiple of 1/2, every sum below 2^24 of them, so float32 holds all of
+    them exactly in any order, and one row that is missing or counted twice changes every column."""
+    g = gen(rows)
+    odd = lambda: (torch.randint(0, 4, (rows, c), generator=g, device="cuda") * 2 - 3).to(dtype)      # noqa: E731  -3, -1, 1, 3
+    x, dy = odd(), odd()
+    mean, rstd = torch.zeros(rows, device="cuda"), torch.full((rows,), 0.5, device="cuda")
+    lib, code = dc()._lib.lib, {F32: 0, F16: 1, BF16: 2}[dtype]
+    dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    ws = torch.empty(lib.dc_layer_norm_backward_workspace_bytes(rows, c, code), dtype=torch.uint8, device="cuda")
+    dx = torch.empty_like(x)
+    for d in (dx.data_ptr(), None):
+        dw.fill_(-1), db.fill_(-1)
+        assert lib.dc_layer_norm_backward(dy.data_ptr(), x.data_ptr(), None, mean.data_ptr(), rstd.data_ptr(), d, dw.data_ptr(), db.data_ptr(), rows, c, code, 0,
+                                          ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(db.double(), dy.double().sum(0)) and torch.equal(dw.double(), (dy.double() * x.double() * 0.5).sum(0))
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("m,n,k", [(8200, 130, 64), (4100, 2051, 40), (129, 33, 96)])
+def test_no_row_is_missing_from_the_bias_gradient(m, n, k, dtype):
+    g = gen(m)
+    x, w, b = randn((m, k), g, dtype), randn((n, k), g, dtype), torch.zeros(n, device="cuda", requires_grad=True)
+    dy = (torch.randint(0, 4, (m, n), generator=g, device="cuda") * 2 - 3).to(dtype)
+    assert torch.equal(torch.autograd.grad(dc().mx4_linear(x, w, b), b, dy)[0].double(), dy.double().sum(0))
+
+
+@pytest.mark.parametrize("inplace", [False, True])
+def test_delta_norm_with_float32_weights_on_half_maps(inplace):
+    d, g = dc(), gen(51)
+    ln = d.DCLayerNorm(24, delta_threshold=0.0, inplace=inplace).cuda()
+    with torch.no_grad():
+        ln.weight.copy_(randn((24,), g, F32, 0.2, 1.0))
+        ln.bias.copy_(randn((24,), g))
+        sp, de = d.DCSparsify(delta_threshold=0.0), d.DCDensify()
+        for t, frame in enumerate(frames(g, F16)):
+            got = de(ln(sp(frame.clone(memory_format=torch.preserve_format))))
+            want = d.layer_norm(frame, ln.weight, ln.bias, EPS)
+            # per frame the accumulated input, the norm, its change and the accumulated output are rounded: four values below 16
+            assert (got.double() - want.double()).abs().max().item() <= 4 * (t + 1) * 16 * torch.finfo(F16).eps / 2
+
+
+# 4096 channels: 524288 rows are 2^31 elements
+LONG = 524288 + 515
+
+
+def test_layer_norm_of_more_than_2_31_elements():
+    d, g = dc(), gen(52)
+    x = torch.empty((LONG, 4096), dtype=BF16, device="cuda").normal_(generator=g).requires_grad_()
+    dy = torch.empty_like(x, requires_grad=False).random_(0, 4, generator=g).mul_(2).sub_(3)          # odd whole numbers: db is exact
+    w, b = randn((4096,), g).requires_grad_(), randn((4096,), g).requires_grad_()
+    y = d.layer_norm(x, w, b)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert torch.equal(db.double(), dy.sum(0, dtype=torch.float64)) and dw.isfinite().all()
+    for part in (slice(0, 515), slice(LONG // 2, LONG // 2 + 515), slice(LONG - 515, LONG)):
+        xs = x.detach()[part].clone().requires_grad_()
+        ys = d.layer_norm(xs, w, b)
+        assert torch.equal(ys, y[part])
+        assert torch.equal(torch.autograd.grad(ys, xs, dy[part])[0], dx[part])
+
+
+def test_delta_norm_of_more_than_2_31_elements():
+    d, g = dc(), gen(53)
+    shape = (8, 64, 2048, 2052)                                                 # 2^31 and 2^22 elements
+    delta = torch.empty(shape, dtype=F16, device="cuda", memory_format=torch.channels_last).normal_(generator=g)
+    prev_in = torch.zeros_like(delta)
+    prev_out = torch.zeros_like(delta)
+    mask = (torch.rand((8, 1, 2048, 2052), generator=g, device="cuda") < 0.3).int()
+    w, b = randn((64,), g, F16), randn((64,), g, F16)
+    part = [t[-1:, :, -3:].clone(memory_format=torch.channels_last) for t in (delta, prev_in, prev_out)]
+    small = d.layer_norm_delta(part[0], mask[-1:, :, -3:].clone(), part[1], part[2], w, b, 0.1)
+    out, out_mask = d.layer_norm_delta(delta, mask, prev_in, prev_out, w, b, 0.1, out=delta)
+    on = (small[1] != 0).expand_as(small[0])
+    assert torch.equal(out_mask[-1:, :, -3:], small[1]) and torch.equal(out[-1:, :, -3:][on], small[0][on])
+    assert torch.equal(prev_in[-1:, :, -3:], part[1]) and torch.equal(prev_out[-1:, :, -3:], part[2])
+    assert torch.equal(out_mask != 0, mask != 0)                                # from nothing every masked pixel changes
+
+
+def scale_rows(q, first):
+    """The scale bytes of the rows from `first`, a multiple of 128, on (those behind the last row are not written)."""
+    s = q.scales[first // 128:].permute(0, 3, 2, 1, 4)
+    return s.reshape(-1, s.shape[3] * 4)[:q.shape[0] - first]
+
+
+def test_mx4_of_more_than_2_31_elements():
+    d, g = dc(), gen(54)
+    x = torch.empty((LONG, 4096), dtype=BF16, device="cuda").normal_(generator=g)
+    q = d.mx4_quantize(x)
+    tail = LONG // 128 * 128 - 128
+    part = d.mx4_quantize(x[tail:])
+    assert torch.equal(q.data[tail:], part.data) and torch.equal(scale_rows(q, tail), scale_rows(part, 0))
+    both, both_t = d.mx4_quantize_both(x)
+    assert torch.equal(both.data, q.data) and torch.equal(scale_rows(both, 0), scale_rows(q, 0))
+    part_t = d.mx4_quantize_both(x[tail:])[1]
+    assert torch.equal(both_t.data[:, tail // 2:], part_t.data)
+    del both, both_t
+    assert torch.equal(d.mx4_dequantize(q, BF16)[tail:], d.mx4_dequantize(part, BF16))
+    del x
+    w = d.mx4_quantize(randn((8, 4096), g))
+    assert torch.equal(d.mx4_matmul(q, w, None, BF16)[tail:], d.mx4_matmul(part, w, None, BF16))
+    wide, few = d.mx4_quantize(randn((4100, 64), g)), d.mx4_quantize(randn((LONG, 64), g))
+    out = d.mx4_matmul(few, wide, None, BF16)                                   # more than 2^31 results
+    end = d.mx4_matmul(d.mx4_quantize(d.mx4_dequantize(few)[tail:]), wide, None, BF16)
+    assert torch.equal(out[tail:], end)
