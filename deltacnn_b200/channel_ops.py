@@ -190,7 +190,8 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
     """``(x - mean) / sqrt(var + eps) * weight + bias`` over the channels, statistics and arithmetic in float32. ``weight`` and
     ``bias``: (C,) in x's type or float32, or None. Differentiable in x, weight and bias, once: gradients of the gradients are
-    refused. The sums over rows are added in a fixed order, so equal inputs give equal bits. No reference counterpart."""
+    refused. Sums are added in an order that follows from the shape, the addresses' alignment (16 bytes, 4, less) and the GPU
+    (``DC_GRID_SHARE`` included): where these are equal, equal inputs give equal bits. No reference counterpart."""
     _no_tangent("layer_norm", x, weight, bias)
     if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad) or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps)

@@ -337,7 +337,8 @@ int dc_layer_norm(const void* x, const void* weight, const void* bias, void* y, 
  *   dx = rstd * (g - mean(g) - n * mean(g * n)),  dweight = sum_rows(dy * n),  dbias = sum_rows(dy).
  * dx, dweight, dbias may be NULL where not wanted. dx may be dy. workspace: dc_layer_norm_backward_workspace_bytes of device
  * memory, 16-byte aligned, only meaningful during the call (per-CTA partial sums of the column reductions, added in a fixed
- * order: the same inputs give the same bits; the means of long rows). May be NULL where only dx is wanted of rows of at most
+ * order; the means of long rows). How rows are split over threads, and with it the order of the sums, follows from rows, c, the
+ * addresses' alignment (16 bytes, 4, less) and the SMs in use (DC_GRID_SHARE): where these are equal, equal inputs give equal bits. May be NULL where only dx is wanted of rows of at most
  * 8192 elements. rows == 0 writes zeros to dweight and dbias. */
 size_t dc_layer_norm_backward_workspace_bytes(int64_t rows, int32_t c, int32_t dtype);
 int dc_layer_norm_backward(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd, void* dx,
