@@ -615,3 +615,20 @@ def test_mx4_of_more_than_2_31_elements():
     out = d.mx4_matmul(few, wide, None, BF16)                                   # more than 2^31 results
     end = d.mx4_matmul(d.mx4_quantize(d.mx4_dequantize(few)[tail:]), wide, None, BF16)
     assert torch.equal(out[tail:], end)
+
+
+def test_delta_norm_is_counted_the_same_in_place_or_not(monkeypatch):
+    from deltacnn_b200.cuda_kernels import DCPerformanceMetricsManager as M
+    counted = []
+    for inplace in (False, True):
+        ln, sp = norm_layer(gen(60), F16, inplace=inplace), dc().DCSparsify(delta_threshold=0.0)
+        M.reset()
+        with torch.no_grad():
+            for frame in frames(gen(61), F16):
+                val, mask = (v.clone() for v in sp(frame.clone(memory_format=torch.preserve_format)))
+                monkeypatch.setattr(M, "enabled", True)                         # the norm alone
+                ln((val, mask))
+                monkeypatch.setattr(M, "enabled", False)
+        counted.append(vars(M.get_metrics()))
+        M.reset()
+    assert counted[0] == counted[1] and counted[0]["mem_write_actual"] > 0
